@@ -257,6 +257,45 @@ int savit_attention_fwd(const void* qkv, void* o, float* lse, int B, int N, int 
 int savit_attention_bwd(const void* qkv, const void* o, const void* d_o, const float* lse, void* dqkv, int B, int N, int H,
                         int head_dim, int ld_qkv, float dq_scale, void* stream);
 
+/* ---- Position in attention: per-head normalisation with the rotation, and learned relative biases.
+ * savit_qk_norm_rope_fwd: rows of the packed buffer (H query heads, Hk key heads, Hk value heads of head_dim columns; Hk < H: shared key /
+ *   value heads), bf16 (is_bf16) or fp32, row pitches ld / ld_out in elements (16-byte multiples, 16-byte aligned bases).  Per head of the
+ *   queries and keys:  n = (x - center * mean x) / sqrt(mean (x - center * mean x)^2 + eps);  out = s * rotate(w * n), s = q_scale for queries
+ *   (the 1/sqrt(head_dim) that savit_attention_fwd expects on them), 1 for keys; values are copied, or left where they are when out == qkv.
+ *   wq, wk fp32 [head_dim], shared by the heads.  table fp32 [table_rows, head_dim] = cosines | sines of head_dim / 2 angles per position
+ *   (NULL: no rotation); pairs are (e, e + head_dim/2), or (2e, 2e+1) when interleaved; angle 0 leaves a pair alone (a class token, a partial
+ *   rotation).  positions int32 [rows] (NULL: row mod N); a position outside [0, table_rows) makes its row NaN.  head_dim % 16 == 0, <= 256.
+ * savit_qk_norm_rope_bwd: dqkv = cotangent of the output, qkv = the forward's INPUT; out receives the gradient of that input (value columns
+ *   copied; out == dqkv: in place, values left alone; out must not be qkv); dwq, dwk fp32 [head_dim] are ACCUMULATED, in a fixed order.
+ *   workspace: savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim). */
+int savit_qk_norm_rope_fwd(const void* qkv, long ld, const float* wq, const float* wk, const float* table, int table_rows, const int* positions,
+                           void* out, long ld_out, int rows, int N, int H, int Hk, int head_dim, int is_bf16, float eps, float q_scale, int center,
+                           int interleaved, void* stream);
+int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void* qkv, long ld, const float* wq, const float* wk, const float* table,
+                           int table_rows, const int* positions, void* out, long ld_out, float* dwq, float* dwk, int rows, int N, int H, int Hk,
+                           int head_dim, int is_bf16, float eps, float q_scale, int center, int interleaved, void* workspace, long workspace_bytes,
+                           void* stream);
+long savit_qk_norm_rope_bwd_workspace_bytes(int H, int Hk, int head_dim);
+/* savit_relpos_bias_fwd: bias[h, i, j] = table[index[i, j], h]; table fp32 [buckets, H], index int32 [N, N] (an entry outside [0, buckets) gives
+ *   NaN), bias fp32 [H, N, ld_bias], ld_bias % 4 == 0 (columns >= N are zeroed).  N <= 32 768.
+ * savit_relpos_bias_bwd: dtable[b, h] += sum of dbias[h, i, j] over the positions of bucket b, in a fixed order.  order int32 [N*N] = positions
+ *   i * N + j sorted by bucket, start int32 [buckets + 1] = where each bucket's list begins.  workspace: savit_relpos_bias_bwd_workspace_bytes. */
+int savit_relpos_bias_fwd(const float* table, const int* index, float* bias, int N, int H, int buckets, int ld_bias, void* stream);
+int savit_relpos_bias_bwd(const float* dbias, const int* order, const int* start, float* dtable, int N, int H, int buckets, int ld_bias, void* workspace,
+                          long workspace_bytes, void* stream);
+long savit_relpos_bias_bwd_workspace_bytes(int N, int H, int buckets);
+/* savit_bias_attention_fwd: savit_attention_fwd with S = q k^T + bias[h], bias fp32 [H, N, ld_bias] shared by the images (ld_bias % 4 == 0).
+ *   lens int32 [B] (NULL: all N): keys and queries at or beyond lens[b] (clamped to [0, N]) take no part; their rows of o are zero, their lse is
+ *   -inf - as those of a query whose bias masks every key.  A bias of -inf masks; so does float's or bfloat16's lowest value.  lse is required.
+ * savit_bias_attention_bwd: dqkv as in savit_attention_bwd (rows of padding are zero); dbias fp32 [H, N, ld_bias] (nullable) = the sum of dS over
+ *   the batch, in a fixed order.  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
+ *   head_dim 16, 32, 48 or 64; N <= 32 768, and one image's rows and one head's bias each below 4 GiB; d_o, o compact [B*N, H*head_dim]. */
+int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
+                             int ld_bias, void* stream);
+int savit_bias_attention_bwd(const void* qkv, const float* bias, const int* lens, const void* d_o, const float* lse, void* dqkv, float* dbias, int B, int N,
+                             int H, int head_dim, int ld_qkv, int ld_bias, float dq_scale, void* workspace, long workspace_bytes, void* stream);
+long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, int ld_bias, int want_dbias);
+
 /* Very short sequences (TNT's inner transformer, tnt.py:68-76: 16 pixel tokens, 4 heads padded to 16 columns): one wave per
  * sequence, scores / softmax / outputs in registers.  Same tensor layout and scaling conventions as savit_attention_fwd/bwd with
  * B = nseq, N = 16, H = 4, head_dim = 16, ld_qkv = 192 - the only geometry accepted (SAVIT_EINVAL otherwise; the tiled kernels
@@ -353,6 +392,22 @@ int savit_scatter_rows(const void* src_bf16, float* dst, void* dst_bf16, long ro
 int savit_softmax_xent(const float* logits, int ld_logits, const int* labels, const int* mix_labels, const float* ratio,
                        float label_smoothing, float grad_scale, float* loss_rows, float* loss_mean, void* dlogits_bf16,
                        int ld_dlogits, float* dbias, float* top1, float* top5, int B, int C, void* stream);
+
+/* ---- distillation from the K largest logits of a teacher, with the hard-label loss beside it.  Per row, q = softmax(logits / T):
+ *   P = softmax(teacher_logits / T) over the row's pairs (teacher_lse NULL), or exp(teacher_logits / T - teacher_lse) with the mass that is left
+ *   spread evenly over the classes that no pair names (teacher_lse [R] = log sum_j exp(t_j / T) over ALL classes)
+ *   loss = row_weight (distill_weight T^2 sum_j P_j (log P_j - log q_j) + hard_weight CE(logits, smoothed label))
+ *   dlogits = grad_scale * d loss / d logits
+ * logits fp32 or bf16 [R, ld], dlogits (nullable) fp32 or bf16 [R, ld_dlogits] - columns >= C are left alone; dlogits == logits is allowed with
+ * equal type and pitch; any alignment of the element type.  teacher_logits fp32, teacher_index int32, both [R, K] compact, K <= 512: an index
+ * outside [0, C) is no pair, one class named twice gets both probabilities; a row without pairs has no distillation term.  labels int32 [R]
+ * (nullable when hard_weight == 0): outside [0, C) drops the row's hard term.  row_weight fp32 [R] (nullable = 1): rows of weight 0 are not read,
+ * their loss and gradient are zero.  A -inf logit has q = 0; a row of nothing but -inf, or with +inf or NaN, is NaN.
+ * loss_rows fp32 [R] (nullable); dbias fp32 [C] (nullable) += column sums of dlogits as stored, in a fixed order. */
+int savit_distill_xent(const void* logits, long ld_logits, int logits_bf16, const float* teacher_logits, const int* teacher_index, int K,
+                       const float* teacher_lse, const int* labels, const float* row_weight, float temperature, float distill_weight, float hard_weight,
+                       float label_smoothing, float grad_scale, float* loss_rows, void* dlogits, long ld_dlogits, int dlogits_bf16, float* dbias, int R,
+                       int C, void* stream);
 
 /* ---- optimizer (train.py:25-27,100; simple_train.py:25-27): out[0] += sum(g^2); then one fused pass
  *   g' = g*grad_scale*clip ; m,v Adam moments ; p -= lr * ( mhat/(sqrt(vhat)+eps) + weight_decay*p )

@@ -1,0 +1,432 @@
+// Distillation from the largest logits of a teacher, with the hard-label loss beside it: loss and gradient in one pass over the student's
+// logits.  Per row, with q = softmax(z / T) and P_j the teacher's probability of class j:
+//   P from K (logit, class) pairs: softmax(t / T) over the pairs, or - given the teacher's log-sum-exp over ALL classes at temperature T -
+//     exp(t / T - lse) for the pairs and the mass that is left spread evenly over the classes no pair names
+//   loss = w_s T^2 sum_j P_j (log P_j - log q_j) + w_h CE(z, (1 - a) onehot(label) + a / C)
+//   dz_j = w_s T (S q_j - P_j) + w_h (softmax(z)_j - y_j),   S = sum_j P_j  (1, or 0 where no pair is usable)
+//
+// Bound by HBM: z is read once and dz written once.  The row stays in registers between the pass that finds the maximum and the sums and the pass
+// that writes the gradient (C 16-byte pieces a thread; what does not fit is read a second time), so there is one block reduction and no re-read.
+// A thread keeps the sums relative to its own maximum and the block joins (maximum, sum) pairs: one barrier instead of two.
+// Exponentials are v_exp_f32 on (z - max) * (log2 e / T), per-thread sums fp32; everything that exists once a row - the pairs, the
+// normalisers, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
+// The gradient is written for every class as if no pair named it, then the at most K + 1 classes with a pair or the label are written again.
+#include "common.h"
+#include "savit.h"
+
+namespace {
+
+constexpr int DS_MAX_K = 512;
+constexpr double LN2 = 0.69314718055994530942;
+
+struct DistillParams {
+  const void* z;
+  const float* top;     // [R, K] teacher logits
+  const int* at;        // [R, K] their classes; outside [0, C): no pair
+  const float* lse;     // [R] or nullptr
+  const int* labels;    // [R] or nullptr; outside [0, C): no hard term for the row
+  const float* weight;  // [R] or nullptr
+  float* loss_rows;     // [R] or nullptr
+  void* dz;             // or nullptr
+  long ldz, lddz;
+  int R, C, K;
+  float soft, hard, smooth, T, c_soft, c_hard, grad_scale;  // c_soft = log2 e / T, c_hard = log2 e
+};
+
+template <typename T>
+struct Piece;  // 16 bytes of a row
+template <>
+struct Piece<float> {
+  static constexpr int E = 4;
+  typedef f32x4 vec __attribute__((aligned(4)));
+  float v[4];
+  __device__ __forceinline__ void load(const float* p) {
+    const vec r = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[i];
+  }
+  __device__ __forceinline__ void load_part(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : -INFINITY;
+  }
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+};
+template <>
+struct Piece<bf16_t> {
+  static constexpr int E = 8;
+  typedef u32x4 vec __attribute__((aligned(2)));
+  uint32_t v[4];
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    const vec r = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[i];
+  }
+  __device__ __forceinline__ void load_part(const bf16_t* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = 2 * i < n ? p[2 * i] : 0xff80u, hi = 2 * i + 1 < n ? p[2 * i + 1] : 0xff80u;
+      v[i] = lo | (hi << 16);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float((i & 1) ? (v[i >> 1] & 0xffff0000u) : (v[i >> 1] << 16)); }
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+// n <= E results to consecutive columns
+template <int E>
+__device__ __forceinline__ void put_piece(float* p, const float (&v)[E], int n) {
+  typedef f32x4 vec __attribute__((aligned(4)));
+  if (n == E) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) *reinterpret_cast<vec*>(p + i) = vec{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) p[i] = v[i];
+  }
+}
+template <int E>
+__device__ __forceinline__ void put_piece(bf16_t* p, const float (&v)[E], int n) {
+  if (n == E) {
+    if constexpr (E == 8) {
+      typedef u32x4 vec __attribute__((aligned(2)));
+      *reinterpret_cast<vec*>(p) = vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    } else {
+      typedef u32x2 vec __attribute__((aligned(2)));
+      *reinterpret_cast<vec*>(p) = vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) p[i] = f32_to_bf16(v[i]);
+  }
+}
+
+// what a thread (a wave, the row) has seen: maximum, sums of exponentials relative to it at temperatures T and 1, sum of z.
+// The maximum starts at the lowest finite value: -inf then counts nothing, and a row of lowest values is uniform.
+struct Seen {
+  float m, s, h, z;
+};
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// W waves a row (4 / W rows a block where W < 4), C pieces of the row kept by a thread.
+template <typename TI, typename TO, int W, int C>
+__global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const DistillParams p) {
+  constexpr int TH = 64 * W, RPB = W < 4 ? 4 / W : 1, E = Piece<TI>::E;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ Seen part[RPB][W];
+  __shared__ double tpart[RPB][W][2], lpart[RPB][W][2];
+  __shared__ int distinct[RPB];
+  const int sub = RPB > 1 ? threadIdx.x / TH : 0;  // row of the block
+  const int tid = RPB > 1 ? threadIdx.x - sub * TH : threadIdx.x;
+  const int wave = tid >> 6;
+  const bool first_lane = (tid & 63) == 0;
+  const int row = blockIdx.x * RPB + sub;
+  const int K = p.K;
+  // LDS of a row: K pairs {P (first the logit / T), z at the class, class}
+  double* P = reinterpret_cast<double*>(smem) + (size_t)sub * K;
+  float* zt = reinterpret_cast<float*>(smem + (size_t)RPB * K * 8) + (size_t)sub * K;
+  int* at = reinterpret_cast<int*>(smem + (size_t)RPB * K * 12) + (size_t)sub * K;
+
+  const float weight = row < p.R ? (p.weight ? p.weight[row] : 1.0f) : 0.0f;
+  const bool live = weight != 0.0f;  // rows of weight 0 are not read
+  const TI* z = reinterpret_cast<const TI*>(p.z) + (size_t)row * p.ldz;
+  const int pieces = (p.C + E - 1) / E, full = p.C / E;  // the last piece may be a partial one
+  const int label = live && p.labels ? p.labels[row] : -1;
+  const bool has_label = p.hard != 0.0f && (unsigned)label < (unsigned)p.C;
+  const bool two = p.hard != 0.0f && p.c_hard != p.c_soft;  // a second sum of exponentials
+  const bool need_z = p.lse != nullptr || p.smooth != 0.0f;
+  auto fetch = [&](Piece<TI>& q, int i) {
+    if (i < full) q.load(z + (size_t)i * E);
+    else q.load_part(z + (size_t)i * E, p.C - i * E);
+  };
+
+  Piece<TI> r[C];
+  Seen me{-3.402823466e38f, 0.f, 0.f, 0.f};
+  double tm = -1.7976931348623157e308;
+  float zl = 0.f;
+  auto see = [&](const Piece<TI>& q, int i) {
+    float m = me.m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, q.get(e));
+    if (m != me.m) {
+      me.s *= __builtin_amdgcn_exp2f((me.m - m) * p.c_soft);
+      if (two) me.h *= __builtin_amdgcn_exp2f((me.m - m) * p.c_hard);
+      me.m = m;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) me.s += __builtin_amdgcn_exp2f((q.get(e) - m) * p.c_soft);
+    if (two) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) me.h += __builtin_amdgcn_exp2f((q.get(e) - m) * p.c_hard);
+    }
+    if (need_z) {
+      const int n = p.C - i * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < n) me.z += q.get(e);
+    }
+  };
+  if (live) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (tid + c * TH < pieces) fetch(r[c], tid + c * TH);
+    for (int k = tid; k < K; k += TH) {  // the pairs, while the row is on its way
+      const int j = p.at[(size_t)row * K + k];
+      const bool ok = (unsigned)j < (unsigned)p.C;
+      const double t = ok ? (double)p.top[(size_t)row * K + k] / (double)p.T : -__builtin_inf();
+      at[k] = ok ? j : -1;
+      zt[k] = ok ? to_float(z[j]) : 0.f;
+      P[k] = t;
+      tm = fmax(tm, t);
+    }
+    if (has_label) zl = to_float(z[label]);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (tid + c * TH < pieces) see(r[c], tid + c * TH);
+    for (int i = tid + C * TH; i < pieces; i += TH) {
+      Piece<TI> q;
+      fetch(q, i);
+      see(q, i);
+    }
+  }
+  if (tid == 0) distinct[sub] = 0;
+  {
+    const float M = wave_max(me.m);
+    const Seen w{M, wave_sum(me.s * __builtin_amdgcn_exp2f((me.m - M) * p.c_soft)),
+                 two ? wave_sum(me.h * __builtin_amdgcn_exp2f((me.m - M) * p.c_hard)) : 0.f, need_z ? wave_sum(me.z) : 0.f};
+    double ts = 0.0;
+    if (64 * wave < K) {
+      tm = wave_max_d(tm);
+      if (live)
+        for (int k = tid; k < K; k += TH) ts += exp(P[k] - tm);
+      ts = wave_sum_d(ts);
+    }
+    if (first_lane) {
+      part[sub][wave] = w;
+      tpart[sub][wave][0] = tm;
+      tpart[sub][wave][1] = ts;
+    }
+  }
+  __syncthreads();
+
+  // the row's maximum and normalisers, in every thread
+  float M = part[sub][0].m;
+  double TM = tpart[sub][0][0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    M = fmaxf(M, part[sub][w].m);
+    TM = fmax(TM, tpart[sub][w][0]);
+  }
+  double S = 0.0, H = 0.0, Z = 0.0, tsum = 0.0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const Seen o = part[sub][w];
+    S += (double)(o.s * __builtin_amdgcn_exp2f((o.m - M) * p.c_soft));
+    if (two) H += (double)(o.h * __builtin_amdgcn_exp2f((o.m - M) * p.c_hard));
+    Z += (double)o.z;
+    if (64 * w < K && tpart[sub][w][1] != 0.0) tsum += tpart[sub][w][1] * exp(tpart[sub][w][0] - TM);
+  }
+  if (!two) H = S;
+
+  // the teacher's probabilities; mass that is left over goes evenly to the classes that no pair names
+  double left = 0.0, share = 0.0, mass;
+  if (p.lse) {
+    const double lse = live ? (double)p.lse[row] : 0.0;
+    int mine = 0;
+    if (live)
+      for (int k = tid; k < K; k += TH) {
+        P[k] = exp(P[k] - lse);
+        bool first = at[k] >= 0;
+        for (int i = 0; first && i < k; ++i) first = at[i] != at[k];
+        mine += first;
+      }
+    if (mine) atomicAdd(&distinct[sub], mine);
+    __syncthreads();
+    const int others = p.C - distinct[sub];
+    mass = tsum == 0.0 ? 0.0 : tsum * exp(TM - lse);
+    if (others > 0) {
+      left = mass < 1.0 ? 1.0 - mass : (mass == mass ? 0.0 : mass);
+      share = left / others;
+    }
+    mass += left;
+  } else {
+    const double inv = tsum == 0.0 ? 0.0 : 1.0 / tsum;
+    if (live)
+      for (int k = tid; k < K; k += TH) P[k] = exp(P[k] - TM) * inv;
+    mass = tsum == 0.0 ? 0.0 : (tsum == tsum ? 1.0 : tsum);
+  }
+
+  const double gs = (double)p.grad_scale * weight;
+  const double hard = p.hard != 0.0f && has_label ? p.hard : 0.0;
+  const float a_soft = (float)(gs * p.soft * p.T * mass / S), a_hard = hard != 0.0 ? (float)(gs * hard / H) : 0.0f;
+  const float a_both = a_soft + a_hard;
+  const float base = (float)(gs * (p.soft * p.T * share + hard * p.smooth / p.C));
+  TO* dz = reinterpret_cast<TO*>(p.dz) + (size_t)row * p.lddz;
+  if (p.dz && row < p.R) {
+    auto give = [&](const Piece<TI>& q, int i) {
+      float d[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float x = q.get(e) - M;
+        d[e] = two ? a_soft * __builtin_amdgcn_exp2f(x * p.c_soft) + a_hard * __builtin_amdgcn_exp2f(x * p.c_hard) - base
+                   : a_both * __builtin_amdgcn_exp2f(x * p.c_soft) - base;
+      }
+      put_piece<E>(dz + (size_t)i * E, d, i < full ? E : p.C - i * E);
+    };
+    if (live) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (tid + c * TH < pieces) give(r[c], tid + c * TH);
+      for (int i = tid + C * TH; i < pieces; i += TH) {
+        Piece<TI> q;
+        fetch(q, i);
+        give(q, i);
+      }
+    } else {
+      const float d[E] = {};
+      for (int i = tid; i < pieces; i += TH) put_piece<E>(dz + (size_t)i * E, d, i < full ? E : p.C - i * E);
+    }
+  }
+  __syncthreads();  // P is whole, and the classes below are written after everybody's pieces
+
+  double kl = 0.0, named = 0.0;
+  if (live) {
+    const double log_s = log(S);
+    for (int k = tid; k < K + 1; k += TH) {
+      const bool is_label = k == K;  // the label's class, unless a pair names it
+      const int j = is_label ? (has_label ? label : -1) : at[k];
+      if (j < 0) continue;
+      double Pj = is_label ? share : 0.0;
+      bool first = true;
+      for (int i = 0; i < K; ++i)
+        if (at[i] == j) {
+          if (i < k) first = false;
+          Pj += P[i];
+        }
+      if (!first) continue;
+      const float x = (is_label ? zl : zt[k]) - M;
+      if (!is_label) {
+        const double lq = (double)x * ((double)p.c_soft * LN2) - log_s;
+        named += lq;
+        if (Pj != 0.0) kl += Pj * (log(Pj) - lq);
+      }
+      if (p.dz) {
+        const double y = (j == label ? 1.0 - p.smooth : 0.0) + (double)p.smooth / p.C;
+        const float q = two ? a_soft * __builtin_amdgcn_exp2f(x * p.c_soft) + a_hard * __builtin_amdgcn_exp2f(x * p.c_hard)
+                            : a_both * __builtin_amdgcn_exp2f(x * p.c_soft);
+        put(dz + j, q - (float)(gs * (p.soft * p.T * Pj + hard * y)));
+      }
+    }
+  }
+  if (p.loss_rows == nullptr) return;
+  if (64 * wave < K) {
+    kl = wave_sum_d(kl);
+    named = wave_sum_d(named);
+  }
+  if (first_lane) {
+    lpart[sub][wave][0] = kl;
+    lpart[sub][wave][1] = named;
+  }
+  __syncthreads();
+  if (tid == 0 && row < p.R) {
+    double loss = 0.0;
+    if (live) {
+      kl = named = 0.0;
+      for (int w = 0; w < W; ++w) {
+        kl += lpart[sub][w][0];
+        named += lpart[sub][w][1];
+      }
+      if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log(S) - named);
+      if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
+      if (hard != 0.0) {
+        double ce = log(H) - (1.0 - p.smooth) * ((double)zl - M);
+        if (p.smooth != 0.0f) ce -= p.smooth * (Z / p.C - M);
+        loss += hard * ce;
+      }
+      loss *= weight;
+    }
+    p.loss_rows[row] = (float)loss;
+  }
+}
+
+// out[c] += sum over rows of g[:, c]: 64 columns a block, 16 row strips, fixed order
+template <typename T>
+__global__ __launch_bounds__(1024) void distill_colsum_kernel(const T* __restrict__ g, long ld, int R, int C, float* __restrict__ out) {
+  __shared__ float red[16][64];
+  const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, col = blockIdx.x * 64 + c;
+  float s = 0.f;
+  if (col < C) {
+#pragma unroll 8
+    for (int r = strip; r < R; r += 16) s += to_float(g[(size_t)r * ld + col]);
+  }
+  red[strip][c] = s;
+  __syncthreads();
+  if (strip == 0 && col < C) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][c];
+    out[col] += s;
+  }
+}
+
+template <typename TI, typename TO, int W, int C>
+int launch_distill(const DistillParams& p, hipStream_t st) {
+  constexpr int RPB = W < 4 ? 4 / W : 1;
+  hipLaunchKernelGGL((distill_kernel<TI, TO, W, C>), dim3((unsigned)((p.R + RPB - 1) / RPB)), dim3(W < 4 ? 256 : 64 * W),
+                     (size_t)RPB * (p.K > 0 ? p.K : 1) * 16, st, p);
+  SAVIT_LAUNCH_RET();
+}
+// A row's threads grow with its pieces: a wave (no idle wave where rows are short), four, sixteen; sixteen keep 4, 8 or 16 pieces each (the
+// register file holds 128 registers a thread at that size: 16 pieces take 64)
+template <typename TI, typename TO>
+int choose_distill(const DistillParams& p, hipStream_t st) {
+  const int pieces = (p.C + Piece<TI>::E - 1) / Piece<TI>::E;
+  if (pieces <= 64 * 2) return launch_distill<TI, TO, 1, 2>(p, st);
+  if (pieces <= 256 * 4) return launch_distill<TI, TO, 4, 4>(p, st);
+  if (pieces <= 1024 * 4) return launch_distill<TI, TO, 16, 4>(p, st);
+  if (pieces <= 1024 * 8) return launch_distill<TI, TO, 16, 8>(p, st);
+  return launch_distill<TI, TO, 16, 16>(p, st);
+}
+
+}  // namespace
+
+extern "C" int savit_distill_xent(const void* logits, long ld_logits, int logits_bf16, const float* teacher_logits, const int* teacher_index, int K,
+                                  const float* teacher_lse, const int* labels, const float* row_weight, float temperature, float distill_weight,
+                                  float hard_weight, float label_smoothing, float grad_scale, float* loss_rows, void* dlogits, long ld_dlogits,
+                                  int dlogits_bf16, float* dbias, int R, int C, void* stream) {
+  SAVIT_CHECK_ARG(logits && R >= 0 && C > 0 && ld_logits >= C && K >= 0 && K <= DS_MAX_K && (K == 0 || (teacher_logits && teacher_index)));
+  SAVIT_CHECK_ARG(temperature > 0.f && temperature < __builtin_inff() && (hard_weight == 0.f || labels) && label_smoothing >= 0.f && label_smoothing <= 1.f);
+  SAVIT_CHECK_ARG((dlogits || loss_rows) && (!dlogits || ld_dlogits >= C) && (!dbias || dlogits));
+  SAVIT_CHECK_ARG(((uintptr_t)logits % (logits_bf16 ? 2 : 4)) == 0 && ((uintptr_t)dlogits % (dlogits_bf16 ? 2 : 4)) == 0);
+  SAVIT_CHECK_ARG(dlogits != logits || (logits_bf16 == dlogits_bf16 && ld_logits == ld_dlogits));
+  if (R == 0) return SAVIT_OK;
+  DistillParams p{};
+  p.z = logits; p.top = teacher_logits; p.at = teacher_index; p.lse = teacher_lse; p.labels = labels; p.weight = row_weight;
+  p.loss_rows = loss_rows; p.dz = dlogits; p.ldz = ld_logits; p.lddz = ld_dlogits; p.R = R; p.C = C; p.K = K;
+  p.soft = distill_weight; p.hard = hard_weight; p.smooth = hard_weight != 0.f ? label_smoothing : 0.f; p.T = temperature;
+  p.c_soft = (float)(1.4426950408889634 / (double)temperature);
+  p.c_hard = 1.44269504088896340736f;
+  p.grad_scale = grad_scale;
+  const hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (logits_bf16) rc = dlogits && !dlogits_bf16 ? choose_distill<bf16_t, float>(p, st) : choose_distill<bf16_t, bf16_t>(p, st);
+  else rc = dlogits && dlogits_bf16 ? choose_distill<float, bf16_t>(p, st) : choose_distill<float, float>(p, st);
+  if (rc != SAVIT_OK || !dbias) return rc;
+  const dim3 grid((unsigned)((C + 63) / 64));
+  if (dlogits_bf16) hipLaunchKernelGGL(distill_colsum_kernel<bf16_t>, grid, dim3(1024), 0, st, (const bf16_t*)dlogits, ld_dlogits, R, C, dbias);
+  else hipLaunchKernelGGL(distill_colsum_kernel<float>, grid, dim3(1024), 0, st, (const float*)dlogits, ld_dlogits, R, C, dbias);
+  SAVIT_LAUNCH_RET();
+}

@@ -106,6 +106,19 @@ _SIGNATURES = {
     "savit_attention_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "savit_attention_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
                                     c_void_p]),
+    "savit_qk_norm_rope_fwd": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long] + [c_int] * 6
+                               + [c_float, c_float, c_int, c_int, c_void_p]),
+    "savit_qk_norm_rope_bwd": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p,
+                                       c_void_p] + [c_int] * 6 + [c_float, c_float, c_int, c_int, c_void_p, c_long, c_void_p]),
+    "savit_qk_norm_rope_bwd_workspace_bytes": (c_long, [c_int, c_int, c_int]),
+    "savit_relpos_bias_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "savit_relpos_bias_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_long, c_void_p]),
+    "savit_relpos_bias_bwd_workspace_bytes": (c_long, [c_int, c_int, c_int]),
+    "savit_bias_attention_fwd": (c_int, [c_void_p] * 5 + [c_int] * 6 + [c_void_p]),
+    "savit_bias_attention_bwd": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_float, c_void_p, c_long, c_void_p]),
+    "savit_bias_attention_bwd_workspace_bytes": (c_long, [c_int] * 5),
+    "savit_distill_xent": (c_int, [c_void_p, c_long, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_float, c_float, c_float, c_float,
+                                   c_float, c_void_p, c_void_p, c_long, c_int, c_void_p, c_int, c_int, c_void_p]),
     "savit_th_attention_fwd": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
     "savit_th_attention_bwd": (c_int, [c_void_p] * 10 + [c_int] * 6 + [c_float, c_void_p, c_long, c_void_p]),
     "savit_th_attention_bwd_workspace_bytes": (c_long, [c_int, c_int, c_int]),

@@ -856,3 +856,335 @@ def seq16_attention_bwd(qkv: torch.Tensor, d_o: torch.Tensor, nseq: int, dq_scal
     _lib.check(_lib.load().savit_seq16_attention_bwd(_p(qkv), _p(d_o), _p(dqkv), nseq, 16, 4, 16, 192, float(dq_scale), _stream()),
                "savit_seq16_attention_bwd")
     return dqkv
+
+
+# --------------------------------------------------------------------------------------------- position in attention
+def _here(*tensors):
+    """Kernels are launched on the current device's current stream: every tensor has to live there."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{cur}")
+
+
+def rope_table(angles: torch.Tensor, device="cuda") -> torch.Tensor:
+    """Rotation table fp32 [positions, head_dim] = cosines | sines of angles [positions, head_dim / 2] (computed in 64 bits)."""
+    a = torch.as_tensor(angles).double()
+    return torch.cat([a.cos(), a.sin()], dim=1).float().to(device).contiguous()
+
+
+def rope_angles_1d(positions: int, head_dim: int, base: float = 10000.0) -> torch.Tensor:
+    """Angles [positions, head_dim / 2] of one axis: position * base^(-2e / head_dim)."""
+    e = torch.arange(head_dim // 2, dtype=torch.float64)
+    return torch.arange(positions, dtype=torch.float64)[:, None] * base ** (-2.0 * e / head_dim)
+
+
+def rope_angles_2d(grid_h: int, grid_w: int, head_dim: int, base: float = 100.0, cls: bool = True) -> torch.Tensor:
+    """Angles of a patch grid (row-major): the first half of the pairs turns with the row, the second with the column; a class token in front
+    (angle 0) stays as it is.  head_dim % 4 == 0."""
+    if head_dim % 4:
+        raise ValueError("rope_angles_2d: head_dim must be a multiple of 4")
+    ay, ax = (rope_angles_1d(n, head_dim // 2, base) for n in (grid_h, grid_w))
+    a = torch.cat([ay[:, None, :].expand(-1, grid_w, -1), ax[None, :, :].expand(grid_h, -1, -1)], dim=2).reshape(grid_h * grid_w, head_dim // 2)
+    return torch.cat([torch.zeros(1, head_dim // 2, dtype=torch.float64), a]) if cls else a
+
+
+def _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions):
+    if qkv.dtype not in (bf16, f32):
+        raise ValueError("qkv: bf16 or fp32")
+    _chk(qkv, qkv.dtype, "qkv", 2)
+    rows, cols, ld = _rows2d(qkv, "qkv")
+    Hk = H if Hk is None else Hk
+    if cols < (H + 2 * Hk) * head_dim:
+        raise ValueError(f"qkv {tuple(qkv.shape)} too narrow for H={H} Hk={Hk} head_dim={head_dim}")
+    for name, w in (("wq", wq), ("wk", wk)):
+        _chk(w, f32, name, 1)
+        if w.numel() != head_dim:
+            raise ValueError(f"{name}: one weight per column of a head")
+    T = 0
+    if table is not None:
+        _chk(table, f32, "table", 2)
+        T = table.shape[0]
+        if table.shape[1] != head_dim or not table.is_contiguous():
+            raise ValueError("table: contiguous [positions, head_dim] cosines | sines")
+        if positions is None and T < min(N, rows):
+            raise ValueError("table: fewer rows than tokens")
+    if positions is not None:
+        _chk(positions, torch.int32, "positions", 1)
+        if positions.numel() != rows:
+            raise ValueError("positions: one per row")
+    return rows, cols, ld, Hk, T
+
+
+def qk_norm_rope_fwd(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, table: Optional[torch.Tensor], N: int, H: int, Hk: Optional[int] = None,
+                     head_dim: int = 64, positions: Optional[torch.Tensor] = None, eps: float = 1e-6, q_scale: float = 1.0, center: bool = False,
+                     interleaved: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Per-head norm (root mean square, or LayerNorm statistics with center=True) of the queries and keys of packed rows
+    [rows, >= (H + 2 Hk) * head_dim] (bf16 or fp32), times wq / wk [head_dim], turned by row `position` of `table` (rope_table; None: no
+    rotation; position = positions[row], or row mod N), queries times q_scale.  Values are copied into `out` (new by default); out=qkv works in
+    place - but backward wants the input.  savit_qk_norm_rope_fwd."""
+    rows, cols, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions)
+    width = (H + 2 * Hk) * head_dim
+    if out is None:
+        out = torch.empty((rows, width), dtype=qkv.dtype, device=qkv.device)
+    _chk(out, qkv.dtype, "out", 2)
+    ro, co, ldo = _rows2d(out, "out")
+    if ro != rows or co < width:
+        raise ValueError("out: qkv's rows and at least its packed width")
+    _here(qkv, wq, wk, table, positions, out)
+    if rows == 0:
+        return out
+    _lib.check(_lib.load().savit_qk_norm_rope_fwd(_p(qkv), ld, _p(wq), _p(wk), _p(table), T, _p(positions), _p(out), ldo, rows, N, H, Hk, head_dim,
+                                                  int(qkv.dtype == bf16), float(eps), float(q_scale), int(center), int(interleaved), _stream()),
+               "savit_qk_norm_rope_fwd")
+    return out
+
+
+def qk_norm_rope_bwd(dqkv: torch.Tensor, qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, table: Optional[torch.Tensor], dwq: torch.Tensor,
+                     dwk: torch.Tensor, N: int, H: int, Hk: Optional[int] = None, head_dim: int = 64, positions: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6, q_scale: float = 1.0, center: bool = False, interleaved: bool = False, out: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Backward of qk_norm_rope_fwd: dqkv is the cotangent of its output, qkv its INPUT.  The gradient replaces dqkv's queries and keys in place
+    (values are left alone), or goes to `out` (values copied).  dwq / dwk [head_dim] accumulate.  q_scale and the flags are the forward's.
+    savit_qk_norm_rope_bwd."""
+    rows, cols, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions)
+    width = (H + 2 * Hk) * head_dim
+    out = dqkv if out is None else out
+    for name, t in (("dqkv", dqkv), ("out", out)):
+        _chk(t, qkv.dtype, name, 2)
+        if t.shape[0] != rows or t.shape[1] < width:
+            raise ValueError(f"{name}: qkv's rows and at least its packed width")
+    for name, t in (("dwq", dwq), ("dwk", dwk)):
+        _chk(t, f32, name, 1)
+        if t.numel() != head_dim:
+            raise ValueError(f"{name}: head_dim elements")
+    if rows == 0:
+        return out
+    L = _lib.load()
+    need = L.savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim)
+    if workspace is None:
+        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=qkv.device)
+    _here(dqkv, qkv, wq, wk, table, positions, out, dwq, dwk, workspace)
+    _lib.check(L.savit_qk_norm_rope_bwd(_p(dqkv), _rows2d(dqkv, "dqkv")[2], _p(qkv), ld, _p(wq), _p(wk), _p(table), T, _p(positions), _p(out),
+                                        _rows2d(out, "out")[2], _p(dwq), _p(dwk), rows, N, H, Hk, head_dim, int(qkv.dtype == bf16), float(eps),
+                                        float(q_scale), int(center), int(interleaved), _p(workspace), workspace.numel() * workspace.element_size(),
+                                        _stream()), "savit_qk_norm_rope_bwd")
+    return out
+
+
+def relpos_index_2d(grid_h: int, grid_w: int, cls: bool = True, device="cuda") -> Tuple[torch.Tensor, int]:
+    """Bucket of (query, key) on a patch grid: one per (row offset, column offset); with a class token in front three more - class token to patch,
+    patch to class token, class token to itself.  Returns (index int32 [N, N], number of buckets)."""
+    t = torch.arange(grid_h * grid_w)
+    y, x = t // grid_w, t % grid_w
+    index = (y[:, None] - y[None, :] + grid_h - 1) * (2 * grid_w - 1) + (x[:, None] - x[None, :] + grid_w - 1)
+    n = (2 * grid_h - 1) * (2 * grid_w - 1)
+    if cls:
+        full = torch.empty((grid_h * grid_w + 1,) * 2, dtype=torch.long)
+        full[1:, 1:] = index
+        full[0, :], full[:, 0], full[0, 0] = n, n + 1, n + 2
+        index, n = full, n + 3
+    return index.to(torch.int32).to(device).contiguous(), n
+
+
+def relpos_index_1d(N: int, buckets: int = 32, max_distance: int = 128, device="cuda") -> Tuple[torch.Tensor, int]:
+    """Bucket of (query, key) by distance: half the buckets for keys behind the query, half for keys before it; in each half the first half is one
+    bucket a distance, the rest grows with its logarithm up to max_distance and the last takes everything beyond."""
+    if buckets < 4 or buckets % 4 or max_distance <= buckets // 4:
+        raise ValueError("relpos_index_1d: buckets a multiple of 4, max_distance > buckets / 4")
+    d = torch.arange(N)[None, :] - torch.arange(N)[:, None]
+    a, half = d.abs(), buckets // 2
+    near = half // 2
+    far = near + (torch.log(a.clamp(min=1).double() / near) / math.log(max_distance / near) * (half - near)).long()
+    index = torch.where(a < near, a, far.clamp(max=half - 1)) + half * (d > 0).long()
+    return index.to(torch.int32).to(device).contiguous(), buckets
+
+
+def relpos_order(index: torch.Tensor, buckets: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Lists that relpos_bias_bwd walks, laid out once per index: (order int32 [N*N] = positions sorted by bucket, start int32 [buckets + 1])."""
+    flat = index.reshape(-1).long()
+    if flat.numel() and (int(flat.min()) < 0 or int(flat.max()) >= buckets):
+        raise ValueError("relpos_order: index outside [0, buckets)")
+    order = torch.sort(flat, stable=True).indices.to(torch.int32)
+    start = torch.zeros(buckets + 1, dtype=torch.int32, device=index.device)
+    start[1:] = torch.bincount(flat, minlength=buckets).cumsum(0)
+    return order, start
+
+
+def _bias_ld(bias: torch.Tensor, H: Optional[int], N: int, name: str) -> int:
+    _chk(bias, f32, name, 3)
+    ld = bias.stride(1)
+    if bias.shape[1] != N or bias.shape[2] != N or (H is not None and bias.shape[0] != H):
+        raise ValueError(f"{name}: expected [H, N, N], got {tuple(bias.shape)}")
+    if ld < N or ld % 4 or (bias.shape[0] > 1 and bias.stride(0) != N * ld) or \
+            bias.untyped_storage().nbytes() < 4 * (bias.storage_offset() + bias.shape[0] * N * ld):
+        raise ValueError(f"{name}: row pitch must be a multiple of 4 elements and heads N rows apart, the last row padded too (see relpos_bias_empty)")
+    return ld
+
+
+def relpos_bias_empty(H: int, N: int, device="cuda") -> torch.Tensor:
+    """An [H, N, N] fp32 bias (or gradient) buffer as the kernels want it: a view with the row pitch rounded up to 4 elements."""
+    return torch.empty((H, N, (N + 3) // 4 * 4), dtype=f32, device=device)[:, :, :N]
+
+
+def relpos_bias_fwd(table: torch.Tensor, index: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bias[h, i, j] = table[index[i, j], h]: table fp32 [buckets, H], index int32 [N, N] -> fp32 [H, N, N] (relpos_bias_empty).  savit_relpos_bias_fwd."""
+    _chk(table, f32, "table", 2)
+    _chk(index, torch.int32, "index", 2)
+    N = index.shape[0]
+    nb, H = table.shape
+    if index.shape[1] != N or not index.is_contiguous() or not table.is_contiguous():
+        raise ValueError("relpos_bias_fwd: contiguous index [N, N] and table [buckets, H]")
+    if out is None:
+        out = relpos_bias_empty(H, N, table.device)
+    ld = _bias_ld(out, H, N, "out")
+    _here(table, index, out)
+    _lib.check(_lib.load().savit_relpos_bias_fwd(_p(table), _p(index), _p(out), N, H, nb, ld, _stream()), "savit_relpos_bias_fwd")
+    return out
+
+
+def relpos_bias_bwd(dbias: torch.Tensor, order: torch.Tensor, start: torch.Tensor, dtable: torch.Tensor,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dtable[b, h] += sum of dbias[h] over the positions of bucket b; (order, start) from relpos_order.  Repeats bit by bit.  savit_relpos_bias_bwd."""
+    _chk(dtable, f32, "dtable", 2)
+    nb, H = dtable.shape
+    N = dbias.shape[1] if dbias.dim() == 3 else -1
+    ld = _bias_ld(dbias, H, N, "dbias")
+    _chk(order, torch.int32, "order", 1)
+    _chk(start, torch.int32, "start", 1)
+    if order.numel() != N * N or start.numel() != nb + 1 or not dtable.is_contiguous():
+        raise ValueError("relpos_bias_bwd: order [N*N], start [buckets + 1], contiguous dtable [buckets, H]")
+    L = _lib.load()
+    need = L.savit_relpos_bias_bwd_workspace_bytes(N, H, nb)
+    if workspace is None and need:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=dbias.device)
+    _here(dbias, order, start, dtable, workspace)
+    wbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _lib.check(L.savit_relpos_bias_bwd(_p(dbias), _p(order), _p(start), _p(dtable), N, H, nb, ld, _p(workspace), wbytes, _stream()), "savit_relpos_bias_bwd")
+    return dtable
+
+
+def _bias_attn_args(qkv, bias, B, N, H, head_dim, lens):
+    _chk(qkv, bf16, "qkv", 2)
+    rows, cols, ld = _rows2d(qkv, "qkv")
+    if B < 0 or N < 1 or H < 1 or rows < B * N or cols < 3 * H * head_dim:
+        raise ValueError(f"qkv {tuple(qkv.shape)} too small for B={B} N={N} H={H}")
+    ldb = _bias_ld(bias, H, N, "bias")
+    if lens is not None:
+        _chk(lens, torch.int32, "lens", 1)
+        if lens.numel() != B:
+            raise ValueError("lens: one per sequence")
+    return ld, ldb
+
+
+def bias_attention_fwd(qkv: torch.Tensor, bias: torch.Tensor, B: int, N: int, H: int, head_dim: int = 64, lens: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+    """attention_fwd with scores q k^T + bias[h] (bias fp32 [H, N, N], shared by the images: relpos_bias_fwd, or any mask / bias in a
+    relpos_bias_empty buffer).  lens int32 [B]: a padded batch.  Returns (o bf16 [B*N, H*head_dim], lse fp32 [B, H, N]).  savit_bias_attention_fwd."""
+    ld, ldb = _bias_attn_args(qkv, bias, B, N, H, head_dim, lens)
+    d = H * head_dim
+    o = out if out is not None else torch.empty((B * N, d), dtype=bf16, device=qkv.device)
+    lse = lse if lse is not None else torch.empty((B, H, N), dtype=f32, device=qkv.device)
+    _chk(o, bf16, "out", 2)
+    _chk(lse, f32, "lse")
+    if not o.is_contiguous() or tuple(o.shape) != (B * N, d) or lse.numel() != B * H * N or not lse.is_contiguous():
+        raise ValueError("bias_attention_fwd: bad output buffers")
+    _here(qkv, bias, lens, o, lse)
+    if B == 0:
+        return o, lse
+    _lib.check(_lib.load().savit_bias_attention_fwd(_p(qkv), _p(bias), _p(lens), _p(o), _p(lse), B, N, H, head_dim, ld, ldb, _stream()),
+               "savit_bias_attention_fwd")
+    return o, lse
+
+
+def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor, lse: torch.Tensor, B: int, N: int, H: int, dq_scale: float,
+                       head_dim: int = 64, lens: Optional[torch.Tensor] = None, dqkv: Optional[torch.Tensor] = None,
+                       dbias: Optional[torch.Tensor] = None, want_dbias: bool = True, workspace: Optional[torch.Tensor] = None):
+    """Backward of bias_attention_fwd.  Returns (dqkv bf16, dbias fp32 [H, N, N] = the bias gradient summed over the batch, or None with
+    want_dbias=False).  savit_bias_attention_bwd."""
+    ld, ldb = _bias_attn_args(qkv, bias, B, N, H, head_dim, lens)
+    d = H * head_dim
+    _chk(d_o, bf16, "d_o", 2)
+    _chk(lse, f32, "lse")
+    if tuple(d_o.shape) != (B * N, d) or not d_o.is_contiguous() or lse.numel() != B * H * N or not lse.is_contiguous():
+        raise ValueError("bias_attention_bwd: d_o contiguous [B*N, d], lse [B, H, N]")
+    if dqkv is None:
+        dqkv = torch.empty((B * N, 3 * d) if ld == 3 * d else (B * N, ld), dtype=bf16, device=qkv.device)
+    _chk(dqkv, bf16, "dqkv", 2)
+    r2, c2, ld2 = _rows2d(dqkv, "dqkv")
+    if r2 < B * N or c2 < 3 * d or (ld2 != ld and B * N > 1):
+        raise ValueError("dqkv must have qkv's shape and row stride")
+    if want_dbias:
+        if dbias is None:
+            dbias = torch.empty((H, N, ldb), dtype=f32, device=qkv.device)[:, :, :N]
+        if _bias_ld(dbias, H, N, "dbias") != ldb:
+            raise ValueError("dbias must have bias's row pitch")
+        if B == 0:
+            dbias.zero_()
+    else:
+        dbias = None
+    if B == 0:
+        return dqkv, dbias
+    L = _lib.load()
+    need = L.savit_bias_attention_bwd_workspace_bytes(B, N, H, ldb, int(want_dbias))
+    if workspace is None:
+        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=qkv.device)
+    _here(qkv, bias, d_o, lse, lens, dqkv, dbias, workspace)
+    _lib.check(L.savit_bias_attention_bwd(_p(qkv), _p(bias), _p(lens), _p(d_o), _p(lse), _p(dqkv), _p(dbias), B, N, H, head_dim, ld, ldb, float(dq_scale),
+                                          _p(workspace), workspace.numel() * workspace.element_size(), _stream()), "savit_bias_attention_bwd")
+    return dqkv, dbias
+
+
+# --------------------------------------------------------------------------------------------- distillation
+def distill_xent(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, temperature: float = 1.0,
+                 distill_weight: float = 1.0, teacher_lse: Optional[torch.Tensor] = None, labels: Optional[torch.Tensor] = None,
+                 hard_weight: float = 0.0, label_smoothing: float = 0.0, row_weight: Optional[torch.Tensor] = None,
+                 grad_scale: Optional[float] = None, loss_rows: Optional[torch.Tensor] = None, dlogits: Optional[torch.Tensor] = None,
+                 dbias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Distillation from a teacher's K largest logits [R, K] and their classes (int32; a class outside [0, C) is no pair), with softmax_xent's
+    hard-label loss beside it: per row
+        distill_weight T^2 KL(P || softmax(logits / T)) + hard_weight CE(logits, smoothed label),
+    P = softmax(teacher_logits / T) over the pairs, or with teacher_lse [R] (the teacher's log-sum-exp over all classes at temperature T) their
+    true probabilities, the rest spread evenly over the other classes.  logits fp32 / bf16 [R, C]; dlogits (optional, fp32 / bf16, may be logits
+    itself) receives grad_scale (1 / R by default) times the gradient; dbias [C] accumulates its column sums.  Returns loss_rows [R].
+    savit_distill_xent."""
+    if logits.dtype not in (bf16, f32):
+        raise ValueError("logits: bf16 or fp32")
+    _chk(logits, logits.dtype, "logits", 2)
+    R, C, ld = _rows2d(logits, "logits")
+    _chk(teacher_logits, f32, "teacher_logits", 2)
+    _chk(teacher_index, torch.int32, "teacher_index", 2)
+    K = teacher_logits.shape[1]
+    if tuple(teacher_logits.shape) != (R, K) or tuple(teacher_index.shape) != (R, K) or not teacher_logits.is_contiguous() or not teacher_index.is_contiguous():
+        raise ValueError("teacher_logits and teacher_index: contiguous [R, K]")
+    if labels is not None:
+        _chk(labels, torch.int32, "labels", 1)
+        if labels.numel() != R:
+            raise ValueError("labels: one per row")
+    elif hard_weight != 0.0:
+        raise ValueError("hard_weight needs labels")
+    ld_dz = 0
+    if dlogits is not None:
+        if dlogits.dtype not in (bf16, f32):
+            raise ValueError("dlogits: bf16 or fp32")
+        _chk(dlogits, dlogits.dtype, "dlogits", 2)
+        r, c, ld_dz = _rows2d(dlogits, "dlogits")
+        if r != R or c < C:
+            raise ValueError("dlogits too small")
+        if dlogits.data_ptr() == logits.data_ptr() and R * C and (dlogits.dtype != logits.dtype or ld_dz != ld):
+            raise ValueError("dlogits in logits' place needs its dtype and row stride")
+    loss_rows = loss_rows if loss_rows is not None else torch.empty((R,), dtype=f32, device=logits.device)
+    for name, t, n in (("teacher_lse", teacher_lse, R), ("row_weight", row_weight, R), ("loss_rows", loss_rows, R), ("dbias", dbias, C)):
+        if t is not None:
+            _chk(t, f32, name, 1)
+            if t.numel() != n:
+                raise ValueError(f"{name}: {n} elements")
+    gs = (1.0 / max(R, 1)) if grad_scale is None else float(grad_scale)
+    _here(logits, teacher_logits, teacher_index, teacher_lse, labels, row_weight, loss_rows, dlogits, dbias)
+    if R == 0:
+        return loss_rows
+    _lib.check(_lib.load().savit_distill_xent(_p(logits), ld, int(logits.dtype == bf16), _p(teacher_logits), _p(teacher_index), K, _p(teacher_lse),
+                                              _p(labels), _p(row_weight), float(temperature), float(distill_weight), float(hard_weight),
+                                              float(label_smoothing), gs, _p(loss_rows), _p(dlogits), ld_dz,
+                                              int(dlogits is not None and dlogits.dtype == bf16), _p(dbias), R, C, _stream()), "savit_distill_xent")
+    return loss_rows
