@@ -11,6 +11,8 @@
 // Exponentials are v_exp_f32 on (z - max) * (log2 e / T), per-thread sums fp32; everything that exists once a row - the pairs, the
 // normalisers, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
 // The gradient is written for every class as if no pair named it, then the at most K + 1 classes with a pair or the label are written again.
+#include <type_traits>
+
 #include "common.h"
 #include "savit.h"
 
@@ -29,7 +31,7 @@ struct DistillParams {
   float* loss_rows;     // [R] or nullptr
   void* dz;             // or nullptr
   long ldz, lddz;
-  int R, C, K;
+  int R, C, K, slots;
   float soft, hard, smooth, T, c_soft, c_hard, grad_scale;  // c_soft = log2 e / T, c_hard = log2 e
 };
 
@@ -40,6 +42,7 @@ struct Piece<float> {
   static constexpr int E = 4;
   typedef f32x4 vec __attribute__((aligned(4)));
   float v[4];
+  __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = -INFINITY; }
   __device__ __forceinline__ void load(const float* p) {
     const vec r = *reinterpret_cast<const vec*>(p);
 #pragma unroll
@@ -56,6 +59,7 @@ struct Piece<bf16_t> {
   static constexpr int E = 8;
   typedef u32x4 vec __attribute__((aligned(2)));
   uint32_t v[4];
+  __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0xff80ff80u; }
   __device__ __forceinline__ void load(const bf16_t* p) {
     const vec r = *reinterpret_cast<const vec*>(p);
 #pragma unroll
@@ -81,7 +85,7 @@ __device__ __forceinline__ void put_piece(float* p, const float (&v)[E], int n) 
   typedef f32x4 vec __attribute__((aligned(4)));
   if (n == E) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<vec*>(p + i) = vec{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    for (int i = 0; i < E; i += 4) __builtin_nontemporal_store(vec{v[i], v[i + 1], v[i + 2], v[i + 3]}, reinterpret_cast<vec*>(p + i));
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)
@@ -93,10 +97,10 @@ __device__ __forceinline__ void put_piece(bf16_t* p, const float (&v)[E], int n)
   if (n == E) {
     if constexpr (E == 8) {
       typedef u32x4 vec __attribute__((aligned(2)));
-      *reinterpret_cast<vec*>(p) = vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+      __builtin_nontemporal_store(vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])}, reinterpret_cast<vec*>(p));
     } else {
       typedef u32x2 vec __attribute__((aligned(2)));
-      *reinterpret_cast<vec*>(p) = vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      __builtin_nontemporal_store(vec{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}, reinterpret_cast<vec*>(p));
     }
   } else {
 #pragma unroll
@@ -111,6 +115,7 @@ struct Seen {
   float m, s, h, z;
 };
 
+__device__ __forceinline__ unsigned hash_of(int j) { return (unsigned)j * 2654435761u >> 16; }
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -122,24 +127,76 @@ __device__ __forceinline__ double wave_max_d(double v) {
   return v;
 }
 
-// W waves a row (4 / W rows a block where W < 4), C pieces of the row kept by a thread.
-template <typename TI, typename TO, int W, int C>
-__global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const DistillParams p) {
-  constexpr int TH = 64 * W, RPB = W < 4 ? 4 / W : 1, E = Piece<TI>::E;
+// exp2((z - m) c) as exp2(fma(z, c, -mb)), mb = m c rounded: one instruction less an element (the exponentials are a third of the kernel's
+// time at 131 072 classes).  The sums are then relative to mb, not m c: residue() puts them right.  Where m c is beyond 1e5 (a row masked with the type's
+// lowest value) the plain form is taken.
+__device__ __forceinline__ bool in_range(float mb) { return fabsf(mb) < 1e5f; }
+__device__ __forceinline__ float residue(float m, float c) { return in_range(m * c) ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -(m * c))) : 1.f; }
+__device__ __forceinline__ float rescale(float from, float to, float c) {
+  return __builtin_amdgcn_exp2f(in_range(from * c) && in_range(to * c) ? from * c - to * c : (from - to) * c);
+}
+template <int G, typename T>
+__device__ __forceinline__ float sum_exps(const Piece<T>* q, float m, float c) {
+  const float mb = m * c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (in_range(mb)) {
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+#pragma unroll
+      for (int e = 0; e < Piece<T>::E; ++e) s[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(q[k].get(e), c, -mb));
+  } else {
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+#pragma unroll
+      for (int e = 0; e < Piece<T>::E; ++e) s[e & 3] += __builtin_amdgcn_exp2f((q[k].get(e) - m) * c);
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// over the W lanes of a group (W = 1, 4, 8, 16)
+template <int W>
+__device__ __forceinline__ float waves_sum(float v) {
+  if constexpr (W >= 4) {
+    v += dpp_mov<0xB1>(v);  // quad_perm [1,0,3,2]
+    v += dpp_mov<0x4E>(v);  // quad_perm [2,3,0,1]
+  }
+  if constexpr (W >= 8) v += dpp_mov<0x141>(v);   // row_half_mirror
+  if constexpr (W >= 16) v += dpp_mov<0x140>(v);  // row_mirror
+  return v;
+}
+template <int W>
+__device__ __forceinline__ float waves_max(float v) {
+  if constexpr (W >= 4) {
+    v = fmaxf(v, dpp_mov<0xB1>(v));
+    v = fmaxf(v, dpp_mov<0x4E>(v));
+  }
+  if constexpr (W >= 8) v = fmaxf(v, dpp_mov<0x141>(v));
+  if constexpr (W >= 16) v = fmaxf(v, dpp_mov<0x140>(v));
+  return v;
+}
+
+// W waves a row (4 / W rows a block where W < 4), C pieces of the row kept by a thread, OCC waves a SIMD.
+template <typename TI, typename TO, int W, int C, int OCC>
+__global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(const DistillParams p) {
+  constexpr int TH = 64 * W, RPB = W < 4 ? 4 / W : 1, E = Piece<TI>::E, GROUP = C % 4 == 0 ? 4 : 2;
+  static_assert(C % GROUP == 0, "whole groups");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ Seen part[RPB][W];
   __shared__ double tpart[RPB][W][2], lpart[RPB][W][2];
-  __shared__ int distinct[RPB];
+  __shared__ int distinct[RPB], repeated[RPB];
   const int sub = RPB > 1 ? threadIdx.x / TH : 0;  // row of the block
   const int tid = RPB > 1 ? threadIdx.x - sub * TH : threadIdx.x;
   const int wave = tid >> 6;
   const bool first_lane = (tid & 63) == 0;
   const int row = blockIdx.x * RPB + sub;
   const int K = p.K;
-  // LDS of a row: K pairs {P (first the logit / T), z at the class, class}
-  double* P = reinterpret_cast<double*>(smem) + (size_t)sub * K;
+  // LDS of a row: K pairs {logit / T, z at the class, class, what the gradient takes off there}, and a hash table of their classes
+  double* tt = reinterpret_cast<double*>(smem) + (size_t)sub * K;
   float* zt = reinterpret_cast<float*>(smem + (size_t)RPB * K * 8) + (size_t)sub * K;
   int* at = reinterpret_cast<int*>(smem + (size_t)RPB * K * 12) + (size_t)sub * K;
+  float* off = reinterpret_cast<float*>(smem + (size_t)RPB * K * 16) + (size_t)sub * K;
+  int* table = reinterpret_cast<int*>(smem + (size_t)RPB * K * 20) + (size_t)sub * p.slots;
+  const unsigned mask = p.slots - 1;
 
   const float weight = row < p.R ? (p.weight ? p.weight[row] : 1.0f) : 0.0f;
   const bool live = weight != 0.0f;  // rows of weight 0 are not read
@@ -147,6 +204,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const Dis
   const int pieces = (p.C + E - 1) / E, full = p.C / E;  // the last piece may be a partial one
   const int label = live && p.labels ? p.labels[row] : -1;
   const bool has_label = p.hard != 0.0f && (unsigned)label < (unsigned)p.C;
+  const float zl = tid == TH - 64 && has_label ? to_float(z[label]) : 0.f;  // read before anything is written in z's place
   const bool two = p.hard != 0.0f && p.c_hard != p.c_soft;  // a second sum of exponentials
   const bool need_z = p.lse != nullptr || p.smooth != 0.0f;
   auto fetch = [&](Piece<TI>& q, int i) {
@@ -155,64 +213,86 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const Dis
   };
 
   Piece<TI> r[C];
-  Seen me{-3.402823466e38f, 0.f, 0.f, 0.f};
-  double tm = -1.7976931348623157e308;
-  float zl = 0.f;
-  auto see = [&](const Piece<TI>& q, int i) {
-    float m = me.m;
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, q.get(e));
-    if (m != me.m) {
-      me.s *= __builtin_amdgcn_exp2f((me.m - m) * p.c_soft);
-      if (two) me.h *= __builtin_amdgcn_exp2f((me.m - m) * p.c_hard);
-      me.m = m;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) me.s += __builtin_amdgcn_exp2f((q.get(e) - m) * p.c_soft);
-    if (two) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) me.h += __builtin_amdgcn_exp2f((q.get(e) - m) * p.c_hard);
-    }
-    if (need_z) {
-      const int n = p.C - i * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < n) me.z += q.get(e);
-    }
-  };
   if (live) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      r[c].clear();
       if (tid + c * TH < pieces) fetch(r[c], tid + c * TH);
-    for (int k = tid; k < K; k += TH) {  // the pairs, while the row is on its way
+    }
+  }
+  for (int i = tid; i < p.slots; i += TH) table[i] = -1;
+  if (tid == 0) distinct[sub] = repeated[sub] = 0;
+  __syncthreads();
+
+  double tm = -1.7976931348623157e308;
+  if (live && 64 * wave < K) {  // the pairs, while the row is on its way
+    int mine = 0;
+    for (int k = tid; k < K; k += TH) {
       const int j = p.at[(size_t)row * K + k];
       const bool ok = (unsigned)j < (unsigned)p.C;
       const double t = ok ? (double)p.top[(size_t)row * K + k] / (double)p.T : -__builtin_inf();
       at[k] = ok ? j : -1;
       zt[k] = ok ? to_float(z[j]) : 0.f;
-      P[k] = t;
+      tt[k] = t;
       tm = fmax(tm, t);
+      if (ok) {  // twice as many slots as pairs: an empty one is always found
+        unsigned s = hash_of(j) & mask;
+        int was;
+        while ((was = atomicCAS(&table[s], -1, j)) != -1 && was != j) s = (s + 1) & mask;
+        if (was == -1) ++mine;
+        else repeated[sub] = 1;
+      }
     }
-    if (has_label) zl = to_float(z[label]);
+    if (mine) atomicAdd(&distinct[sub], mine);
+  }
+  Seen me{-3.402823466e38f, 0.f, 0.f, 0.f};
+  if (live) {
+    // G pieces at a time: one comparison with the running maximum, then independent exponentials (a piece at a time its short dependent
+    // chains left a third of the time idle); pieces beyond the row are -inf and add nothing
+    auto see = [&](const Piece<TI>* q, int i0, auto g) {
+      constexpr int G = decltype(g)::value;
+      float m = me.m;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (tid + c * TH < pieces) see(r[c], tid + c * TH);
+      for (int k = 0; k < G; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, q[k].get(e));
+      if (m != me.m) {
+        me.s *= rescale(me.m, m, p.c_soft);
+        if (two) me.h *= rescale(me.m, m, p.c_hard);
+        me.m = m;
+      }
+      me.s += sum_exps<G>(q, m, p.c_soft);
+      if (two) me.h += sum_exps<G>(q, m, p.c_hard);
+      if (need_z) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          const int n = p.C - (i0 + k * TH) * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (e < n) me.z += q[k].get(e);
+        }
+      }
+    };
+#pragma unroll
+    for (int c = 0; c < C; c += GROUP)
+      if (c * TH < pieces) see(r + c, tid + c * TH, std::integral_constant<int, GROUP>{});
     for (int i = tid + C * TH; i < pieces; i += TH) {
       Piece<TI> q;
       fetch(q, i);
-      see(q, i);
+      see(&q, i, std::integral_constant<int, 1>{});
     }
   }
-  if (tid == 0) distinct[sub] = 0;
   {
+    me.s *= residue(me.m, p.c_soft);
+    if (two) me.h *= residue(me.m, p.c_hard);
     const float M = wave_max(me.m);
     const Seen w{M, wave_sum(me.s * __builtin_amdgcn_exp2f((me.m - M) * p.c_soft)),
                  two ? wave_sum(me.h * __builtin_amdgcn_exp2f((me.m - M) * p.c_hard)) : 0.f, need_z ? wave_sum(me.z) : 0.f};
     double ts = 0.0;
     if (64 * wave < K) {
-      tm = wave_max_d(tm);
+      tm = p.lse ? (live ? (double)p.lse[row] : 0.0) : wave_max_d(tm);  // what this wave's sum is relative to
       if (live)
-        for (int k = tid; k < K; k += TH) ts += exp(P[k] - tm);
+        for (int k = tid; k < K; k += TH) ts += exp(tt[k] - tm);
       ts = wave_sum_d(ts);
     }
     if (first_lane) {
@@ -223,71 +303,52 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const Dis
   }
   __syncthreads();
 
-  // the row's maximum and normalisers, in every thread
-  float M = part[sub][0].m;
-  double TM = tpart[sub][0][0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) {
-    M = fmaxf(M, part[sub][w].m);
-    TM = fmax(TM, tpart[sub][w][0]);
-  }
-  double S = 0.0, H = 0.0, Z = 0.0, tsum = 0.0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const Seen o = part[sub][w];
-    S += (double)(o.s * __builtin_amdgcn_exp2f((o.m - M) * p.c_soft));
-    if (two) H += (double)(o.h * __builtin_amdgcn_exp2f((o.m - M) * p.c_hard));
-    Z += (double)o.z;
-    if (64 * w < K && tpart[sub][w][1] != 0.0) tsum += tpart[sub][w][1] * exp(tpart[sub][w][0] - TM);
-  }
-  if (!two) H = S;
-
-  // the teacher's probabilities; mass that is left over goes evenly to the classes that no pair names
-  double left = 0.0, share = 0.0, mass;
-  if (p.lse) {
-    const double lse = live ? (double)p.lse[row] : 0.0;
-    int mine = 0;
-    if (live)
-      for (int k = tid; k < K; k += TH) {
-        P[k] = exp(P[k] - lse);
-        bool first = at[k] >= 0;
-        for (int i = 0; first && i < k; ++i) first = at[i] != at[k];
-        mine += first;
-      }
-    if (mine) atomicAdd(&distinct[sub], mine);
-    __syncthreads();
-    const int others = p.C - distinct[sub];
-    mass = tsum == 0.0 ? 0.0 : tsum * exp(TM - lse);
-    if (others > 0) {
-      left = mass < 1.0 ? 1.0 - mass : (mass == mass ? 0.0 : mass);
-      share = left / others;
+  // mass of the pairs with what is left over for the classes that no pair names
+  auto masses = [&](double& mass, double& left) {
+    left = mass = 0.0;
+    for (int w = 0; w < W && 64 * w < K; ++w) mass += tpart[sub][w][1];
+    if (p.lse) {
+      if (p.C > distinct[sub]) left = mass < 1.0 ? 1.0 - mass : (mass == mass ? 0.0 : mass);
+      mass += left;
+    } else if (mass > 0.0) {
+      mass = 1.0;  // (NaN goes on)
     }
-    mass += left;
-  } else {
-    const double inv = tsum == 0.0 ? 0.0 : 1.0 / tsum;
-    if (live)
-      for (int k = tid; k < K; k += TH) P[k] = exp(P[k] - TM) * inv;
-    mass = tsum == 0.0 ? 0.0 : (tsum == tsum ? 1.0 : tsum);
-  }
-
+  };
   const double gs = (double)p.grad_scale * weight;
-  const double hard = p.hard != 0.0f && has_label ? p.hard : 0.0;
-  const float a_soft = (float)(gs * p.soft * p.T * mass / S), a_hard = hard != 0.0 ? (float)(gs * hard / H) : 0.0f;
+  const double hard = has_label ? p.hard : 0.0;
+  float M, a_soft, a_hard = 0.f, base;
+  {  // the waves' partials, one a lane: every group of W lanes joins them
+    const Seen s = part[sub][tid & (W - 1)];
+    M = waves_max<W>(s.m);
+    const float S = waves_sum<W>(s.s * __builtin_amdgcn_exp2f((s.m - M) * p.c_soft));
+    if (hard != 0.0) a_hard = (float)(gs * hard) / (two ? waves_sum<W>(s.h * __builtin_amdgcn_exp2f((s.m - M) * p.c_hard)) : S);
+    double mass, left;
+    masses(mass, left);
+    a_soft = (float)(gs * p.soft * p.T * mass) / S;
+    base = (float)(gs * p.soft * p.T * left) / (float)(left != 0.0 ? p.C - distinct[sub] : 1) + (float)(gs * hard * p.smooth) / (float)p.C;
+  }
+  // the gradient but for the target.  FAST: relative to M c rounded, the difference in the factor
+  const bool fast = in_range(M * p.c_soft) && in_range(M * p.c_hard);
+  const float Ms = M * p.c_soft, Mh = M * p.c_hard;
+  a_soft *= 1.f / residue(M, p.c_soft);
+  a_hard *= 1.f / residue(M, p.c_hard);
   const float a_both = a_soft + a_hard;
-  const float base = (float)(gs * (p.soft * p.T * share + hard * p.smooth / p.C));
+  auto gradient = [&](float zj, auto is_fast) {
+    constexpr bool FAST = decltype(is_fast)::value;
+    const float es = __builtin_amdgcn_exp2f(FAST ? __builtin_fmaf(zj, p.c_soft, -Ms) : (zj - M) * p.c_soft);
+    if (!two) return a_both * es;
+    return a_soft * es + a_hard * __builtin_amdgcn_exp2f(FAST ? __builtin_fmaf(zj, p.c_hard, -Mh) : (zj - M) * p.c_hard);
+  };
+  auto gradient_any = [&](float zj) { return fast ? gradient(zj, std::true_type{}) : gradient(zj, std::false_type{}); };
   TO* dz = reinterpret_cast<TO*>(p.dz) + (size_t)row * p.lddz;
   if (p.dz && row < p.R) {
-    auto give = [&](const Piece<TI>& q, int i) {
-      float d[E];
+    auto give_all = [&](auto is_fast) {
+      auto give = [&](const Piece<TI>& q, int i) {
+        float d[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float x = q.get(e) - M;
-        d[e] = two ? a_soft * __builtin_amdgcn_exp2f(x * p.c_soft) + a_hard * __builtin_amdgcn_exp2f(x * p.c_hard) - base
-                   : a_both * __builtin_amdgcn_exp2f(x * p.c_soft) - base;
-      }
-      put_piece<E>(dz + (size_t)i * E, d, i < full ? E : p.C - i * E);
-    };
-    if (live) {
+        for (int e = 0; e < E; ++e) d[e] = gradient(q.get(e), is_fast) - base;
+        put_piece<E>(dz + (size_t)i * E, d, i < full ? E : p.C - i * E);
+      };
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (tid + c * TH < pieces) give(r[c], tid + c * TH);
@@ -296,71 +357,97 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void distill_kernel(const Dis
         fetch(q, i);
         give(q, i);
       }
+    };
+    if (live) {
+      if (fast) give_all(std::true_type{});
+      else give_all(std::false_type{});
     } else {
       const float d[E] = {};
       for (int i = tid; i < pieces; i += TH) put_piece<E>(dz + (size_t)i * E, d, i < full ? E : p.C - i * E);
     }
   }
-  __syncthreads();  // P is whole, and the classes below are written after everybody's pieces
 
-  double kl = 0.0, named = 0.0;
-  if (live) {
-    const double log_s = log(S);
-    for (int k = tid; k < K + 1; k += TH) {
-      const bool is_label = k == K;  // the label's class, unless a pair names it
-      const int j = is_label ? (has_label ? label : -1) : at[k];
+  // the named classes' share of the loss, and what the gradient takes off there (while the stores above drain)
+  auto join = [&](float c, bool h) {  // a sum of exponentials, in 64 bits (only after the gradient, whose registers it would take)
+    double s = 0.0;
+#pragma unroll 1
+    for (int w = 0; w < W; ++w) s += (double)((h ? part[sub][w].h : part[sub][w].s) * __builtin_amdgcn_exp2f((part[sub][w].m - M) * c));
+    return s;
+  };
+  asm volatile("" ::: "memory");
+  if (live && 64 * wave < K) {
+    double ref = tpart[sub][0][0], inv = 1.0;  // P = exp(t - ref) inv
+    if (!p.lse) {
+      double sum = 0.0;
+      for (int w = 1; w < W && 64 * w < K; ++w) ref = fmax(ref, tpart[sub][w][0]);
+      for (int w = 0; w < W && 64 * w < K; ++w) sum += tpart[sub][w][1] == 0.0 ? 0.0 : tpart[sub][w][1] * exp(tpart[sub][w][0] - ref);
+      inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+    }
+    const double log_s = log(join(p.c_soft, false));
+    double kl = 0.0, named = 0.0;
+    for (int k = tid; k < K; k += TH) {
+      const int j = at[k];
       if (j < 0) continue;
-      double Pj = is_label ? share : 0.0;
+      double P = exp(tt[k] - ref) * inv;
       bool first = true;
-      for (int i = 0; i < K; ++i)
-        if (at[i] == j) {
-          if (i < k) first = false;
-          Pj += P[i];
-        }
-      if (!first) continue;
-      const float x = (is_label ? zl : zt[k]) - M;
-      if (!is_label) {
-        const double lq = (double)x * ((double)p.c_soft * LN2) - log_s;
-        named += lq;
-        if (Pj != 0.0) kl += Pj * (log(Pj) - lq);
+      if (repeated[sub]) {  // a class named more than once has the sum, and counts once
+        P = 0.0;
+        for (int i = 0; i < K; ++i)
+          if (at[i] == j) {
+            if (i < k) first = false;
+            P += exp(tt[i] - ref) * inv;
+          }
       }
-      if (p.dz) {
-        const double y = (j == label ? 1.0 - p.smooth : 0.0) + (double)p.smooth / p.C;
-        const float q = two ? a_soft * __builtin_amdgcn_exp2f(x * p.c_soft) + a_hard * __builtin_amdgcn_exp2f(x * p.c_hard)
-                            : a_both * __builtin_amdgcn_exp2f(x * p.c_soft);
-        put(dz + j, q - (float)(gs * (p.soft * p.T * Pj + hard * y)));
+      off[k] = (float)(gs * (p.soft * p.T * P + hard * ((j == label ? 1.0 - p.smooth : 0.0) + (double)p.smooth / p.C)));
+      if (first) {
+        const double lq = (double)(zt[k] - M) * ((double)p.c_soft * LN2) - log_s;
+        named += lq;
+        if (P != 0.0) kl += P * (log(P) - lq);
       }
     }
-  }
-  if (p.loss_rows == nullptr) return;
-  if (64 * wave < K) {
     kl = wave_sum_d(kl);
     named = wave_sum_d(named);
-  }
-  if (first_lane) {
-    lpart[sub][wave][0] = kl;
-    lpart[sub][wave][1] = named;
-  }
-  __syncthreads();
-  if (tid == 0 && row < p.R) {
-    double loss = 0.0;
-    if (live) {
-      kl = named = 0.0;
-      for (int w = 0; w < W; ++w) {
-        kl += lpart[sub][w][0];
-        named += lpart[sub][w][1];
-      }
-      if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log(S) - named);
-      if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
-      if (hard != 0.0) {
-        double ce = log(H) - (1.0 - p.smooth) * ((double)zl - M);
-        if (p.smooth != 0.0f) ce -= p.smooth * (Z / p.C - M);
-        loss += hard * ce;
-      }
-      loss *= weight;
+    if (first_lane) {
+      lpart[sub][wave][0] = kl;
+      lpart[sub][wave][1] = named;
     }
-    p.loss_rows[row] = (float)loss;
   }
+  __syncthreads();  // the named classes are written after everybody's pieces
+
+  if (!live) {
+    if (tid == 0 && row < p.R && p.loss_rows) p.loss_rows[row] = 0.f;
+    return;
+  }
+  if (p.dz) {
+    for (int k = tid; k < K; k += TH)
+      if (at[k] >= 0) put(dz + at[k], gradient_any(zt[k]) - off[k]);
+  }
+  if (tid != TH - 64) return;  // the row's scalars: a thread of the wave with the fewest pairs
+  double mass, left;
+  masses(mass, left);
+  const double share = left != 0.0 ? left / (p.C - distinct[sub]) : 0.0;
+  if (p.dz && has_label) {  // the label's class, unless a pair names it
+    unsigned s = hash_of(label) & mask;
+    while (table[s] != -1 && table[s] != label) s = (s + 1) & mask;
+    if (table[s] == -1) put(dz + label, gradient_any(zl) - (float)(gs * (p.soft * p.T * share + hard * (1.0 - p.smooth + (double)p.smooth / p.C))));
+  }
+  if (p.loss_rows == nullptr) return;
+  double kl = 0.0, named = 0.0, loss = 0.0;
+  for (int w = 0; w < W && 64 * w < K; ++w) {
+    kl += lpart[sub][w][0];
+    named += lpart[sub][w][1];
+  }
+  const double log_s = log(join(p.c_soft, false));
+  double Z = 0.0;
+  for (int w = 0; w < W; ++w) Z += (double)part[sub][w].z;
+  if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log_s - named);
+  if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
+  if (hard != 0.0) {
+    double ce = (two ? log(join(p.c_hard, true)) : log_s) - (1.0 - p.smooth) * ((double)zl - M);
+    if (p.smooth != 0.0f) ce -= p.smooth * (Z / p.C - M);
+    loss += hard * ce;
+  }
+  p.loss_rows[row] = (float)(loss * weight);
 }
 
 // out[c] += sum over rows of g[:, c]: 64 columns a block, 16 row strips, fixed order
@@ -382,23 +469,22 @@ __global__ __launch_bounds__(1024) void distill_colsum_kernel(const T* __restric
   }
 }
 
-template <typename TI, typename TO, int W, int C>
+template <typename TI, typename TO, int W, int C, int OCC>
 int launch_distill(const DistillParams& p, hipStream_t st) {
   constexpr int RPB = W < 4 ? 4 / W : 1;
-  hipLaunchKernelGGL((distill_kernel<TI, TO, W, C>), dim3((unsigned)((p.R + RPB - 1) / RPB)), dim3(W < 4 ? 256 : 64 * W),
-                     (size_t)RPB * (p.K > 0 ? p.K : 1) * 16, st, p);
+  hipLaunchKernelGGL((distill_kernel<TI, TO, W, C, OCC>), dim3((unsigned)((p.R + RPB - 1) / RPB)), dim3(W < 4 ? 256 : 64 * W),
+                     (size_t)RPB * (p.K * 20 + p.slots * 4), st, p);
   SAVIT_LAUNCH_RET();
 }
-// A row's threads grow with its pieces: a wave (no idle wave where rows are short), four, sixteen; sixteen keep 4, 8 or 16 pieces each (the
-// register file holds 128 registers a thread at that size: 16 pieces take 64)
+// A row's threads grow with its pieces: a wave (no idle wave where rows are short), four, sixteen; two workgroups of sixteen waves share a CU (64
+// registers a thread), so that one row loads while another computes or stores
 template <typename TI, typename TO>
 int choose_distill(const DistillParams& p, hipStream_t st) {
   const int pieces = (p.C + Piece<TI>::E - 1) / Piece<TI>::E;
-  if (pieces <= 64 * 2) return launch_distill<TI, TO, 1, 2>(p, st);
-  if (pieces <= 256 * 4) return launch_distill<TI, TO, 4, 4>(p, st);
-  if (pieces <= 1024 * 4) return launch_distill<TI, TO, 16, 4>(p, st);
-  if (pieces <= 1024 * 8) return launch_distill<TI, TO, 16, 8>(p, st);
-  return launch_distill<TI, TO, 16, 16>(p, st);
+  if (pieces <= 64 * 2) return launch_distill<TI, TO, 1, 2, 4>(p, st);
+  if (pieces <= 256 * 4) return launch_distill<TI, TO, 4, 4, 6>(p, st);
+  if (pieces <= 512 * 12) return launch_distill<TI, TO, 8, 12, 4>(p, st);
+  return launch_distill<TI, TO, 16, 16, 4>(p, st);
 }
 
 }  // namespace
@@ -420,6 +506,7 @@ extern "C" int savit_distill_xent(const void* logits, long ld_logits, int logits
   p.c_soft = (float)(1.4426950408889634 / (double)temperature);
   p.c_hard = 1.44269504088896340736f;
   p.grad_scale = grad_scale;
+  for (p.slots = 16; p.slots < 2 * K; p.slots *= 2) {}
   const hipStream_t st = (hipStream_t)stream;
   int rc;
   if (logits_bf16) rc = dlogits && !dlogits_bf16 ? choose_distill<bf16_t, float>(p, st) : choose_distill<bf16_t, bf16_t>(p, st);

@@ -16,7 +16,8 @@ f32 = torch.float32
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current device's current stream as a raw handle (the Stream object of torch.cuda.current_stream() costs 4 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -26,7 +27,7 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 def _chk(t: torch.Tensor, dtype, name: str, ndim: Optional[int] = None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA (HIP) tensor - there is no CPU path")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
     if ndim is not None and t.dim() != ndim:
         raise ValueError(f"{name}: expected {ndim} dims, got {tuple(t.shape)}")
@@ -859,12 +860,43 @@ def seq16_attention_bwd(qkv: torch.Tensor, d_o: torch.Tensor, nseq: int, dq_scal
 
 
 # --------------------------------------------------------------------------------------------- position in attention
-def _here(*tensors):
-    """Kernels are launched on the current device's current stream: every tensor has to live there."""
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{cur}")
+def _dev(t) -> int:
+    """The current device, for an operator whose first operand is t: kernels are launched on its current stream, so every tensor has to live there."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("expected a CUDA (HIP) tensor - there is no CPU path")
+    return torch._C._cuda_getDevice()
+
+
+def _whole(t, dtype, shape, name: str, dev: int):
+    """t is a contiguous tensor of this type and shape on the current device."""
+    if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return
+    _chk(t, dtype, name, len(shape))
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, but the current device is cuda:{dev}")
+    raise ValueError(f"{name}: expected a contiguous {tuple(shape)} tensor, got {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _packed(t, dtype, rows: int, cols: int, name: str, dev: int) -> int:
+    """t is a 2-D row-major view on the current device with at least rows x cols elements; returns its row pitch."""
+    if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype and t.dim() == 2:
+        r, c = t.shape
+        sr, sc = t.stride()
+        if r >= rows and c >= cols and (sc == 1 or c == 1):
+            return sr if r > 1 else max(sr, c)
+    _chk(t, dtype, name, 2)
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, but the current device is cuda:{dev}")
+    raise ValueError(f"{name}: expected at least [{rows}, {cols}], got {tuple(t.shape)}")
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, device, dev: int):
+    """The caller's workspace, or a new one -> (tensor, its bytes)."""
+    if workspace is None:
+        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor on the current device")
+    return workspace, workspace.numel() * workspace.element_size()
 
 
 def rope_table(angles: torch.Tensor, device="cuda") -> torch.Tensor:
@@ -889,31 +921,24 @@ def rope_angles_2d(grid_h: int, grid_w: int, head_dim: int, base: float = 100.0,
     return torch.cat([torch.zeros(1, head_dim // 2, dtype=torch.float64), a]) if cls else a
 
 
-def _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions):
-    if qkv.dtype not in (bf16, f32):
+def _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions, dev):
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype not in (bf16, f32):
         raise ValueError("qkv: bf16 or fp32")
-    _chk(qkv, qkv.dtype, "qkv", 2)
-    rows, cols, ld = _rows2d(qkv, "qkv")
     Hk = H if Hk is None else Hk
-    if cols < (H + 2 * Hk) * head_dim:
-        raise ValueError(f"qkv {tuple(qkv.shape)} too narrow for H={H} Hk={Hk} head_dim={head_dim}")
-    for name, w in (("wq", wq), ("wk", wk)):
-        _chk(w, f32, name, 1)
-        if w.numel() != head_dim:
-            raise ValueError(f"{name}: one weight per column of a head")
+    width = (H + 2 * Hk) * head_dim
+    ld = _packed(qkv, qkv.dtype, 0, width, "qkv", dev)
+    rows = qkv.shape[0]
+    _whole(wq, f32, (head_dim,), "wq", dev)
+    _whole(wk, f32, (head_dim,), "wk", dev)
     T = 0
     if table is not None:
-        _chk(table, f32, "table", 2)
         T = table.shape[0]
-        if table.shape[1] != head_dim or not table.is_contiguous():
-            raise ValueError("table: contiguous [positions, head_dim] cosines | sines")
+        _whole(table, f32, (T, head_dim), "table", dev)
         if positions is None and T < min(N, rows):
             raise ValueError("table: fewer rows than tokens")
     if positions is not None:
-        _chk(positions, torch.int32, "positions", 1)
-        if positions.numel() != rows:
-            raise ValueError("positions: one per row")
-    return rows, cols, ld, Hk, T
+        _whole(positions, torch.int32, (rows,), "positions", dev)
+    return rows, width, ld, Hk, T
 
 
 def qk_norm_rope_fwd(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, table: Optional[torch.Tensor], N: int, H: int, Hk: Optional[int] = None,
@@ -923,20 +948,17 @@ def qk_norm_rope_fwd(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, tabl
     [rows, >= (H + 2 Hk) * head_dim] (bf16 or fp32), times wq / wk [head_dim], turned by row `position` of `table` (rope_table; None: no
     rotation; position = positions[row], or row mod N), queries times q_scale.  Values are copied into `out` (new by default); out=qkv works in
     place - but backward wants the input.  savit_qk_norm_rope_fwd."""
-    rows, cols, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions)
-    width = (H + 2 * Hk) * head_dim
+    dev = _dev(qkv)
+    rows, width, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions, dev)
     if out is None:
         out = torch.empty((rows, width), dtype=qkv.dtype, device=qkv.device)
-    _chk(out, qkv.dtype, "out", 2)
-    ro, co, ldo = _rows2d(out, "out")
-    if ro != rows or co < width:
-        raise ValueError("out: qkv's rows and at least its packed width")
-    _here(qkv, wq, wk, table, positions, out)
+        ldo = width
+    else:
+        ldo = _packed(out, qkv.dtype, rows, width, "out", dev)
     if rows == 0:
         return out
-    _lib.check(_lib.load().savit_qk_norm_rope_fwd(_p(qkv), ld, _p(wq), _p(wk), _p(table), T, _p(positions), _p(out), ldo, rows, N, H, Hk, head_dim,
-                                                  int(qkv.dtype == bf16), float(eps), float(q_scale), int(center), int(interleaved), _stream()),
-               "savit_qk_norm_rope_fwd")
+    _lib.check(_lib.load().savit_qk_norm_rope_fwd(qkv.data_ptr(), ld, wq.data_ptr(), wk.data_ptr(), _p(table), T, _p(positions), out.data_ptr(), ldo, rows, N, H,
+                                                  Hk, head_dim, qkv.dtype is bf16, eps, q_scale, center, interleaved, _stream()), "savit_qk_norm_rope_fwd")
     return out
 
 
@@ -947,28 +969,22 @@ def qk_norm_rope_bwd(dqkv: torch.Tensor, qkv: torch.Tensor, wq: torch.Tensor, wk
     """Backward of qk_norm_rope_fwd: dqkv is the cotangent of its output, qkv its INPUT.  The gradient replaces dqkv's queries and keys in place
     (values are left alone), or goes to `out` (values copied).  dwq / dwk [head_dim] accumulate.  q_scale and the flags are the forward's.
     savit_qk_norm_rope_bwd."""
-    rows, cols, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions)
-    width = (H + 2 * Hk) * head_dim
-    out = dqkv if out is None else out
-    for name, t in (("dqkv", dqkv), ("out", out)):
-        _chk(t, qkv.dtype, name, 2)
-        if t.shape[0] != rows or t.shape[1] < width:
-            raise ValueError(f"{name}: qkv's rows and at least its packed width")
-    for name, t in (("dwq", dwq), ("dwk", dwk)):
-        _chk(t, f32, name, 1)
-        if t.numel() != head_dim:
-            raise ValueError(f"{name}: head_dim elements")
+    dev = _dev(qkv)
+    rows, width, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions, dev)
+    ldd = _packed(dqkv, qkv.dtype, rows, width, "dqkv", dev)
+    if out is None:
+        out, ldo = dqkv, ldd
+    else:
+        ldo = _packed(out, qkv.dtype, rows, width, "out", dev)
+    _whole(dwq, f32, (head_dim,), "dwq", dev)
+    _whole(dwk, f32, (head_dim,), "dwk", dev)
     if rows == 0:
         return out
     L = _lib.load()
-    need = L.savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim)
-    if workspace is None:
-        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=qkv.device)
-    _here(dqkv, qkv, wq, wk, table, positions, out, dwq, dwk, workspace)
-    _lib.check(L.savit_qk_norm_rope_bwd(_p(dqkv), _rows2d(dqkv, "dqkv")[2], _p(qkv), ld, _p(wq), _p(wk), _p(table), T, _p(positions), _p(out),
-                                        _rows2d(out, "out")[2], _p(dwq), _p(dwk), rows, N, H, Hk, head_dim, int(qkv.dtype == bf16), float(eps),
-                                        float(q_scale), int(center), int(interleaved), _p(workspace), workspace.numel() * workspace.element_size(),
-                                        _stream()), "savit_qk_norm_rope_bwd")
+    ws, n = _scratch(workspace, L.savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim), qkv.device, dev)
+    _lib.check(L.savit_qk_norm_rope_bwd(dqkv.data_ptr(), ldd, qkv.data_ptr(), ld, wq.data_ptr(), wk.data_ptr(), _p(table), T, _p(positions), out.data_ptr(), ldo,
+                                        dwq.data_ptr(), dwk.data_ptr(), rows, N, H, Hk, head_dim, qkv.dtype is bf16, eps, q_scale, center, interleaved,
+                                        ws.data_ptr(), n, _stream()), "savit_qk_norm_rope_bwd")
     return out
 
 
@@ -1011,15 +1027,19 @@ def relpos_order(index: torch.Tensor, buckets: int) -> Tuple[torch.Tensor, torch
     return order, start
 
 
-def _bias_ld(bias: torch.Tensor, H: Optional[int], N: int, name: str) -> int:
+def _bias_ld(bias: torch.Tensor, H: int, N: int, name: str, dev: int) -> int:
+    """Row pitch of an [H, N, N] fp32 bias (or gradient) whose rows are padded to 4 elements, the last one too."""
+    if isinstance(bias, torch.Tensor) and bias.get_device() == dev and bias.dtype is f32 and bias.shape == (H, N, N):
+        sh, ld, sc = bias.stride()
+        if (sc == 1 or N == 1) and ld >= N and ld % 4 == 0 and (H == 1 or sh == N * ld) and \
+                bias.untyped_storage().nbytes() >= 4 * (bias.storage_offset() + H * N * ld):
+            return ld
     _chk(bias, f32, name, 3)
-    ld = bias.stride(1)
-    if bias.shape[1] != N or bias.shape[2] != N or (H is not None and bias.shape[0] != H):
-        raise ValueError(f"{name}: expected [H, N, N], got {tuple(bias.shape)}")
-    if ld < N or ld % 4 or (bias.shape[0] > 1 and bias.stride(0) != N * ld) or \
-            bias.untyped_storage().nbytes() < 4 * (bias.storage_offset() + bias.shape[0] * N * ld):
-        raise ValueError(f"{name}: row pitch must be a multiple of 4 elements and heads N rows apart, the last row padded too (see relpos_bias_empty)")
-    return ld
+    if bias.get_device() != dev:
+        raise ValueError(f"{name}: on {bias.device}, but the current device is cuda:{dev}")
+    if bias.shape != (H, N, N):
+        raise ValueError(f"{name}: expected {(H, N, N)}, got {tuple(bias.shape)}")
+    raise ValueError(f"{name}: rows must be a multiple of 4 elements apart and heads N rows, the last row padded too (see relpos_bias_empty)")
 
 
 def relpos_bias_empty(H: int, N: int, device="cuda") -> torch.Tensor:
@@ -1029,109 +1049,99 @@ def relpos_bias_empty(H: int, N: int, device="cuda") -> torch.Tensor:
 
 def relpos_bias_fwd(table: torch.Tensor, index: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bias[h, i, j] = table[index[i, j], h]: table fp32 [buckets, H], index int32 [N, N] -> fp32 [H, N, N] (relpos_bias_empty).  savit_relpos_bias_fwd."""
+    dev = _dev(table)
     _chk(table, f32, "table", 2)
-    _chk(index, torch.int32, "index", 2)
-    N = index.shape[0]
     nb, H = table.shape
-    if index.shape[1] != N or not index.is_contiguous() or not table.is_contiguous():
-        raise ValueError("relpos_bias_fwd: contiguous index [N, N] and table [buckets, H]")
+    _whole(table, f32, (nb, H), "table", dev)
+    N = index.shape[0]
+    _whole(index, torch.int32, (N, N), "index", dev)
     if out is None:
-        out = relpos_bias_empty(H, N, table.device)
-    ld = _bias_ld(out, H, N, "out")
-    _here(table, index, out)
-    _lib.check(_lib.load().savit_relpos_bias_fwd(_p(table), _p(index), _p(out), N, H, nb, ld, _stream()), "savit_relpos_bias_fwd")
+        ld = (N + 3) // 4 * 4
+        out = torch.empty((H, N, ld), dtype=f32, device=table.device)
+        if ld != N:
+            out = out[:, :, :N]
+    else:
+        ld = _bias_ld(out, H, N, "out", dev)
+    _lib.check(_lib.load().savit_relpos_bias_fwd(table.data_ptr(), index.data_ptr(), out.data_ptr(), N, H, nb, ld, _stream()), "savit_relpos_bias_fwd")
     return out
 
 
 def relpos_bias_bwd(dbias: torch.Tensor, order: torch.Tensor, start: torch.Tensor, dtable: torch.Tensor,
                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """dtable[b, h] += sum of dbias[h] over the positions of bucket b; (order, start) from relpos_order.  Repeats bit by bit.  savit_relpos_bias_bwd."""
+    dev = _dev(dbias)
     _chk(dtable, f32, "dtable", 2)
     nb, H = dtable.shape
-    N = dbias.shape[1] if dbias.dim() == 3 else -1
-    ld = _bias_ld(dbias, H, N, "dbias")
-    _chk(order, torch.int32, "order", 1)
-    _chk(start, torch.int32, "start", 1)
-    if order.numel() != N * N or start.numel() != nb + 1 or not dtable.is_contiguous():
-        raise ValueError("relpos_bias_bwd: order [N*N], start [buckets + 1], contiguous dtable [buckets, H]")
+    _whole(dtable, f32, (nb, H), "dtable", dev)
+    _chk(dbias, f32, "dbias", 3)
+    N = dbias.shape[1]
+    ld = _bias_ld(dbias, H, N, "dbias", dev)
+    _whole(order, torch.int32, (N * N,), "order", dev)
+    _whole(start, torch.int32, (nb + 1,), "start", dev)
     L = _lib.load()
     need = L.savit_relpos_bias_bwd_workspace_bytes(N, H, nb)
-    if workspace is None and need:
-        workspace = torch.empty((need,), dtype=torch.uint8, device=dbias.device)
-    _here(dbias, order, start, dtable, workspace)
-    wbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    _lib.check(L.savit_relpos_bias_bwd(_p(dbias), _p(order), _p(start), _p(dtable), N, H, nb, ld, _p(workspace), wbytes, _stream()), "savit_relpos_bias_bwd")
+    ws, n = _scratch(workspace, need, dbias.device, dev) if need else (None, 0)
+    _lib.check(L.savit_relpos_bias_bwd(dbias.data_ptr(), order.data_ptr(), start.data_ptr(), dtable.data_ptr(), N, H, nb, ld, _p(ws), n, _stream()),
+               "savit_relpos_bias_bwd")
     return dtable
-
-
-def _bias_attn_args(qkv, bias, B, N, H, head_dim, lens):
-    _chk(qkv, bf16, "qkv", 2)
-    rows, cols, ld = _rows2d(qkv, "qkv")
-    if B < 0 or N < 1 or H < 1 or rows < B * N or cols < 3 * H * head_dim:
-        raise ValueError(f"qkv {tuple(qkv.shape)} too small for B={B} N={N} H={H}")
-    ldb = _bias_ld(bias, H, N, "bias")
-    if lens is not None:
-        _chk(lens, torch.int32, "lens", 1)
-        if lens.numel() != B:
-            raise ValueError("lens: one per sequence")
-    return ld, ldb
 
 
 def bias_attention_fwd(qkv: torch.Tensor, bias: torch.Tensor, B: int, N: int, H: int, head_dim: int = 64, lens: Optional[torch.Tensor] = None,
                        out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
     """attention_fwd with scores q k^T + bias[h] (bias fp32 [H, N, N], shared by the images: relpos_bias_fwd, or any mask / bias in a
     relpos_bias_empty buffer).  lens int32 [B]: a padded batch.  Returns (o bf16 [B*N, H*head_dim], lse fp32 [B, H, N]).  savit_bias_attention_fwd."""
-    ld, ldb = _bias_attn_args(qkv, bias, B, N, H, head_dim, lens)
+    dev = _dev(qkv)
     d = H * head_dim
-    o = out if out is not None else torch.empty((B * N, d), dtype=bf16, device=qkv.device)
-    lse = lse if lse is not None else torch.empty((B, H, N), dtype=f32, device=qkv.device)
-    _chk(o, bf16, "out", 2)
-    _chk(lse, f32, "lse")
-    if not o.is_contiguous() or tuple(o.shape) != (B * N, d) or lse.numel() != B * H * N or not lse.is_contiguous():
-        raise ValueError("bias_attention_fwd: bad output buffers")
-    _here(qkv, bias, lens, o, lse)
+    ld = _packed(qkv, bf16, B * N, 3 * d, "qkv", dev)
+    ldb = _bias_ld(bias, H, N, "bias", dev)
+    if lens is not None:
+        _whole(lens, torch.int32, (B,), "lens", dev)
+    if out is None:
+        out = torch.empty((B * N, d), dtype=bf16, device=qkv.device)
+    else:
+        _whole(out, bf16, (B * N, d), "out", dev)
+    if lse is None:
+        lse = torch.empty((B, H, N), dtype=f32, device=qkv.device)
+    else:
+        _whole(lse, f32, (B, H, N), "lse", dev)
     if B == 0:
-        return o, lse
-    _lib.check(_lib.load().savit_bias_attention_fwd(_p(qkv), _p(bias), _p(lens), _p(o), _p(lse), B, N, H, head_dim, ld, ldb, _stream()),
+        return out, lse
+    _lib.check(_lib.load().savit_bias_attention_fwd(qkv.data_ptr(), bias.data_ptr(), _p(lens), out.data_ptr(), lse.data_ptr(), B, N, H, head_dim, ld, ldb, _stream()),
                "savit_bias_attention_fwd")
-    return o, lse
+    return out, lse
 
 
 def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor, lse: torch.Tensor, B: int, N: int, H: int, dq_scale: float,
                        head_dim: int = 64, lens: Optional[torch.Tensor] = None, dqkv: Optional[torch.Tensor] = None,
                        dbias: Optional[torch.Tensor] = None, want_dbias: bool = True, workspace: Optional[torch.Tensor] = None):
-    """Backward of bias_attention_fwd.  Returns (dqkv bf16, dbias fp32 [H, N, N] = the bias gradient summed over the batch, or None with
-    want_dbias=False).  savit_bias_attention_bwd."""
-    ld, ldb = _bias_attn_args(qkv, bias, B, N, H, head_dim, lens)
+    """Backward of bias_attention_fwd.  Returns (dqkv bf16 with qkv's row pitch, dbias fp32 [H, N, N] = the bias gradient summed over the batch, or None
+    with want_dbias=False).  savit_bias_attention_bwd."""
+    dev = _dev(qkv)
     d = H * head_dim
-    _chk(d_o, bf16, "d_o", 2)
-    _chk(lse, f32, "lse")
-    if tuple(d_o.shape) != (B * N, d) or not d_o.is_contiguous() or lse.numel() != B * H * N or not lse.is_contiguous():
-        raise ValueError("bias_attention_bwd: d_o contiguous [B*N, d], lse [B, H, N]")
+    ld = _packed(qkv, bf16, B * N, 3 * d, "qkv", dev)
+    ldb = _bias_ld(bias, H, N, "bias", dev)
+    _whole(d_o, bf16, (B * N, d), "d_o", dev)
+    _whole(lse, f32, (B, H, N), "lse", dev)
+    if lens is not None:
+        _whole(lens, torch.int32, (B,), "lens", dev)
     if dqkv is None:
-        dqkv = torch.empty((B * N, 3 * d) if ld == 3 * d else (B * N, ld), dtype=bf16, device=qkv.device)
-    _chk(dqkv, bf16, "dqkv", 2)
-    r2, c2, ld2 = _rows2d(dqkv, "dqkv")
-    if r2 < B * N or c2 < 3 * d or (ld2 != ld and B * N > 1):
-        raise ValueError("dqkv must have qkv's shape and row stride")
-    if want_dbias:
-        if dbias is None:
-            dbias = torch.empty((H, N, ldb), dtype=f32, device=qkv.device)[:, :, :N]
-        if _bias_ld(dbias, H, N, "dbias") != ldb:
-            raise ValueError("dbias must have bias's row pitch")
-        if B == 0:
-            dbias.zero_()
-    else:
+        dqkv = torch.empty((B * N, ld), dtype=bf16, device=qkv.device)
+    elif _packed(dqkv, bf16, B * N, 3 * d, "dqkv", dev) != ld and B * N > 1:
+        raise ValueError("dqkv must have qkv's row stride")
+    if not want_dbias:
         dbias = None
+    elif dbias is None:
+        dbias = torch.empty((H, N, ldb), dtype=f32, device=qkv.device)
+        if ldb != N:
+            dbias = dbias[:, :, :N]
+    elif _bias_ld(dbias, H, N, "dbias", dev) != ldb:
+        raise ValueError("dbias must have bias's row pitch")
     if B == 0:
-        return dqkv, dbias
+        return dqkv, None if dbias is None else dbias.zero_()
     L = _lib.load()
-    need = L.savit_bias_attention_bwd_workspace_bytes(B, N, H, ldb, int(want_dbias))
-    if workspace is None:
-        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=qkv.device)
-    _here(qkv, bias, d_o, lse, lens, dqkv, dbias, workspace)
-    _lib.check(L.savit_bias_attention_bwd(_p(qkv), _p(bias), _p(lens), _p(d_o), _p(lse), _p(dqkv), _p(dbias), B, N, H, head_dim, ld, ldb, float(dq_scale),
-                                          _p(workspace), workspace.numel() * workspace.element_size(), _stream()), "savit_bias_attention_bwd")
+    ws, n = _scratch(workspace, L.savit_bias_attention_bwd_workspace_bytes(B, N, H, ldb, want_dbias), qkv.device, dev)
+    _lib.check(L.savit_bias_attention_bwd(qkv.data_ptr(), bias.data_ptr(), _p(lens), d_o.data_ptr(), lse.data_ptr(), dqkv.data_ptr(), _p(dbias), B, N, H, head_dim,
+                                          ld, ldb, dq_scale, ws.data_ptr(), n, _stream()), "savit_bias_attention_bwd")
     return dqkv, dbias
 
 
@@ -1148,43 +1158,36 @@ def distill_xent(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     true probabilities, the rest spread evenly over the other classes.  logits fp32 / bf16 [R, C]; dlogits (optional, fp32 / bf16, may be logits
     itself) receives grad_scale (1 / R by default) times the gradient; dbias [C] accumulates its column sums.  Returns loss_rows [R].
     savit_distill_xent."""
-    if logits.dtype not in (bf16, f32):
+    dev = _dev(logits)
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (bf16, f32):
         raise ValueError("logits: bf16 or fp32")
-    _chk(logits, logits.dtype, "logits", 2)
-    R, C, ld = _rows2d(logits, "logits")
-    _chk(teacher_logits, f32, "teacher_logits", 2)
-    _chk(teacher_index, torch.int32, "teacher_index", 2)
-    K = teacher_logits.shape[1]
-    if tuple(teacher_logits.shape) != (R, K) or tuple(teacher_index.shape) != (R, K) or not teacher_logits.is_contiguous() or not teacher_index.is_contiguous():
-        raise ValueError("teacher_logits and teacher_index: contiguous [R, K]")
+    ld = _packed(logits, logits.dtype, 0, 1, "logits", dev)
+    R, C = logits.shape
+    K = teacher_logits.shape[-1]
+    _whole(teacher_logits, f32, (R, K), "teacher_logits", dev)
+    _whole(teacher_index, torch.int32, (R, K), "teacher_index", dev)
     if labels is not None:
-        _chk(labels, torch.int32, "labels", 1)
-        if labels.numel() != R:
-            raise ValueError("labels: one per row")
+        _whole(labels, torch.int32, (R,), "labels", dev)
     elif hard_weight != 0.0:
         raise ValueError("hard_weight needs labels")
     ld_dz = 0
     if dlogits is not None:
         if dlogits.dtype not in (bf16, f32):
             raise ValueError("dlogits: bf16 or fp32")
-        _chk(dlogits, dlogits.dtype, "dlogits", 2)
-        r, c, ld_dz = _rows2d(dlogits, "dlogits")
-        if r != R or c < C:
-            raise ValueError("dlogits too small")
-        if dlogits.data_ptr() == logits.data_ptr() and R * C and (dlogits.dtype != logits.dtype or ld_dz != ld):
+        ld_dz = _packed(dlogits, dlogits.dtype, R, C, "dlogits", dev)
+        if dlogits.data_ptr() == logits.data_ptr() and (dlogits.dtype is not logits.dtype or ld_dz != ld):
             raise ValueError("dlogits in logits' place needs its dtype and row stride")
-    loss_rows = loss_rows if loss_rows is not None else torch.empty((R,), dtype=f32, device=logits.device)
-    for name, t, n in (("teacher_lse", teacher_lse, R), ("row_weight", row_weight, R), ("loss_rows", loss_rows, R), ("dbias", dbias, C)):
+    if loss_rows is None:
+        loss_rows = torch.empty((R,), dtype=f32, device=logits.device)
+    else:
+        _whole(loss_rows, f32, (R,), "loss_rows", dev)
+    for name, t, n in (("teacher_lse", teacher_lse, R), ("row_weight", row_weight, R), ("dbias", dbias, C)):
         if t is not None:
-            _chk(t, f32, name, 1)
-            if t.numel() != n:
-                raise ValueError(f"{name}: {n} elements")
-    gs = (1.0 / max(R, 1)) if grad_scale is None else float(grad_scale)
-    _here(logits, teacher_logits, teacher_index, teacher_lse, labels, row_weight, loss_rows, dlogits, dbias)
+            _whole(t, f32, (n,), name, dev)
     if R == 0:
         return loss_rows
-    _lib.check(_lib.load().savit_distill_xent(_p(logits), ld, int(logits.dtype == bf16), _p(teacher_logits), _p(teacher_index), K, _p(teacher_lse),
-                                              _p(labels), _p(row_weight), float(temperature), float(distill_weight), float(hard_weight),
-                                              float(label_smoothing), gs, _p(loss_rows), _p(dlogits), ld_dz,
-                                              int(dlogits is not None and dlogits.dtype == bf16), _p(dbias), R, C, _stream()), "savit_distill_xent")
+    _lib.check(_lib.load().savit_distill_xent(logits.data_ptr(), ld, logits.dtype is bf16, _p(teacher_logits) or None, _p(teacher_index) or None, K,
+                                              _p(teacher_lse), _p(labels), _p(row_weight), temperature, distill_weight, hard_weight, label_smoothing,
+                                              1.0 / R if grad_scale is None else grad_scale, loss_rows.data_ptr(), _p(dlogits), ld_dz,
+                                              dlogits is not None and dlogits.dtype is bf16, _p(dbias), R, C, _stream()), "savit_distill_xent")
     return loss_rows
