@@ -16,6 +16,8 @@
 // The bias gradient is a kernel of its own: a workgroup keeps one [queries x 64 keys] tile of one head in registers and walks over the
 // images, so the sum over the batch is in a fixed order and touches memory once; long batches are cut into parts that a last launch adds.  It
 // recomputes two products; a sum by atomics would move N^2 values per image and head through memory and repeat in no fixed order.
+#include <type_traits>
+
 #include "attn_tiles.h"
 #include "common.h"
 #include "savit.h"
@@ -36,7 +38,8 @@ struct BiasAttnParams {
   float* stat;         // backward: [B, H, 2, Np]: -lse log2 e (-inf where the query takes no part), delta
   float* dbias;        // [H, N, ldb], or the slab [parts][H, N, ldb]
   int B, N, H, ld, d, ldb, Np;
-  int blocks;          // query (key) blocks of W * 32 rows
+  int hd;
+  int blocks;          // query (key) blocks of a sequence
   int key_blocks, parts;
   float dq_scale;
 };
@@ -44,10 +47,12 @@ struct BiasAttnParams {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, size_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (uint32_t)bytes, 0x00020000);
 }
-constexpr uint32_t OUTSIDE = 0xfffffff0u;  // beyond every descriptor's range: loads return zero
+constexpr uint32_t OUTSIDE = 0xfffffff0u;  // beyond every descriptor's range (below 0xfff00000): loads return zero
+constexpr uint32_t BEYOND = 0xfff00000u;   // the same for an offset that something below 1 MB is still added to
 
-__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) { return __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0); }
-__device__ __forceinline__ f32x4 load4f(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) { return __builtin_bit_cast(f32x4, load16(r, voff, soff)); }
+// (the scalar offset of these loads takes no part in the range check: it is always 0 here)
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+__device__ __forceinline__ f32x4 load4f(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_bit_cast(f32x4, load16(r, off)); }
 
 __device__ __forceinline__ int length_of(const BiasAttnParams& p, int b) {
   if (p.lens == nullptr) return p.N;
@@ -67,8 +72,8 @@ struct Segment {
     for (int k = 0; k < LOADS; ++k) {
       const int i = threadIdx.x + k * 64 * W, t = row0 + (i >> 3), c = i & 7;
       const bool in = t < len && c < 2 * KS;
-      a[k] = load16(ra, in ? (uint32_t)t * lda2 + col_a2 + 16 * c : OUTSIDE, 0);
-      b[k] = load16(rb, in ? (uint32_t)t * ldb2 + col_b2 + 16 * c : OUTSIDE, 0);
+      a[k] = load16(ra, in ? (uint32_t)t * lda2 + col_a2 + 16 * c : OUTSIDE);
+      b[k] = load16(rb, in ? (uint32_t)t * ldb2 + col_b2 + 16 * c : OUTSIDE);
     }
   }
   __device__ __forceinline__ void put(char* img) const {
@@ -95,11 +100,11 @@ struct Lane {
   __device__ __forceinline__ int reg(int r) const { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 };
 
-// bias of a transposed tile: query on the lane (row offset in voff), keys k0 .. k0 + 31 in registers
-__device__ __forceinline__ void load_bias_t(f32x16& s, __amdgpu_buffer_rsrc_t r, uint32_t voff, int k0, int N) {
+// bias of a transposed tile: query on the lane (voff: its row; BEYOND: none), keys k0 .. k0 + 31 in registers
+__device__ __forceinline__ void load_bias_t(f32x16& s, __amdgpu_buffer_rsrc_t r, uint32_t voff, int k0) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const f32x4 v = load4f(r, voff, (uint32_t)(k0 + 8 * g) * 4);
+    const f32x4 v = load4f(r, voff + (uint32_t)(k0 + 8 * g) * 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[4 * g + i] = v[i];
   }
@@ -135,6 +140,13 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// keys k0 + .. of a transposed tile that lie at or beyond len get v
+__device__ __forceinline__ void mask_keys(f32x16& s, int k0, int len, const Lane& L, float v) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (k0 + L.reg(r) >= len) s[r] = v;
+}
+
 // workgroup -> (head, image, block): all blocks and images of a head in a row, and consecutive numbers on one XCD, so that its L2 holds the
 // head's bias for every image
 __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b, int& blk) {
@@ -146,7 +158,7 @@ __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b,
 }
 
 template <int W, int KS>
-__global__ __launch_bounds__(64 * W) void bias_attn_fwd_kernel(const BiasAttnParams p) {
+__global__ __launch_bounds__(64 * W, 3) void bias_attn_fwd_kernel(const BiasAttnParams p) {
   typedef Segment<W, KS> Seg;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
   constexpr int hd = 16 * KS;
@@ -160,7 +172,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_fwd_kernel(const BiasAttnPar
   const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
   const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
-  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : OUTSIDE;
+  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : BEYOND;
   const uint32_t ck = (uint32_t)(p.d + h * hd) * 2, cv = ck + (uint32_t)p.d * 2;
   const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;  // a block beyond the sequence only clears its rows
   Seg sg;
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_fwd_kernel(const BiasAttnPar
     sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, 0, len);
     load_frags<KS>(qf, img, q, p.ld, h * hd, L.half, ok);
     f32x16 next;
-    load_bias_t(next, rb, boff, 0, p.N);
+    load_bias_t(next, rb, boff, 0);
     sg.put(smem);
     __syncthreads();
     for (int s = 0; s < nseg; ++s) {
@@ -184,13 +196,9 @@ __global__ __launch_bounds__(64 * W) void bias_attn_fwd_kernel(const BiasAttnPar
         const int k0 = s * Seg::SEG + 32 * t;
         if (k0 >= len) break;
         f32x16 sc = next;
-        load_bias_t(next, rb, boff, k0 + 32, p.N);
+        load_bias_t(next, rb, boff, k0 + 32);
         tile_product<KS>(sc, imgK, 32 * t + L.ql, qf, L.half);
-        if (k0 + 32 > len) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (k0 + L.reg(r) >= len) sc[r] = -INFINITY;
-        }
+        if (k0 + 32 > len) mask_keys(sc, k0, len, L, -INFINITY);
         float top = sc[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
@@ -231,7 +239,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_fwd_kernel(const BiasAttnPar
 
 // dQ, and the statistics the other two kernels read.  Two loops over the keys: delta, then dQ.
 template <int W, int KS>
-__global__ __launch_bounds__(64 * W) void bias_attn_dq_kernel(const BiasAttnParams p) {
+__global__ __launch_bounds__(64 * W, 2) void bias_attn_dq_kernel(const BiasAttnParams p) {
   typedef Segment<W, KS> Seg;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
   constexpr int hd = 16 * KS;
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dq_kernel(const BiasAttnPara
   const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
   const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
-  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : OUTSIDE;
+  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : BEYOND;
   const uint32_t ck = (uint32_t)(p.d + h * hd) * 2, cv = ck + (uint32_t)p.d * 2;
   const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
   float nl = -INFINITY, delta = 0.f;
@@ -253,6 +261,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dq_kernel(const BiasAttnPara
     const float v = p.lse[((size_t)b * p.H + h) * p.N + q];
     nl = v == -INFINITY ? -INFINITY : -LOG2E_F * v;
   }
+  constexpr int T = Seg::SEG / 32;
   Seg sg;
   f32x16 dq[2] = {zero16(), zero16()};
   if (nseg > 0) {
@@ -260,41 +269,56 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dq_kernel(const BiasAttnPara
     sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, 0, len);
     load_frags<KS>(qf, img, q, p.ld, h * hd, L.half, ok);
     load_frags<KS>(df, p.d_o, (size_t)b * p.N + q, p.d, h * hd, L.half, ok);
-    f32x16 next;
-    load_bias_t(next, rb, boff, 0, p.N);
+    f32x16 next[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_bias_t(next[t], rb, boff, 32 * t);
     sg.put(smem);
     __syncthreads();
     for (int s2 = 0; s2 < 2 * nseg; ++s2) {
       const bool second = s2 >= nseg, more = s2 + 1 < 2 * nseg;
-      const int s = second ? s2 - nseg : s2, sn = s + 1 < nseg ? s + 1 : 0;
-      if (more) sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, sn * Seg::SEG, len);
+      const int k0 = (second ? s2 - nseg : s2) * Seg::SEG, kn = k0 + Seg::SEG < len ? k0 + Seg::SEG : 0;
+      if (more) sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, kn, len);
       if (s2 == nseg) delta = half_sum(delta);
       const char* imgK = smem + (s2 & 1) * 2 * Seg::IMG;
       const char* imgV = imgK + Seg::IMG;
+      auto tiles = [&](auto count) {
+        constexpr int M = decltype(count)::value;
+        f32x16 sc[M], dp[M];
 #pragma unroll
-      for (int t = 0; t < Seg::SEG / 32; ++t) {
-        const int k0 = s * Seg::SEG + 32 * t;
-        if (k0 >= len) break;
-        f32x16 sc = next;
-        load_bias_t(next, rb, boff, k0 + 32 < len ? k0 + 32 : 0, p.N);
-        f32x16 dp = zero16();
-        tile_product<KS>(sc, imgK, 32 * t + L.ql, qf, L.half);
-        tile_product<KS>(dp, imgV, 32 * t + L.ql, df, L.half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, nl));
-          if (k0 + 32 > len && k0 + L.reg(r) >= len) pr = 0.f;
-          sc[r] = pr;
+        for (int t = 0; t < M; ++t) {
+          sc[t] = next[t];
+          dp[t] = zero16();
         }
+        if (more) {
+#pragma unroll
+          for (int t = 0; t < T; ++t) load_bias_t(next[t], rb, boff, kn + 32 * t);
+        }
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+          tile_product<KS>(sc[t], imgK, 32 * t + L.ql, qf, L.half);
+          tile_product<KS>(dp[t], imgV, 32 * t + L.ql, df, L.half);
+        }
+#pragma unroll
+        for (int t = 0; t < M; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+        if (k0 + 32 * M > len) mask_keys(sc[M - 1], k0 + 32 * (M - 1), len, L, 0.f);
         if (!second) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) delta += sc[r] * dp[r];
+          for (int t = 0; t < M; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) delta += sc[t][r] * dp[t][r];
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[r] *= dp[r] - delta;
-          tile_accumulate<KS>(dq, imgK, 32 * t, sc, L);
+          for (int t = 0; t < M; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[t][r] *= dp[t][r] - delta;
+            tile_accumulate<KS>(dq, imgK, 32 * t, sc[t], L);
+          }
         }
-      }
+      };
+      if (T == 2 && k0 + 32 < len) tiles(std::integral_constant<int, T>{});
+      else tiles(std::integral_constant<int, 1>{});
       if (more) {
         sg.put(smem + ((s2 + 1) & 1) * 2 * Seg::IMG);
         __syncthreads();
@@ -314,7 +338,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dq_kernel(const BiasAttnPara
 
 // dK and dV: key on the lane, queries in registers
 template <int W, int KS>
-__global__ __launch_bounds__(64 * W) void bias_attn_dkv_kernel(const BiasAttnParams p) {
+__global__ __launch_bounds__(64 * W, 2) void bias_attn_dkv_kernel(const BiasAttnParams p) {
   typedef Segment<W, KS> Seg;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
   constexpr int hd = 16 * KS;
@@ -332,7 +356,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dkv_kernel(const BiasAttnPar
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
   const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
   const uint32_t cq = (uint32_t)(h * hd) * 2;
-  const uint32_t boff = ok ? (uint32_t)(4 * L.half * p.ldb + key) * 4 : OUTSIDE;
+  const uint32_t boff = (uint32_t)(4 * L.half * p.ldb + key) * 4;
   const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
   Seg sg;
   f32x16 dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
@@ -345,7 +369,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dkv_kernel(const BiasAttnPar
     auto load_bias = [&](int q0) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        next[r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, boff, (uint32_t)((q0 + (r & 3) + 8 * (r >> 2)) * p.ldb) * 4, 0));
+        next[r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, boff + (uint32_t)((q0 + (r & 3) + 8 * (r >> 2)) * p.ldb) * 4, 0, 0));
     };
     load_bias(0);
     sg.put(smem);
@@ -362,8 +386,8 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dkv_kernel(const BiasAttnPar
         f32x4 nl[4], dl[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          nl[g] = load4f(rt, (uint32_t)(4 * L.half) * 4, (uint32_t)(q0 + 8 * g) * 4);
-          dl[g] = load4f(rt, (uint32_t)(4 * L.half) * 4, (uint32_t)(p.Np + q0 + 8 * g) * 4);
+          nl[g] = load4f(rt, (uint32_t)(4 * L.half + q0 + 8 * g) * 4);
+          dl[g] = load4f(rt, (uint32_t)(4 * L.half + p.Np + q0 + 8 * g) * 4);
         }
         f32x16 sc = next;
         load_bias(q0 + 32);
@@ -394,7 +418,7 @@ __global__ __launch_bounds__(64 * W) void bias_attn_dkv_kernel(const BiasAttnPar
 
 // dbias of a tile of 32 W queries x SEG keys of one head, summed over the images of a part
 template <int W, int KS>
-__global__ __launch_bounds__(64 * W) void bias_attn_db_kernel(const BiasAttnParams p) {
+__global__ __launch_bounds__(64 * W, 2) void bias_attn_db_kernel(const BiasAttnParams p) {
   typedef Segment<W, KS> Seg;
   constexpr int T = Seg::SEG / 32;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
@@ -414,13 +438,21 @@ __global__ __launch_bounds__(64 * W) void bias_attn_db_kernel(const BiasAttnPara
   f32x16 bias[T], acc[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    load_bias_t(bias[t], rb, q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : OUTSIDE, k0 + 32 * t, p.N);
+    load_bias_t(bias[t], rb, q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : BEYOND, k0 + 32 * t);
     acc[t] = zero16();
   }
   Seg sg;
-  auto fetch = [&](int b) {
+  bf16x8 qn[KS], dn[KS];
+  float nln, deltan;
+  auto fetch = [&](int b) {  // an image's operands, one image ahead
+    const int len = length_of(p, b);
     const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)p.N * p.ld * 2);
-    sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, k0, length_of(p, b));
+    sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, k0, len);
+    load_frags<KS>(qn, p.qkv, (size_t)b * p.N + q, p.ld, h * hd, L.half, q < len);
+    load_frags<KS>(dn, p.d_o, (size_t)b * p.N + q, p.d, h * hd, L.half, q < len);
+    const float* st = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + q;
+    nln = q < len ? st[0] : -INFINITY;
+    deltan = q < len ? st[p.Np] : 0.f;
   };
   if (b0 < b1) {
     fetch(b0);
@@ -431,24 +463,30 @@ __global__ __launch_bounds__(64 * W) void bias_attn_db_kernel(const BiasAttnPara
     const bool more = b + 1 < b1;
     const int len = length_of(p, b);
     bf16x8 qf[KS], df[KS];
-    load_frags<KS>(qf, p.qkv, (size_t)b * p.N + q, p.ld, h * hd, L.half, q < len);
-    load_frags<KS>(df, p.d_o, (size_t)b * p.N + q, p.d, h * hd, L.half, q < len);
-    const float* st = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + q;
-    const float nl = q < len ? st[0] : -INFINITY, delta = q < len ? st[p.Np] : 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = qn[ks];
+      df[ks] = dn[ks];
+    }
+    const float nl = nln, delta = deltan;
     if (more) fetch(b + 1);
     const char* imgK = smem + ((b - b0) & 1) * 2 * Seg::IMG;
     const char* imgV = imgK + Seg::IMG;
+    f32x16 sc[T], dp[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      f32x16 sc = bias[t], dp = zero16();
-      tile_product<KS>(sc, imgK, 32 * t + L.ql, qf, L.half);
-      tile_product<KS>(dp, imgV, 32 * t + L.ql, df, L.half);
-      const bool edge = k0 + 32 * t + 32 > len;
+      sc[t] = bias[t];
+      dp[t] = zero16();
+      tile_product<KS>(sc[t], imgK, 32 * t + L.ql, qf, L.half);
+      tile_product<KS>(dp[t], imgV, 32 * t + L.ql, df, L.half);
+    }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, nl)) * (dp[r] - delta);
-        acc[t][r] += edge && k0 + 32 * t + L.reg(r) >= len ? 0.f : ds;
-      }
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl)) * (dp[t][r] - delta);
+      if (k0 + 32 * t + 32 > len) mask_keys(sc[t], k0 + 32 * t, len, L, 0.f);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] += sc[t][r];
     }
     if (more) {
       sg.put(smem + ((b - b0 + 1) & 1) * 2 * Seg::IMG);
@@ -466,37 +504,253 @@ __global__ __launch_bounds__(64 * W) void bias_attn_db_kernel(const BiasAttnPara
   }
 }
 
-// out = sum of the parts, in order: 64 16-byte columns a block, four strips of parts
+// ------------------------------------------------------------------------------------------ dQ and dbias, short sequences (N <= 16 KT, KT <= 14)
+// A workgroup holds all keys of an (image, head) in LDS; a wave owns 16 queries (v_mfma_f32_16x16x32), so that P and dP of ALL keys (8 KT registers)
+// stay in registers between delta and dS - no score is computed twice - and the wave's dS, added up over the images, too (4 KT): the
+// bias gradient costs 4 additions a tile instead of a kernel that computes dS again.  32 queries a wave would need 512 registers for this.
+// Persistent over the images of one head, with two K / V image pairs: the next image's rows are fetched into registers (in groups where they are many) while this one is
+// computed, and put into the other pair half an image later; the only barrier is the one between images.  The score tiles are independent
+// accumulators: every LDS and MFMA latency is covered by the other tiles of the same wave.
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// rows row0 .. row0 + 3 and row0 + 16 .. + 19 (row0 = 4 (lane / 16)) of columns col0 .. + 15: A operand whose k order is that of two stacked 16 x 16
+// accumulators
+__device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
+  const int o = img_off(row, col >> 3) + ((col & 7) << 1);  // (16 rows on: the same swizzle)
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o + 16 * ROWB));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// sum over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float quarters_sum(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  return half_sum(a + b);
+}
+
+template <int KT, int KS2, bool DB>
+__global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_kernel(const BiasAttnParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int IMG = KT * 16 * ROWB, PIECES = KT * 16 * 8 * 2, RES_GROUPS = KT <= 6 ? 1 : KT <= 8 ? 2 : 4;
+  constexpr bool AHEAD = KT <= 8;  // the next image's bias and queries ahead too: longer rows leave no registers for them (14 tiles: 93 spills, twice the time)
+  const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int t0 = xcd_remap(blockIdx.x, gridDim.x);
+  const int part = t0 % p.parts;
+  t0 /= p.parts;
+  const int blk = t0 % p.blocks, h = t0 / p.blocks;
+  const int b0 = (int)((long)p.B * part / p.parts), b1 = (int)((long)p.B * (part + 1) / p.parts);
+  const int q = (blk * (int)(blockDim.x >> 6) + wave) * 16 + ql;
+  const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
+  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * g) * 4 : BEYOND;
+  const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, hcol = (uint32_t)(h * p.hd) * 2;
+
+  // the next image's K and V rows: PIECES 16-byte pieces in RES_GROUPS groups ; rows at and beyond its length are out of the descriptor's range (zero),
+  // columns at and beyond hd repeat others (they meet zeros of the query fragments, or output rows that are not stored)
+  constexpr int LEAST = 64 * (KT <= 8 ? KT - 1 : KT / 2), MAXL = (PIECES / RES_GROUPS + LEAST - 1) / LEAST;  // threads, pieces a thread and group
+  u32x4 st[MAXL];
+  const int chunks = p.hd / 8;
+  auto fetch = [&](__amdgpu_buffer_rsrc_t rs, int grp) {
+#pragma unroll
+    for (int k = 0; k < MAXL; ++k) {
+      const int u = grp * (PIECES / RES_GROUPS) + threadIdx.x + k * blockDim.x;
+      const int t = (u >> 4), c = (u & 7) < chunks ? (u & 7) : 0;
+      const bool in = threadIdx.x + k * blockDim.x < PIECES / RES_GROUPS;
+      st[k] = load16(rs, in ? (uint32_t)t * ld2 + ((u & 8) ? 2 * d2 : d2) + hcol + 16 * c : OUTSIDE);
+    }
+  };
+  auto put = [&](int grp, int buf) {
+#pragma unroll
+    for (int k = 0; k < MAXL; ++k) {
+      const int u = grp * (PIECES / RES_GROUPS) + threadIdx.x + k * blockDim.x;
+      if (threadIdx.x + k * blockDim.x < PIECES / RES_GROUPS)
+        *reinterpret_cast<u32x4*>(smem + buf * 2 * IMG + ((u & 8) ? IMG : 0) + img_off(u >> 4, u & 7)) = st[k];
+    }
+  };
+  auto image = [&](int b, int len) { return rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2); };
+  bf16x8 qf[KS2], df[KS2];
+  float lse;
+  auto load_queries = [&](int b, int len) {
+    const auto rs = image(b, len), rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2), rl = rsrc_of(p.lse + ((size_t)b * p.H + h) * p.N, (size_t)len * 4);
+#pragma unroll
+    for (int ks = 0; ks < KS2; ++ks) {
+      const int c = 32 * ks + 8 * g;
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
+      df[ks] = __builtin_bit_cast(bf16x8, load16(rd, c < p.hd ? (uint32_t)q * d2 + hcol + 2 * c : OUTSIDE));
+    }
+    lse = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rl, (uint32_t)q * 4, 0, 0));
+  };
+
+  f32x4 acc[DB ? KT : 1];
+  if constexpr (DB) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int len = length_of(p, b0);
+  {
+    const auto rs = image(b0, len);
+    for (int i = 0; i < RES_GROUPS; ++i) {
+      fetch(rs, i);
+      put(i, 0);
+    }
+  }
+  load_queries(b0, len);
+  f32x4 sc[KT], dp[KT];
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) sc[t] = load4f(rb, boff + 64 * t);
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int buf = (b - b0) & 1, bn = b + 1 < b1 ? b + 1 : b, lenn = length_of(p, bn);  // (the last image fetches itself again)
+    const auto rn = image(bn, lenn);
+    const char* imgK = smem + buf * 2 * IMG;
+    const char* imgV = imgK + IMG;
+    if constexpr (!AHEAD) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) sc[t] = load4f(rb, boff + 64 * t);
+    }
+    __syncthreads();  // this image's rows are there, and everybody is done with the other pair
+    fetch(rn, 0);
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS2; ++ks) {
+        sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+        dp[t] = mfma16(lds_row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
+      }
+    }
+    const float nl = q < len && lse != -INFINITY ? -LOG2E_F * lse : -INFINITY;
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+      if (16 * t + 16 > len) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * t + 4 * g + r >= len) sc[t][r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) d[r] += sc[t][r] * dp[t][r];
+    }
+    const float delta = quarters_sum((d[0] + d[1]) + (d[2] + d[3]));
+    if constexpr (RES_GROUPS >= 2) {
+      put(0, buf ^ 1);
+      fetch(rn, 1);
+    }
+    f32x4 dq[2 * KS2];
+#pragma unroll
+    for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < KT; t += 2) {
+      union { uint32_t u[4]; bf16x8 v; } f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sc[t + k][r] *= dp[t + k][r] - delta;
+          if constexpr (DB) acc[t + k][r] += sc[t + k][r];
+        }
+        f.u[2 * k] = pack_bf16x2(sc[t + k][0], sc[t + k][1]);
+        f.u[2 * k + 1] = pack_bf16x2(sc[t + k][2], sc[t + k][3]);
+      }
+#pragma unroll
+      for (int eb = 0; eb < 2 * KS2; ++eb)
+        dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), f.v, dq[eb]);
+      if constexpr (RES_GROUPS == 4) {
+        if (t == KT / 6 * 2) { put(1, buf ^ 1); fetch(rn, 2); }
+        if (t == KT / 6 * 4) { put(2, buf ^ 1); fetch(rn, 3); }
+      }
+      if constexpr (AHEAD) {  // into registers that have just become free
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sc[t + k] = load4f(rb, boff + 64 * (t + k));
+        if (t == KT / 4 * 2) load_queries(bn, lenn);
+      }
+    }
+    if (q < p.N) {
+      bf16_t* row = p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd + 4 * g;
+#pragma unroll
+      for (int eb = 0; eb < 2 * KS2; ++eb)
+        if (16 * eb < p.hd)
+          *reinterpret_cast<uint2*>(row + 16 * eb) = make_uint2(pack_bf16x2(dq[eb][0] * p.dq_scale, dq[eb][1] * p.dq_scale),
+                                                                pack_bf16x2(dq[eb][2] * p.dq_scale, dq[eb][3] * p.dq_scale));
+    }
+    {  // statistics of the queries, and of the padding up to Np (fewer than three times the rows here) that the dK / dV kernel's tiles read
+      const int row = q + g * (int)(blockDim.x >> 6) * 16 * p.blocks;
+      if (row < p.Np) {
+        float* s = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + row;
+        s[0] = g == 0 ? nl : -INFINITY;
+        s[p.Np] = g == 0 ? delta : 0.f;
+      }
+    }
+    put(RES_GROUPS - 1, buf ^ 1);
+    if constexpr (!AHEAD) load_queries(bn, lenn);
+    len = lenn;
+  }
+  if constexpr (DB) {
+    if (q < p.N) {
+      float* out = p.dbias + (((size_t)part * p.H + h) * p.N + q) * p.ldb + 4 * g;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+        if (16 * t + 4 * g < p.N) *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
+    }
+  }
+}
+
+// out = sum of the parts: 16 16-byte columns a block, 16 strips of parts, fixed order
 __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __restrict__ slab, float* __restrict__ out, long n4, int parts) {
-  __shared__ f32x4 red[4][64];
-  const int c = threadIdx.x & 63, strip = threadIdx.x >> 6;
-  const long i = (long)blockIdx.x * 64 + c;
+  __shared__ f32x4 red[16][16];
+  const int c = threadIdx.x & 15, strip = threadIdx.x >> 4;
+  const long i = (long)blockIdx.x * 16 + c;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (i < n4) {
 #pragma unroll 4
-    for (int k = strip; k < parts; k += 4) s += reinterpret_cast<const f32x4*>(slab)[(size_t)k * n4 + i];
+    for (int k = strip; k < parts; k += 16) s += reinterpret_cast<const f32x4*>(slab)[(size_t)k * n4 + i];
   }
   red[strip][c] = s;
   __syncthreads();
-  if (strip == 0 && i < n4) reinterpret_cast<f32x4*>(out)[i] = s + red[1][c] + red[2][c] + red[3][c];
+  if (strip == 0 && i < n4) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][c];
+    reinterpret_cast<f32x4*>(out)[i] = s;
+  }
 }
 
 int waves_of(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : 4; }
 int padded(int N) { return (N + 63) / 64 * 64; }
 
-// parts of the batch in the dbias kernel: about four workgroups a CU, no more than there are images
-int parts_of(int B, int N, int H) {
-  const int W = waves_of(N);
-  const long tiles = (long)H * ((N + 32 * W - 1) / (32 * W)) * ((N + (W == 1 ? 31 : 63)) / (W == 1 ? 32 : 64));
-  const long want = 1024 * (4 / W) / tiles;
-  return (int)(want < 1 ? 1 : want > B ? (B > 0 ? B : 1) : want);
+// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel
+constexpr int RESIDENT_N = 224;
+bool resident(int N) { return N <= RESIDENT_N; }
+constexpr int CUS = 256;  // not the device's or a budget's: the parts set the order of the bias gradient's sum
+
+int clamp_parts(long want, int B) { return (int)(want < 1 ? 1 : want > B ? (B > 0 ? B : 1) : want); }
+// waves of the resident kernel: one a 16 queries, two workgroups a sequence beyond eight
+int resident_waves(int N) {
+  const int nq = (N + 15) / 16;
+  return nq > 8 ? (nq + 1) / 2 : nq;
 }
+int resident_blocks(int N) { return (N + 15) / 16 > 8 ? 2 : 1; }
+// parts of the batch, a workgroup each: the persistent kernel's fill the chip once (160 KB of LDS a CU; 8, 12 or 16 waves by its registers) ...
+int resident_parts(int B, int N, int H) {
+  const int kt = (N + 31) / 32 * 2, W = resident_waves(N);
+  int per_cu = (kt <= 4 ? 16 : kt <= 8 ? 12 : 8) / W;
+  if (per_cu > 160 / (8 * kt)) per_cu = 160 / (8 * kt);
+  return clamp_parts((long)CUS * (per_cu < 1 ? 1 : per_cu) / ((long)H * resident_blocks(N)), B);
+}
+// ... the dbias kernel's are about four workgroups a CU
+int db_parts(int B, int N, int H) {
+  const long tiles = (long)H * ((N + 127) / 128) * ((N + 63) / 64);
+  return clamp_parts(4L * CUS / tiles, B);
+}
+int dbias_parts(int B, int N, int H) { return resident(N) ? resident_parts(B, N, H) : db_parts(B, N, H); }
 
 bool size_ok(int B, int N, int H, int hd, int ld, int ldb) {
   if (!(B >= 0 && N > 0 && N <= 32768 && H > 0 && (hd == 16 || hd == 32 || hd == 48 || hd == 64))) return false;
   if (!(ld >= 3L * H * hd && ld % 8 == 0 && ldb >= N && ldb % 4 == 0)) return false;
   // 32-bit offsets inside one image's rows and one head's bias
-  if ((long)(N + 64) * ld * 2 >= 0xfffffff0L || (long)(N + 64) * ldb * 4 >= 0xfffffff0L) return false;
+  if ((long)(N + 128) * ld * 2 >= 0xfff00000L || (long)(N + 128) * ldb * 4 >= 0xfff00000L) return false;
   return (long)B * H * ((N + 31) / 32) <= 0x7fffffffL;
 }
 bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
@@ -515,6 +769,30 @@ bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
     if (e_ != hipSuccess) return (int)e_;                                                                                                           \
   } while (0)
 
+template <int KT, int KS2, bool DB>
+int launch_resident_k(const BiasAttnParams& p, hipStream_t st) {
+  auto kfn = bias_attn_dq_resident_kernel<KT, KS2, DB>;
+  SAVIT_LDS_ONCE(kfn);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)(p.parts * p.H * p.blocks)), dim3(64 * resident_waves(p.N)), (size_t)4 * KT * 16 * ROWB, st, p);
+  SAVIT_LAUNCH_RET();
+}
+template <int KT>
+int launch_resident_kt(const BiasAttnParams& p, bool db, hipStream_t st) {
+  if (p.hd <= 32) return db ? launch_resident_k<KT, 1, true>(p, st) : launch_resident_k<KT, 1, false>(p, st);
+  return db ? launch_resident_k<KT, 2, true>(p, st) : launch_resident_k<KT, 2, false>(p, st);
+}
+int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
+  switch ((p.N + 31) / 32) {
+    case 1: return launch_resident_kt<2>(p, db, st);
+    case 2: return launch_resident_kt<4>(p, db, st);
+    case 3: return launch_resident_kt<6>(p, db, st);
+    case 4: return launch_resident_kt<8>(p, db, st);
+    case 5: return launch_resident_kt<10>(p, db, st);
+    case 6: return launch_resident_kt<12>(p, db, st);
+    default: return launch_resident_kt<14>(p, db, st);
+  }
+}
+
 }  // namespace
 
 extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
@@ -523,7 +801,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
   if (B == 0) return SAVIT_OK;
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.o = (bf16_t*)o; p.lse = lse;
-  p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.ldb = ld_bias;
+  p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias;
   const int W = waves_of(N);
   const hipStream_t st = (hipStream_t)stream;
   p.blocks = (N + 32 * W - 1) / (32 * W);
@@ -533,7 +811,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
 
 extern "C" long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, int ld_bias, int want_dbias) {
   if (!(B >= 0 && N > 0 && N <= 32768 && H > 0 && ld_bias >= N)) return 0;
-  const int parts = parts_of(B, N, H);
+  const int parts = dbias_parts(B, N, H);
   return (long)B * H * 2 * padded(N) * 4 + (want_dbias && parts > 1 ? (long)parts * H * N * ld_bias * 4 : 0);
 }
 
@@ -547,24 +825,36 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   SAVIT_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= savit_bias_attention_bwd_workspace_bytes(B, N, H, ld_bias, dbias != nullptr));
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.d_o = (const bf16_t*)d_o; p.lse = const_cast<float*>(lse); p.dqkv = (bf16_t*)dqkv;
-  p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.ldb = ld_bias; p.dq_scale = dq_scale;
+  p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias; p.dq_scale = dq_scale;
   p.Np = padded(N);
   p.stat = (float*)workspace;
+  const int parts = dbias_parts(B, N, H);
+  float* slab = parts == 1 ? dbias : p.stat + (size_t)B * H * 2 * p.Np;
+  p.parts = parts;
+  p.dbias = slab;
+  if (resident(N)) {
+    p.blocks = resident_blocks(N);
+    const int rc = launch_resident(p, dbias != nullptr, st);
+    if (rc != SAVIT_OK) return rc;
+  } else {
+    constexpr int W = 4;
+    p.blocks = (N + 127) / 128;
+    BIAS_ATTN_LAUNCH(bias_attn_dq_kernel, (long)B * H * p.blocks);
+  }
   const int W = waves_of(N);
   p.blocks = (N + 32 * W - 1) / (32 * W);
-  BIAS_ATTN_LAUNCH(bias_attn_dq_kernel, (long)B * H * p.blocks);
   BIAS_ATTN_LAUNCH(bias_attn_dkv_kernel, (long)B * H * p.blocks);
   if (dbias) {
-    p.parts = parts_of(B, N, H);
-    const int seg = W == 1 ? 32 : 64;
-    p.key_blocks = (N + seg - 1) / seg;
-    p.dbias = p.parts == 1 ? dbias : p.stat + (size_t)B * H * 2 * p.Np;
-    const long grid = (long)p.parts * H * p.blocks * p.key_blocks;
-    SAVIT_CHECK_ARG(grid <= 0x7fffffffL);
-    BIAS_ATTN_LAUNCH(bias_attn_db_kernel, grid);
+    if (!resident(N)) {
+      constexpr int W = 4;
+      p.key_blocks = (N + 63) / 64;
+      const long grid = (long)p.parts * H * p.blocks * p.key_blocks;
+      SAVIT_CHECK_ARG(grid <= 0x7fffffffL);
+      BIAS_ATTN_LAUNCH(bias_attn_db_kernel, grid);
+    }
     if (p.parts > 1) {
       const long n4 = (long)H * N * ld_bias / 4;
-      hipLaunchKernelGGL(bias_attn_parts_kernel, dim3((unsigned)((n4 + 63) / 64)), dim3(256), 0, st, p.dbias, dbias, n4, p.parts);
+      hipLaunchKernelGGL(bias_attn_parts_kernel, dim3((unsigned)((n4 + 15) / 16)), dim3(256), 0, st, slab, dbias, n4, p.parts);
       SAVIT_LAUNCH_RET();
     }
   }

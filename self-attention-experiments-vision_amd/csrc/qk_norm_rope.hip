@@ -22,11 +22,11 @@ struct QknParams {
   const void* x;       // raw rows (forward input, saved for backward)
   const void* g;       // backward: cotangent rows
   void* y;             // forward: output rows; backward: gradient rows
-  const float* w[2];   // query, key weights [hd]
+  const float *wq, *wk;  // query, key weights [hd]
   const float* table;  // [T, hd] cosines | sines; nullptr: no rotation
   const int* pos;      // [rows] or nullptr: row % N
   float* slab;         // backward: [gridDim.x][2 * hd] partial weight gradients
-  float* dw[2];        // backward, one block: added to directly
+  float *dwq, *dwk;    // backward, one block: added to directly
   long ldx, ldg, ldy;
   int rows, N, H, Hk, hd, T;
   int nq, nk, nv;      // chunks of HS heads in each section (nv = 0: values stay where they are)
@@ -150,10 +150,11 @@ __global__ __launch_bounds__(256) void qkn_fwd_kernel(const QknParams p) {
   float wa[8], wb[8];
   if (sec < 2 && on) {
     const float sc = sec == 0 ? p.q_scale : 1.0f;
+    const float* w = sec == 0 ? p.wq : p.wk;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      wa[i] = p.w[sec][8 * l + i] * sc;
-      wb[i] = p.w[sec][p.hd / 2 + 8 * l + i] * sc;
+      wa[i] = w[8 * l + i] * sc;
+      wb[i] = w[p.hd / 2 + 8 * l + i] * sc;
     }
   }
   for (int row = grp / chunks; row < p.rows; row += step) {
@@ -216,10 +217,10 @@ __global__ __launch_bounds__(256) void qkn_fwd_kernel(const QknParams p) {
   }
 }
 
-constexpr int QKN_BWD_THREADS = 512;
+constexpr int QKN_BWD_THREADS = 256;
 
 template <typename T, int G, int HS>
-__global__ __launch_bounds__(QKN_BWD_THREADS) void qkn_bwd_kernel(const QknParams p) {
+__global__ __launch_bounds__(QKN_BWD_THREADS, 3) void qkn_bwd_kernel(const QknParams p) {
   constexpr int GPB = QKN_BWD_THREADS / G;
   __shared__ float red[QKN_BWD_THREADS * 16];
   const int l = threadIdx.x & (G - 1);
@@ -238,10 +239,11 @@ __global__ __launch_bounds__(QKN_BWD_THREADS) void qkn_bwd_kernel(const QknParam
     float wa[8], wb[8];
     const float sc = sec == 0 ? p.q_scale : 1.0f;
     if (sec < 2 && on) {
+      const float* w = sec == 0 ? p.wq : p.wk;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        wa[i] = p.w[sec][8 * l + i];
-        wb[i] = p.w[sec][p.hd / 2 + 8 * l + i];
+        wa[i] = w[8 * l + i];
+        wb[i] = w[p.hd / 2 + 8 * l + i];
       }
     }
     for (int row = grp / chunks; row < p.rows; row += step) {
@@ -336,32 +338,38 @@ __global__ __launch_bounds__(QKN_BWD_THREADS) void qkn_bwd_kernel(const QknParam
     mine[8 * G + 8 * l + i] = db[i];
   }
   __syncthreads();
-  const int cols = 2 * p.hd, parts = QKN_BWD_THREADS / cols;
-  const int col = threadIdx.x % cols, part = threadIdx.x / cols;
-  float s = 0.f;
-  if (part < parts) {
-    const int sec = col / p.hd, e = col - sec * p.hd;
-    const int at = e < p.hd / 2 ? e : 8 * G + e - p.hd / 2;
-    const int c_lo = sec == 0 ? 0 : p.nq, c_hi = sec == 0 ? p.nq : p.nq + p.nk;
-    int c = (int)(((unsigned)blockIdx.x * GPB + part) % (unsigned)chunks);
-    const int c_step = parts % chunks;
-    for (int g = part; g < GPB; g += parts) {
-      if (c >= c_lo && c < c_hi) s += red[g * 16 * G + at];
-      c += c_step;
-      if (c >= chunks) c -= chunks;
+  const int cols = 2 * p.hd, parts = cols < QKN_BWD_THREADS ? QKN_BWD_THREADS / cols : 1;
+  float s[2] = {0.f, 0.f};  // 512 columns at the most
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int item = threadIdx.x + k * QKN_BWD_THREADS;
+    const int col = item % cols, part = item / cols;
+    if (part < parts) {
+      const int sec = col / p.hd, e = col - sec * p.hd;
+      const int at = e < p.hd / 2 ? e : 8 * G + e - p.hd / 2;
+      const int c_lo = sec == 0 ? 0 : p.nq, c_hi = sec == 0 ? p.nq : p.nq + p.nk;
+      int c = (int)(((unsigned)blockIdx.x * GPB + part) % (unsigned)chunks);
+      const int c_step = parts % chunks;
+      for (int g = part; g < GPB; g += parts) {
+        if (c >= c_lo && c < c_hi) s[k] += red[g * 16 * G + at];
+        c += c_step;
+        if (c >= chunks) c -= chunks;
+      }
     }
   }
   __syncthreads();
-  if (part < parts) red[part * cols + col] = s;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if ((int)threadIdx.x + k * QKN_BWD_THREADS < cols * parts) red[threadIdx.x + k * QKN_BWD_THREADS] = s[k];
   __syncthreads();
-  if ((int)threadIdx.x < cols) {
-    s = red[col];
-    for (int k = 1; k < parts; ++k) s += red[k * cols + col];
+  for (int col = threadIdx.x; col < cols; col += QKN_BWD_THREADS) {
+    float sum = red[col];
+    for (int k = 1; k < parts; ++k) sum += red[k * cols + col];
     if (gridDim.x == 1) {
       const int sec = col / p.hd;
-      p.dw[sec][col - sec * p.hd] += s;
+      (sec == 0 ? p.dwq : p.dwk)[col - sec * p.hd] += sum;
     } else {
-      p.slab[(size_t)blockIdx.x * cols + col] = s;
+      p.slab[(size_t)blockIdx.x * cols + col] = sum;
     }
   }
 }
@@ -399,7 +407,7 @@ int chunks_of(int H, int Hk, bool values, QknParams* p) {
 }
 bool wide_chunks(long rows, int H, int Hk, int G) { return rows * (H + 2 * Hk) / 4 * G >= 256L * 1024; }
 
-constexpr int QKN_BWD_BLOCKS = 512;  // two per CU
+constexpr int QKN_BWD_BLOCKS = 1024;  // four per CU
 
 bool geometry_ok(int rows, int N, int H, int Hk, int hd) {
   return rows >= 0 && rows <= (1 << 30) && N > 0 && H > 0 && Hk > 0 && H <= 4096 && Hk <= 4096 && hd >= 16 && hd <= 256 && hd % 16 == 0;
@@ -429,7 +437,7 @@ int launch_bwd(QknParams& p, bool values, long ws_bytes, hipStream_t st) {
   if (blocks > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL(qkn_dw_kernel, dim3((unsigned)(2 * p.hd / 16)), dim3(256), 0, st, p.slab, (int)blocks, p.hd, p.dw[0], p.dw[1]);
+    hipLaunchKernelGGL(qkn_dw_kernel, dim3((unsigned)(2 * p.hd / 16)), dim3(256), 0, st, p.slab, (int)blocks, p.hd, p.dwq, p.dwk);
   }
   SAVIT_LAUNCH_RET();
 }
@@ -447,7 +455,7 @@ extern "C" int savit_qk_norm_rope_fwd(const void* qkv, long ld, const float* wq,
   SAVIT_CHECK_ARG(out != qkv || ld == ld_out);
   if (rows == 0) return SAVIT_OK;
   QknParams p{};
-  p.x = qkv; p.y = out; p.w[0] = wq; p.w[1] = wk; p.table = table; p.pos = positions;
+  p.x = qkv; p.y = out; p.wq = wq; p.wk = wk; p.table = table; p.pos = positions;
   p.ldx = ld; p.ldy = ld_out; p.rows = rows; p.N = N; p.H = H; p.Hk = Hk; p.hd = head_dim; p.T = table_rows;
   p.eps = eps; p.q_scale = q_scale; p.center = center; p.inter = interleaved;
   const bool values = out != qkv;
@@ -487,8 +495,8 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
   SAVIT_CHECK_ARG(out != dqkv || ld_dqkv == ld_out);
   if (rows == 0) return SAVIT_OK;
   QknParams p{};
-  p.x = qkv; p.g = dqkv; p.y = out; p.w[0] = wq; p.w[1] = wk; p.table = table; p.pos = positions;
-  p.slab = (float*)workspace; p.dw[0] = dwq; p.dw[1] = dwk;
+  p.x = qkv; p.g = dqkv; p.y = out; p.wq = wq; p.wk = wk; p.table = table; p.pos = positions;
+  p.slab = (float*)workspace; p.dwq = dwq; p.dwk = dwk;
   p.ldx = ld; p.ldg = ld_dqkv; p.ldy = ld_out; p.rows = rows; p.N = N; p.H = H; p.Hk = Hk; p.hd = head_dim; p.T = table_rows;
   p.eps = eps; p.q_scale = q_scale; p.center = center; p.inter = interleaved;
   const bool values = out != dqkv;
@@ -496,9 +504,9 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
   const bool wide = wide_chunks(rows, H, Hk, G);
 #define QKN_BWD(GV)                                                                                                                     \
   case GV:                                                                                                                              \
-    return is_bf16 ? (wide ? launch_bwd<bf16_t, GV, 4>(p, values, workspace_bytes, (hipStream_t)stream)                                  \
+    return is_bf16 ? (wide ? launch_bwd<bf16_t, GV, 2>(p, values, workspace_bytes, (hipStream_t)stream)                                  \
                            : launch_bwd<bf16_t, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream))                                 \
-                   : (wide ? launch_bwd<float, GV, 2>(p, values, workspace_bytes, (hipStream_t)stream)                                   \
+                   : (wide ? launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream)                                   \
                            : launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream));
   switch (G) {
     QKN_BWD(1)

@@ -6,8 +6,8 @@
 // Forward is bound by the writes of the [H, N, ld] bias (the table and the index stay in L2): a thread writes 4 columns of 4 heads as 16-byte pieces.
 // Backward is a gather along a list of positions sorted by bucket, laid out once with the index: every table entry is one sum in a fixed order -
 // an atomic per position would make the gradient depend on scheduling, and the few buckets that far positions share would serialise.
-// A wave takes one bucket's list for 4 heads (the list is read once for them); where lists are long (N^2 / buckets >= 512) each is cut
-// into parts whose sums a second launch adds in order.
+// A wave takes one bucket's list for 4 heads (the list is read once for them); where lists are long it takes a fixed number of entries instead,
+// and a second launch adds the pieces of a bucket.
 #include "common.h"
 #include "savit.h"
 
@@ -15,6 +15,8 @@ namespace {
 
 constexpr int RB_HEADS = 4;
 
+// VEC: H % 4 == 0 and the table 16-byte aligned - a bucket's four heads are one load (four times fewer gathers)
+template <bool VEC>
 __global__ __launch_bounds__(256) void relpos_bias_kernel(const float* __restrict__ table, const int* __restrict__ index, float* __restrict__ bias, int N,
                                                           int H, int nb, int ld) {
   const int quads = ld / 4;
@@ -26,33 +28,29 @@ __global__ __launch_bounds__(256) void relpos_bias_kernel(const float* __restric
   int b[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) b[k] = j0 + k < N ? row[j0 + k] : -1;
+  float v[4][RB_HEADS];  // [column][head]
 #pragma unroll
-  for (int k4 = 0; k4 < RB_HEADS; ++k4) {
-    const int h = h0 + k4;
-    if (h < H) {
-      float v[4];
+  for (int k = 0; k < 4; ++k) {
+    const float none = j0 + k < N ? __builtin_nanf("") : 0.f;
+    const bool in = (unsigned)b[k] < (unsigned)nb;
+    if constexpr (VEC) {
+      float4 w = make_float4(none, none, none, none);
+      if (in) w = *reinterpret_cast<const float4*>(table + (size_t)b[k] * H + h0);
+      v[k][0] = w.x; v[k][1] = w.y; v[k][2] = w.z; v[k][3] = w.w;
+    } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = (unsigned)b[k] < (unsigned)nb ? table[(size_t)b[k] * H + h] : j0 + k < N ? __builtin_nanf("") : 0.f;
-      *reinterpret_cast<float4*>(bias + ((size_t)h * N + i) * ld + j0) = make_float4(v[0], v[1], v[2], v[3]);
+      for (int h = 0; h < RB_HEADS; ++h) v[k][h] = in && h0 + h < H ? table[(size_t)b[k] * H + h0 + h] : none;
     }
   }
+#pragma unroll
+  for (int h = 0; h < RB_HEADS; ++h)
+    if (h0 + h < H) *reinterpret_cast<float4*>(bias + ((size_t)(h0 + h) * N + i) * ld + j0) = make_float4(v[0][h], v[1][h], v[2][h], v[3][h]);
 }
 
-// out: dtable (parts == 1, added to) or the slab [parts][nb * H]
-__global__ __launch_bounds__(256) void relpos_grad_kernel(const float* __restrict__ dbias, const int* __restrict__ order, const int* __restrict__ start,
-                                                          float* __restrict__ out, int N, int H, int nb, int ld, int parts) {
+// sum of positions order[p0 .. p1) of RB_HEADS heads over a wave; every lane gets the sums
+__device__ __forceinline__ void sum_list(const float* __restrict__ dbias, const int* __restrict__ order, unsigned p0, unsigned p1, int N, int ld, int h0, int nh,
+                                         unsigned total, float (&out)[RB_HEADS]) {
   const int lane = threadIdx.x & 63;
-  const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (long)nb * parts) return;
-  const int b = (int)(item / parts), part = (int)(item - (long)b * parts);
-  const int h0 = blockIdx.y * RB_HEADS, nh = (H - h0) < RB_HEADS ? H - h0 : RB_HEADS;
-  const unsigned total = (unsigned)N * (unsigned)N;
-  unsigned lo = (unsigned)start[b], hi = (unsigned)start[b + 1];
-  if (lo > total) lo = total;  // a bad list is cut, never followed outside
-  if (hi > total) hi = total;
-  const unsigned len = hi > lo ? hi - lo : 0;
-  const unsigned per = (len + parts - 1) / parts;
-  const unsigned p0 = lo + (per * part < len ? per * part : len), p1 = lo + (per * (part + 1) < len ? per * (part + 1) : len);
   const float* base[RB_HEADS];
 #pragma unroll
   for (int k = 0; k < RB_HEADS; ++k) base[k] = dbias + (size_t)(h0 + (k < nh ? k : 0)) * N * ld;
@@ -67,61 +65,117 @@ __global__ __launch_bounds__(256) void relpos_grad_kernel(const float* __restric
     for (int k = 0; k < RB_HEADS; ++k) s[k] += base[k][at];
   }
 #pragma unroll
-  for (int k = 0; k < RB_HEADS; ++k) {
-    const float v = wave_sum(s[k]);
-    if (lane == 0 && k < nh) {
-      float* to = out + ((size_t)part * nb + b) * H + h0 + k;
-      *to = parts == 1 ? *to + v : v;
+  for (int k = 0; k < RB_HEADS; ++k) out[k] = wave_sum(s[k]);
+}
+// where bucket b's list begins; a bad list is cut, never followed outside
+__device__ __forceinline__ unsigned list_at(const int* start, int b, unsigned total) {
+  const unsigned v = (unsigned)start[b];
+  return v < total ? v : total;
+}
+
+// short lists: a wave a bucket
+__global__ __launch_bounds__(256) void relpos_grad_kernel(const float* __restrict__ dbias, const int* __restrict__ order, const int* __restrict__ start,
+                                                          float* __restrict__ dtable, int N, int H, int nb, int ld) {
+  const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b >= nb) return;
+  const int h0 = blockIdx.y * RB_HEADS, nh = (H - h0) < RB_HEADS ? H - h0 : RB_HEADS;
+  const unsigned total = (unsigned)N * (unsigned)N;
+  float s[RB_HEADS];
+  sum_list(dbias, order, list_at(start, b, total), list_at(start, b + 1, total), N, ld, h0, nh, total, s);
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int k = 0; k < RB_HEADS; ++k)
+      if (k < nh) dtable[(size_t)b * H + h0 + k] += s[k];
+  }
+}
+
+// long lists: a wave RB_CHUNK entries, whatever buckets they belong to; the piece of bucket b in chunk c goes to slab row c + b (every new piece
+// is a new chunk, a new bucket or both, so rows are not shared)
+constexpr int RB_CHUNK = 1024;
+__global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __restrict__ dbias, const int* __restrict__ order, const int* __restrict__ start,
+                                                                 float* __restrict__ slab, int N, int H, int nb, int ld, int chunks) {
+  const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c >= chunks) return;
+  const int h0 = blockIdx.y * RB_HEADS, nh = (H - h0) < RB_HEADS ? H - h0 : RB_HEADS;
+  const unsigned total = (unsigned)N * (unsigned)N;
+  const unsigned c0 = (unsigned)c * RB_CHUNK, c1 = c0 + RB_CHUNK < total ? c0 + RB_CHUNK : total;
+  int lo = 0, hi = nb;  // first bucket whose list ends behind c0
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (list_at(start, mid + 1, total) > c0) hi = mid;
+    else lo = mid + 1;
+  }
+  for (int b = lo; b < nb; ++b) {
+    const unsigned l0 = list_at(start, b, total), l1 = list_at(start, b + 1, total);
+    if (l0 >= c1) break;
+    const unsigned p0 = l0 > c0 ? l0 : c0, p1 = l1 < c1 ? l1 : c1;
+    if (p0 >= p1) continue;
+    float s[RB_HEADS];
+    sum_list(dbias, order, p0, p1, N, ld, h0, nh, total, s);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < RB_HEADS; ++k)
+        if (k < nh) slab[((size_t)c + b) * H + h0 + k] = s[k];
     }
   }
 }
 
-__global__ __launch_bounds__(256) void relpos_parts_kernel(const float* __restrict__ slab, float* __restrict__ dtable, int n, int parts) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+// dtable[b, h] += the bucket's pieces: a wave an entry, lanes and tree in a fixed order
+__global__ __launch_bounds__(256) void relpos_pieces_kernel(const float* __restrict__ slab, const int* __restrict__ start, float* __restrict__ dtable, int N,
+                                                            int H, int nb) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= nb * H) return;
+  const int b = i / H, h = i - b * H;
+  const unsigned total = (unsigned)N * (unsigned)N;
+  const unsigned l0 = list_at(start, b, total), l1 = list_at(start, b + 1, total);
   float s = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < parts; ++k) s += slab[(size_t)k * n + i];
-  dtable[i] += s;
+  if (l0 < l1)
+    for (unsigned c = l0 / RB_CHUNK + (threadIdx.x & 63); c <= (l1 - 1) / RB_CHUNK; c += 64) s += slab[((size_t)c + b) * H + h];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) dtable[i] += s;
 }
 
 bool size_ok(int N, int H, int nb, int ld) { return N > 0 && N <= 32768 && H > 0 && H <= 65536 && nb > 0 && (long)nb * H <= (1L << 30) && ld >= N && ld % 4 == 0; }
 
-int parts_of(int N, int nb) {
-  const long p = (long)N * N / ((long)nb * 512);
-  return p < 1 ? 1 : p > 128 ? 128 : (int)p;
-}
+// lists of 512 positions and more on average are cut into chunks: one wave a bucket leaves the far buckets' lists to a few waves (1500 tokens,
+// 32 buckets, 8 heads: 90 us against the chunks' RB_LONG_US); below, chunks of many short pieces only serialise
+bool long_lists(int N, int nb) { return (long)N * N >= 512L * nb; }
+int chunks_of(int N) { return (int)(((long)N * N + RB_CHUNK - 1) / RB_CHUNK); }
 
 }  // namespace
 
 extern "C" int savit_relpos_bias_fwd(const float* table, const int* index, float* bias, int N, int H, int buckets, int ld_bias, void* stream) {
   SAVIT_CHECK_ARG(table && index && bias && size_ok(N, H, buckets, ld_bias) && ((uintptr_t)bias % 16) == 0);
   const long blocks = ((long)N * (ld_bias / 4) + 255) / 256;
-  SAVIT_CHECK_ARG(blocks <= 0x7fffffffL);
-  hipLaunchKernelGGL(relpos_bias_kernel, dim3((unsigned)blocks, (unsigned)((H + RB_HEADS - 1) / RB_HEADS)), dim3(256), 0, (hipStream_t)stream, table, index,
-                     bias, N, H, buckets, ld_bias);
+  SAVIT_CHECK_ARG(blocks <= 0x7fffffffL && H <= 4 * 65535);
+  const dim3 grid((unsigned)blocks, (unsigned)((H + RB_HEADS - 1) / RB_HEADS));
+  if (H % RB_HEADS == 0 && ((uintptr_t)table % 16) == 0)
+    hipLaunchKernelGGL(relpos_bias_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, table, index, bias, N, H, buckets, ld_bias);
+  else
+    hipLaunchKernelGGL(relpos_bias_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, table, index, bias, N, H, buckets, ld_bias);
   SAVIT_LAUNCH_RET();
 }
 
 extern "C" long savit_relpos_bias_bwd_workspace_bytes(int N, int H, int buckets) {
-  if (!size_ok(N, H, buckets, (N + 3) / 4 * 4)) return 0;
-  const int parts = parts_of(N, buckets);
-  return parts == 1 ? 0 : (long)parts * buckets * H * 4;
+  if (!size_ok(N, H, buckets, (N + 3) / 4 * 4) || !long_lists(N, buckets)) return 0;
+  return ((long)chunks_of(N) + buckets) * H * 4;
 }
 
 extern "C" int savit_relpos_bias_bwd(const float* dbias, const int* order, const int* start, float* dtable, int N, int H, int buckets, int ld_bias,
                                      void* workspace, long workspace_bytes, void* stream) {
   SAVIT_CHECK_ARG(dbias && order && start && dtable && size_ok(N, H, buckets, ld_bias));
-  const int parts = parts_of(N, buckets);
-  SAVIT_CHECK_ARG(parts == 1 || (workspace && ((uintptr_t)workspace % 4) == 0 && workspace_bytes >= (long)parts * buckets * H * 4));
-  const long waves = (long)buckets * parts;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(relpos_grad_kernel, dim3((unsigned)((waves + 3) / 4), (unsigned)((H + RB_HEADS - 1) / RB_HEADS)), dim3(256), 0, st, dbias, order, start,
-                     parts == 1 ? dtable : (float*)workspace, N, H, buckets, ld_bias, parts);
-  if (parts > 1) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL(relpos_parts_kernel, dim3((unsigned)((buckets * H + 255) / 256)), dim3(256), 0, st, (const float*)workspace, dtable, buckets * H, parts);
+  const unsigned hg = (unsigned)((H + RB_HEADS - 1) / RB_HEADS);
+  if (!long_lists(N, buckets)) {
+    hipLaunchKernelGGL(relpos_grad_kernel, dim3((unsigned)((buckets + 3) / 4), hg), dim3(256), 0, st, dbias, order, start, dtable, N, H, buckets, ld_bias);
+    SAVIT_LAUNCH_RET();
   }
+  SAVIT_CHECK_ARG(workspace && ((uintptr_t)workspace % 4) == 0 && workspace_bytes >= savit_relpos_bias_bwd_workspace_bytes(N, H, buckets));
+  const int chunks = chunks_of(N);
+  hipLaunchKernelGGL(relpos_grad_chunks_kernel, dim3((unsigned)((chunks + 3) / 4), hg), dim3(256), 0, st, dbias, order, start, (float*)workspace, N, H, buckets,
+                     ld_bias, chunks);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(relpos_pieces_kernel, dim3((unsigned)((buckets * H + 3) / 4)), dim3(256), 0, st, (const float*)workspace, start, dtable, N, H, buckets);
   SAVIT_LAUNCH_RET();
 }
