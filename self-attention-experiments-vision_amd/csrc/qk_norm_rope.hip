@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void qkn_fwd_kernel(const QknParams p) {
 constexpr int QKN_BWD_THREADS = 256;
 
 template <typename T, int G, int HS>
-__global__ __launch_bounds__(QKN_BWD_THREADS, 3) void qkn_bwd_kernel(const QknParams p) {
+__global__ __launch_bounds__(QKN_BWD_THREADS, sizeof(T) == 2 ? 4 : 3) void qkn_bwd_kernel(const QknParams p) {
   constexpr int GPB = QKN_BWD_THREADS / G;
   __shared__ float red[QKN_BWD_THREADS * 16];
   const int l = threadIdx.x & (G - 1);
@@ -374,20 +374,25 @@ __global__ __launch_bounds__(QKN_BWD_THREADS, 3) void qkn_bwd_kernel(const QknPa
   }
 }
 
-// dw += column sums of the slab: 16 columns a block, 16 rows at a time, fixed order
-__global__ __launch_bounds__(256) void qkn_dw_kernel(const float* __restrict__ slab, int rows, int hd, float* __restrict__ dwq, float* __restrict__ dwk) {
-  __shared__ float red[16][17];
+// dw += column sums of the slab: 16 columns a block, 64 strips of rows, fixed order
+__global__ __launch_bounds__(1024) void qkn_dw_kernel(const float* __restrict__ slab, int rows, int hd, float* __restrict__ dwq, float* __restrict__ dwk) {
+  __shared__ float red[64][17];
   const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
   float s = 0.f;
 #pragma unroll 4
-  for (int r = r0; r < rows; r += 16) s += slab[(size_t)r * (2 * hd) + col];
+  for (int r = r0; r < rows; r += 64) s += slab[(size_t)r * (2 * hd) + col];
   red[r0][c] = s;
   __syncthreads();
-  if (r0 == 0) {
+  if (threadIdx.x < 64) {  // four partial sums a column
+    s = 0.f;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += red[k][c];
+    for (int k = 0; k < 16; ++k) s += red[r0 + 4 * k][c];
+    red[r0][c] = s;
+  }
+  __syncthreads();
+  if (r0 == 0) {
     float* dw = col < hd ? dwq + col : dwk + col - hd;
-    *dw += s;
+    *dw += (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
   }
 }
 
@@ -437,7 +442,7 @@ int launch_bwd(QknParams& p, bool values, long ws_bytes, hipStream_t st) {
   if (blocks > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL(qkn_dw_kernel, dim3((unsigned)(2 * p.hd / 16)), dim3(256), 0, st, p.slab, (int)blocks, p.hd, p.dwq, p.dwk);
+    hipLaunchKernelGGL(qkn_dw_kernel, dim3((unsigned)(2 * p.hd / 16)), dim3(1024), 0, st, p.slab, (int)blocks, p.hd, p.dwq, p.dwk);
   }
   SAVIT_LAUNCH_RET();
 }
@@ -501,13 +506,10 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
   p.eps = eps; p.q_scale = q_scale; p.center = center; p.inter = interleaved;
   const bool values = out != dqkv;
   const int G = lanes_of(head_dim);
-  const bool wide = wide_chunks(rows, H, Hk, G);
-#define QKN_BWD(GV)                                                                                                                     \
-  case GV:                                                                                                                              \
-    return is_bf16 ? (wide ? launch_bwd<bf16_t, GV, 2>(p, values, workspace_bytes, (hipStream_t)stream)                                  \
-                           : launch_bwd<bf16_t, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream))                                 \
-                   : (wide ? launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream)                                   \
-                           : launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream));
+#define QKN_BWD(GV)                                                                                        \
+  case GV:                                                                                                 \
+    return is_bf16 ? launch_bwd<bf16_t, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream)             \
+                   : launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream);
   switch (G) {
     QKN_BWD(1)
     QKN_BWD(2)

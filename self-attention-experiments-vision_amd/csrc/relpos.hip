@@ -55,14 +55,23 @@ __device__ __forceinline__ void sum_list(const float* __restrict__ dbias, const 
 #pragma unroll
   for (int k = 0; k < RB_HEADS; ++k) base[k] = dbias + (size_t)(h0 + (k < nh ? k : 0)) * N * ld;
   float s[RB_HEADS] = {};
-#pragma unroll 4
-  for (unsigned q = p0 + lane; q < p1; q += 64) {
-    const unsigned e = (unsigned)order[q];
-    if (e >= total) continue;
-    const unsigned i = e / (unsigned)N;
-    const size_t at = (size_t)i * ld + (e - i * (unsigned)N);
+  constexpr int U = 4;  // entries a lane has under way: the list, then all heads' values (a lane without an entry reads position 0 and drops it)
+  for (unsigned q = p0 + lane; q < p1; q += 64 * U) {
+    unsigned e[U];
 #pragma unroll
-    for (int k = 0; k < RB_HEADS; ++k) s[k] += base[k][at];
+    for (int u = 0; u < U; ++u) e[u] = q + 64 * u < p1 ? (unsigned)order[q + 64 * u] : 0xffffffffu;
+    float v[U][RB_HEADS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned x = e[u] < total ? e[u] : 0, i = x / (unsigned)N;
+      const size_t at = (size_t)i * ld + (x - i * (unsigned)N);
+#pragma unroll
+      for (int k = 0; k < RB_HEADS; ++k) v[u][k] = base[k][at];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < RB_HEADS; ++k) s[k] += e[u] < total ? v[u][k] : 0.f;
   }
 #pragma unroll
   for (int k = 0; k < RB_HEADS; ++k) out[k] = wave_sum(s[k]);
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(256) void relpos_grad_kernel(const float* __restric
 
 // long lists: a wave RB_CHUNK entries, whatever buckets they belong to; the piece of bucket b in chunk c goes to slab row c + b (every new piece
 // is a new chunk, a new bucket or both, so rows are not shared)
-constexpr int RB_CHUNK = 1024;
+constexpr int RB_CHUNK = 256;  // 1024: 36 us against 24 at 1500 tokens and 8 heads (a wave's few loads in flight are all latency)
 __global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __restrict__ dbias, const int* __restrict__ order, const int* __restrict__ start,
                                                                  float* __restrict__ slab, int N, int H, int nb, int ld, int chunks) {
   const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -120,19 +129,22 @@ __global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __
   }
 }
 
-// dtable[b, h] += the bucket's pieces: a wave an entry, lanes and tree in a fixed order
+// dtable[b, h] += the bucket's pieces: a block an entry, threads and tree in a fixed order
 __global__ __launch_bounds__(256) void relpos_pieces_kernel(const float* __restrict__ slab, const int* __restrict__ start, float* __restrict__ dtable, int N,
-                                                            int H, int nb) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= nb * H) return;
-  const int b = i / H, h = i - b * H;
+                                                            int H) {
+  __shared__ float red[4];
+  const int i = blockIdx.x, b = i / H, h = i - b * H;
   const unsigned total = (unsigned)N * (unsigned)N;
   const unsigned l0 = list_at(start, b, total), l1 = list_at(start, b + 1, total);
   float s = 0.f;
-  if (l0 < l1)
-    for (unsigned c = l0 / RB_CHUNK + (threadIdx.x & 63); c <= (l1 - 1) / RB_CHUNK; c += 64) s += slab[((size_t)c + b) * H + h];
+  if (l0 < l1) {
+#pragma unroll 4
+    for (unsigned c = l0 / RB_CHUNK + threadIdx.x; c <= (l1 - 1) / RB_CHUNK; c += 256) s += slab[((size_t)c + b) * H + h];
+  }
   s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) dtable[i] += s;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) dtable[i] += (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 bool size_ok(int N, int H, int nb, int ld) { return N > 0 && N <= 32768 && H > 0 && H <= 65536 && nb > 0 && (long)nb * H <= (1L << 30) && ld >= N && ld % 4 == 0; }
@@ -176,6 +188,6 @@ extern "C" int savit_relpos_bias_bwd(const float* dbias, const int* order, const
                      ld_bias, chunks);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(relpos_pieces_kernel, dim3((unsigned)((buckets * H + 3) / 4)), dim3(256), 0, st, (const float*)workspace, start, dtable, N, H, buckets);
+  hipLaunchKernelGGL(relpos_pieces_kernel, dim3((unsigned)(buckets * H)), dim3(256), 0, st, (const float*)workspace, start, dtable, N, H);
   SAVIT_LAUNCH_RET();
 }
