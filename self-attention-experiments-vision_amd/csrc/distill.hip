@@ -212,6 +212,11 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     else q.load_part(z + (size_t)i * E, p.C - i * E);
   };
 
+  // Requests in this order: the pairs, the row, the logits at the pairs' classes (memory answers in order: pairs asked for behind the row would
+  // only come with it, and the logits at their classes one more round trip later)
+  const bool paired = live && tid < K;
+  const int j0 = paired ? p.at[(size_t)row * K + tid] : -1;
+  const float t0 = paired ? p.top[(size_t)row * K + tid] : 0.f;
   Piece<TI> r[C];
   if (live) {
 #pragma unroll
@@ -225,16 +230,15 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
   __syncthreads();
 
   double tm = -1.7976931348623157e308;
-  if (live && 64 * wave < K) {  // the pairs, while the row is on its way
+  float z0 = 0.f;
+  if (live && 64 * wave < K) {
     int mine = 0;
-    for (int k = tid; k < K; k += TH) {
-      const int j = p.at[(size_t)row * K + k];
+    auto pair = [&](int k, int j, float t) {
       const bool ok = (unsigned)j < (unsigned)p.C;
-      const double t = ok ? (double)p.top[(size_t)row * K + k] / (double)p.T : -__builtin_inf();
+      const double td = ok ? (double)t / (double)p.T : -__builtin_inf();
       at[k] = ok ? j : -1;
-      zt[k] = ok ? to_float(z[j]) : 0.f;
-      tt[k] = t;
-      tm = fmax(tm, t);
+      tt[k] = td;
+      tm = fmax(tm, td);
       if (ok) {  // twice as many slots as pairs: an empty one is always found
         unsigned s = hash_of(j) & mask;
         int was;
@@ -242,7 +246,10 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
         if (was == -1) ++mine;
         else repeated[sub] = 1;
       }
-    }
+      return ok ? to_float(z[j]) : 0.f;
+    };
+    if (tid < K) z0 = pair(tid, j0, t0);
+    for (int k = tid + TH; k < K; k += TH) zt[k] = pair(k, p.at[(size_t)row * K + k], p.top[(size_t)row * K + k]);
     if (mine) atomicAdd(&distinct[sub], mine);
   }
   Seen me{-3.402823466e38f, 0.f, 0.f, 0.f};
@@ -282,6 +289,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       see(&q, i, std::integral_constant<int, 1>{});
     }
   }
+  if (tid < K) zt[tid] = z0;
   {
     me.s *= residue(me.m, p.c_soft);
     if (two) me.h *= residue(me.m, p.c_hard);

@@ -890,10 +890,10 @@ def _packed(t, dtype, rows: int, cols: int, name: str, dev: int) -> int:
     raise ValueError(f"{name}: expected at least [{rows}, {cols}], got {tuple(t.shape)}")
 
 
-def _scratch(workspace: Optional[torch.Tensor], need: int, device, dev: int):
+def _scratch(workspace: Optional[torch.Tensor], need: int, like: torch.Tensor, dev: int):
     """The caller's workspace, or a new one -> (tensor, its bytes)."""
     if workspace is None:
-        workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=device)
+        workspace = like.new_empty((max(need, 16),), dtype=torch.uint8)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace: a contiguous tensor on the current device")
     return workspace, workspace.numel() * workspace.element_size()
@@ -951,7 +951,7 @@ def qk_norm_rope_fwd(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, tabl
     dev = _dev(qkv)
     rows, width, ld, Hk, T = _qkn_args(qkv, wq, wk, table, N, H, Hk, head_dim, positions, dev)
     if out is None:
-        out = torch.empty((rows, width), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((rows, width))
         ldo = width
     else:
         ldo = _packed(out, qkv.dtype, rows, width, "out", dev)
@@ -981,7 +981,7 @@ def qk_norm_rope_bwd(dqkv: torch.Tensor, qkv: torch.Tensor, wq: torch.Tensor, wk
     if rows == 0:
         return out
     L = _lib.load()
-    ws, n = _scratch(workspace, L.savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim), qkv.device, dev)
+    ws, n = _scratch(workspace, L.savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim), qkv, dev)
     _lib.check(L.savit_qk_norm_rope_bwd(dqkv.data_ptr(), ldd, qkv.data_ptr(), ld, wq.data_ptr(), wk.data_ptr(), _p(table), T, _p(positions), out.data_ptr(), ldo,
                                         dwq.data_ptr(), dwk.data_ptr(), rows, N, H, Hk, head_dim, qkv.dtype is bf16, eps, q_scale, center, interleaved,
                                         ws.data_ptr(), n, _stream()), "savit_qk_norm_rope_bwd")
@@ -1057,7 +1057,7 @@ def relpos_bias_fwd(table: torch.Tensor, index: torch.Tensor, out: Optional[torc
     _whole(index, torch.int32, (N, N), "index", dev)
     if out is None:
         ld = (N + 3) // 4 * 4
-        out = torch.empty((H, N, ld), dtype=f32, device=table.device)
+        out = table.new_empty((H, N, ld))
         if ld != N:
             out = out[:, :, :N]
     else:
@@ -1080,7 +1080,7 @@ def relpos_bias_bwd(dbias: torch.Tensor, order: torch.Tensor, start: torch.Tenso
     _whole(start, torch.int32, (nb + 1,), "start", dev)
     L = _lib.load()
     need = L.savit_relpos_bias_bwd_workspace_bytes(N, H, nb)
-    ws, n = _scratch(workspace, need, dbias.device, dev) if need else (None, 0)
+    ws, n = _scratch(workspace, need, dbias, dev) if need else (None, 0)
     _lib.check(L.savit_relpos_bias_bwd(dbias.data_ptr(), order.data_ptr(), start.data_ptr(), dtable.data_ptr(), N, H, nb, ld, _p(ws), n, _stream()),
                "savit_relpos_bias_bwd")
     return dtable
@@ -1097,11 +1097,11 @@ def bias_attention_fwd(qkv: torch.Tensor, bias: torch.Tensor, B: int, N: int, H:
     if lens is not None:
         _whole(lens, torch.int32, (B,), "lens", dev)
     if out is None:
-        out = torch.empty((B * N, d), dtype=bf16, device=qkv.device)
+        out = qkv.new_empty((B * N, d))
     else:
         _whole(out, bf16, (B * N, d), "out", dev)
     if lse is None:
-        lse = torch.empty((B, H, N), dtype=f32, device=qkv.device)
+        lse = bias.new_empty((B, H, N))
     else:
         _whole(lse, f32, (B, H, N), "lse", dev)
     if B == 0:
@@ -1125,13 +1125,13 @@ def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor,
     if lens is not None:
         _whole(lens, torch.int32, (B,), "lens", dev)
     if dqkv is None:
-        dqkv = torch.empty((B * N, ld), dtype=bf16, device=qkv.device)
+        dqkv = qkv.new_empty((B * N, ld))
     elif _packed(dqkv, bf16, B * N, 3 * d, "dqkv", dev) != ld and B * N > 1:
         raise ValueError("dqkv must have qkv's row stride")
     if not want_dbias:
         dbias = None
     elif dbias is None:
-        dbias = torch.empty((H, N, ldb), dtype=f32, device=qkv.device)
+        dbias = bias.new_empty((H, N, ldb))
         if ldb != N:
             dbias = dbias[:, :, :N]
     elif _bias_ld(dbias, H, N, "dbias", dev) != ldb:
@@ -1139,7 +1139,7 @@ def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor,
     if B == 0:
         return dqkv, None if dbias is None else dbias.zero_()
     L = _lib.load()
-    ws, n = _scratch(workspace, L.savit_bias_attention_bwd_workspace_bytes(B, N, H, ldb, want_dbias), qkv.device, dev)
+    ws, n = _scratch(workspace, L.savit_bias_attention_bwd_workspace_bytes(B, N, H, ldb, want_dbias), qkv, dev)
     _lib.check(L.savit_bias_attention_bwd(qkv.data_ptr(), bias.data_ptr(), _p(lens), d_o.data_ptr(), lse.data_ptr(), dqkv.data_ptr(), _p(dbias), B, N, H, head_dim,
                                           ld, ldb, dq_scale, ws.data_ptr(), n, _stream()), "savit_bias_attention_bwd")
     return dqkv, dbias
@@ -1178,7 +1178,7 @@ def distill_xent(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
         if dlogits.data_ptr() == logits.data_ptr() and (dlogits.dtype is not logits.dtype or ld_dz != ld):
             raise ValueError("dlogits in logits' place needs its dtype and row stride")
     if loss_rows is None:
-        loss_rows = torch.empty((R,), dtype=f32, device=logits.device)
+        loss_rows = teacher_logits.new_empty((R,))
     else:
         _whole(loss_rows, f32, (R,), "loss_rows", dev)
     for name, t, n in (("teacher_lse", teacher_lse, R), ("row_weight", row_weight, R), ("dbias", dbias, C)):
