@@ -4,16 +4,16 @@
 // The batch may be padded: keys and queries at or beyond lens[b] take no part, their rows of O and of the gradients are zero, their
 // log-sum-exp -inf.  So are those of a query whose bias leaves no key (-inf, or the lowest value of float or bfloat16: scaled by log2 e it is -inf).
 //
-// Tiles: a wave owns 32 queries (forward, dQ) or 32 keys (dK, dV); the other side streams through LDS in segments of 64 rows shared by the
+// Tiles: a wave owns 16 or 32 queries (forward, dQ) or 16 keys (dK, dV); the other side streams through LDS in segments of 64 rows shared by the
 // W waves of a workgroup, fetched into registers under the arithmetic of the segment before and written to the other of two LDS buffers: one barrier a
 // segment.  Scores are computed transposed (query on the lane, keys in registers) where the softmax runs along keys: its statistics are
-// in-register reductions plus one half-wave exchange, and the score tile is the next product's operand without an LDS round trip.  The bias tile
-// is fetched one tile ahead and is the INITIAL value of the score accumulators: adding it costs nothing.  W = 1, 2 or 4 by the sequence
-// length, so that short sequences (windows) leave no wave idle.
+// in-register reductions plus an exchange between the lanes of a query, and the score tile is the next product's operand without an LDS round trip.
+// The bias tile is fetched one tile ahead and is the INITIAL value of the score accumulators: adding it costs nothing.  W = 1, 2 or 4 by the sequence
+// length, so that short sequences leave no wave idle.
 //
 // delta is summed from the fp32 probabilities, in a loop of its own over the keys, not taken as rowsum(dO . O): O is rounded to bf16, and the table
 // gradient that dS feeds is an fp32 parameter gradient (2^-9 of O in delta is 1e-4 of the gradient; this way it is 1e-6).
-// The bias gradient is a kernel of its own: a workgroup keeps one [queries x 64 keys] tile of one head in registers and walks over the
+// Up to 224 tokens dQ and the bias gradient are one kernel with the keys resident (below).  Beyond, the bias gradient is a kernel of its own: a workgroup keeps one [queries x 64 keys] tile of one head in registers and walks over the
 // images, so the sum over the batch is in a fixed order and touches memory once; long batches are cut into parts that a last launch adds.  It
 // recomputes two products; a sum by atomics would move N^2 values per image and head through memory and repeat in no fixed order.
 #include <type_traits>
@@ -65,13 +65,13 @@ template <int W, int KS>
 struct Segment {
   static constexpr int SEG = W == 1 ? 32 : 64, LOADS = SEG * 8 / (64 * W), IMG = SEG * ROWB;
   u32x4 a[LOADS], b[LOADS];
-  // rows row0 .. row0 + SEG - 1 of two column ranges of the image behind ra / rb; rows >= len and columns >= 16 KS are zero
+  // rows row0 .. row0 + SEG - 1 of two column ranges of the image behind ra / rb; rows >= len and 16-byte chunks >= `chunks` of a row are zero
   __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t ra, uint32_t lda2, uint32_t col_a2, __amdgpu_buffer_rsrc_t rb, uint32_t ldb2, uint32_t col_b2, int row0,
-                                        int len) {
+                                        int len, int chunks = 2 * KS) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int i = threadIdx.x + k * 64 * W, t = row0 + (i >> 3), c = i & 7;
-      const bool in = t < len && c < 2 * KS;
+      const bool in = t < len && c < chunks;
       a[k] = load16(ra, in ? (uint32_t)t * lda2 + col_a2 + 16 * c : OUTSIDE);
       b[k] = load16(rb, in ? (uint32_t)t * ldb2 + col_b2 + 16 * c : OUTSIDE);
     }
@@ -147,6 +147,42 @@ __device__ __forceinline__ void mask_keys(f32x16& s, int k0, int len, const Lane
     if (k0 + L.reg(r) >= len) s[r] = v;
 }
 
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// rows row0 .. row0 + 3 and row0 + 16 .. + 19 (row0 = 4 (lane / 16)) of columns col0 .. + 15: A operand whose k order is that of two stacked 16 x 16
+// accumulators
+__device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
+  const int o = img_off(row, col >> 3) + ((col & 7) << 1);  // (16 rows on: the same swizzle)
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o + 16 * ROWB));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// sum over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float quarters_sum(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  return half_sum(a + b);
+}
+
+__device__ __forceinline__ float quarters_max(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  return half_max(fmaxf(a, b));
+}
+// Columns of the 2 KS2 accumulators of a lane's row (16 eb + 4 (lane / 16) ..), scaled, rounded and stored 16 bytes at a time: lanes 16 apart trade pieces of
+// two accumulators first.  Columns >= hd are skipped.
+template <int KS2>
+__device__ __forceinline__ void store_row16(bf16_t* row, const f32x4 (&o)[2 * KS2], int g, int hd, float sc) {
+#pragma unroll
+  for (int eb = 0; eb < 2 * KS2; eb += 2) {
+    uint32_t a0 = pack_bf16x2(o[eb][0] * sc, o[eb][1] * sc), a1 = pack_bf16x2(o[eb][2] * sc, o[eb][3] * sc);
+    uint32_t b0 = pack_bf16x2(o[eb + 1][0] * sc, o[eb + 1][1] * sc), b1 = pack_bf16x2(o[eb + 1][2] * sc, o[eb + 1][3] * sc);
+    const auto r0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false), r1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+    const unsigned x0 = r0[0], y0 = r0[1], x1 = r1[0], y1 = r1[1];
+    const int col = (g & 1) ? 16 * (eb + 1) + 4 * (g - 1) : 16 * eb + 4 * g;
+    if (col < hd) *reinterpret_cast<uint4*>(row + col) = make_uint4(x0, x1, y0, y1);
+  }
+}
+
 // workgroup -> (head, image, block): all blocks and images of a head in a row, and consecutive numbers on one XCD, so that its L2 holds the
 // head's bias for every image
 __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b, int& blk) {
@@ -157,8 +193,9 @@ __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b,
   h = r / p.B;
 }
 
-template <int W, int KS>
-__global__ __launch_bounds__(64 * W, 3) void bias_attn_fwd_kernel(const BiasAttnParams p) {
+template <int KS>
+__global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnParams p) {
+  constexpr int W = 4;
   typedef Segment<W, KS> Seg;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
   constexpr int hd = 16 * KS;
@@ -237,9 +274,113 @@ __global__ __launch_bounds__(64 * W, 3) void bias_attn_fwd_kernel(const BiasAttn
   }
 }
 
+// The same with 16 queries a wave: twice the waves of half the registers, for narrow heads, short sequences and grids that leave SIMDs empty.  What
+// it reads from LDS serves half as many queries.
+template <int W, int KS2>
+__global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel(const BiasAttnParams p) {
+  typedef Segment<W, 2 * KS2> Seg;
+  constexpr int T = Seg::SEG / 16;
+  __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
+  const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int h, b, blk;
+  item_of(p, h, b, blk);
+  const int len = length_of(p, b);
+  const int q = (blk * W + wave) * 16 + ql;
+  const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, hcol = (uint32_t)(h * p.hd) * 2;
+  const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2);
+  const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
+  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * g) * 4 : BEYOND;
+  const int nseg = blk * W * 16 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
+  Seg sg;
+  f32x4 o[2 * KS2];
+#pragma unroll
+  for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = LOWEST, l = 0.f;  // running reference (log2 units) and sum
+  if (nseg > 0) {
+    bf16x8 qf[KS2];
+    sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, 0, len, p.hd / 8);
+#pragma unroll
+    for (int ks = 0; ks < KS2; ++ks) {
+      const int c = 32 * ks + 8 * g;
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
+    }
+    f32x4 sc[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) sc[t] = load4f(rb, boff + 64 * t);
+    sg.put(smem);
+    __syncthreads();
+    for (int s = 0; s < nseg; ++s) {
+      const bool more = s + 1 < nseg;
+      const int k0 = s * Seg::SEG;
+      if (more) sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, k0 + Seg::SEG, len, p.hd / 8);
+      const char* imgK = smem + (s & 1) * 2 * Seg::IMG;
+      const char* imgV = imgK + Seg::IMG;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS2; ++ks) sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+      if (k0 + Seg::SEG > len) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (k0 + 16 * t + 4 * g + r >= len) sc[t][r] = -INFINITY;
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
+      top = quarters_max(top) * LOG2E_F;
+      if (__any(top > m + 8.f)) {  // as above
+        const float mn = fmaxf(m, top);
+        const float alpha = __builtin_amdgcn_exp2f(m - mn);
+        l *= alpha;
+#pragma unroll
+        for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] *= alpha;
+        m = mn;
+      }
+#pragma unroll
+      for (int t = 0; t < T; t += 2) {
+        union { uint32_t u[4]; bf16x8 v; } pf;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x4& x = sc[t + k];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], LOG2E_F, -m));
+            l += x[r];
+          }
+          pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
+          pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
+          if (more) x = load4f(rb, boff + (uint32_t)(k0 + Seg::SEG + 16 * (t + k)) * 4);
+        }
+#pragma unroll
+        for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = mfma16(lds_tr_pair(imgV, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, o[eb]);
+      }
+      if (more) {
+        sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
+        __syncthreads();
+      }
+    }
+  }
+  l = quarters_sum(l);
+  if (q < p.N) {
+    const bool some = q < len && l != 0.f;
+    if (!some) {
+#pragma unroll
+      for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    store_row16<KS2>(p.o + ((size_t)b * p.N + q) * p.d + h * p.hd, o, g, p.hd, some ? 1.0f / l : 0.f);
+    if (g == 0) p.lse[((size_t)b * p.H + h) * p.N + q] = some ? (m + __log2f(l)) * LN2_F : -INFINITY;
+  }
+}
+
 // dQ, and the statistics the other two kernels read.  Two loops over the keys: delta, then dQ.
-template <int W, int KS>
-__global__ __launch_bounds__(64 * W, 2) void bias_attn_dq_kernel(const BiasAttnParams p) {
+template <int KS>
+__global__ __launch_bounds__(256, 2) void bias_attn_dq_kernel(const BiasAttnParams p) {
+  constexpr int W = 4;
   typedef Segment<W, KS> Seg;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
   constexpr int hd = 16 * KS;
@@ -336,89 +477,122 @@ __global__ __launch_bounds__(64 * W, 2) void bias_attn_dq_kernel(const BiasAttnP
   }
 }
 
-// dK and dV: key on the lane, queries in registers
-template <int W, int KS>
-__global__ __launch_bounds__(64 * W, 2) void bias_attn_dkv_kernel(const BiasAttnParams p) {
-  typedef Segment<W, KS> Seg;
+// dK and dV: a wave owns 16 keys (on the lane; queries in registers), Q and dO stream.  16 and not 32 keys a wave: 64 accumulators fewer leave room for four waves
+// a SIMD instead of two, which is worth more than the LDS reads that 32 keys would share
+template <int W, int KS2>
+__global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(const BiasAttnParams p) {
+  typedef Segment<W, 2 * KS2> Seg;
+  constexpr int T = Seg::SEG / 16;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
-  constexpr int hd = 16 * KS;
-  const Lane L;
+  __shared__ float stats[2][2][Seg::SEG];  // of the two buffers: -lse log2 e, delta
+  const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
   item_of(p, h, b, blk);
   const int len = length_of(p, b);
-  const int key = (blk * W + wave) * 32 + L.ql;
+  const int key = (blk * W + wave) * 16 + ql;
   const bool ok = key < len;
-  const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
-  const bf16_t* imd = p.d_o + (size_t)b * p.N * p.d;
-  const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
-  const auto rd = rsrc_of(imd, (size_t)p.N * p.d * 2);
+  const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, hcol = (uint32_t)(h * p.hd) * 2;
+  const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2);
+  const auto rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
   const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
-  const uint32_t cq = (uint32_t)(h * hd) * 2;
-  const uint32_t boff = (uint32_t)(4 * L.half * p.ldb + key) * 4;
-  const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
+  const uint32_t boff = (uint32_t)(4 * g * p.ldb + key) * 4, brow = (uint32_t)p.ldb * 4;
+  const int nseg = blk * W * 16 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
   Seg sg;
-  f32x16 dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
-  if (nseg > 0) {
-    bf16x8 kf[KS], vf[KS];
-    sg.fetch(rs, (uint32_t)p.ld * 2, cq, rd, (uint32_t)p.d * 2, cq, 0, len);
-    load_frags<KS>(kf, img, key, p.ld, p.d + h * hd, L.half, ok);
-    load_frags<KS>(vf, img, key, p.ld, 2 * p.d + h * hd, L.half, ok);
-    f32x16 next;
-    auto load_bias = [&](int q0) {
+  float st = 0.f;
+  auto fetch = [&](int q0) {
+    sg.fetch(rs, ld2, hcol, rd, d2, hcol, q0, len, p.hd / 8);
+    if (threadIdx.x < 2 * Seg::SEG) {
+      const int i = threadIdx.x % Seg::SEG;
+      st = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, (uint32_t)(q0 + i + (threadIdx.x < Seg::SEG ? 0 : p.Np)) * 4, 0, 0));
+    }
+  };
+  auto put = [&](int buf) {
+    sg.put(smem + buf * 2 * Seg::IMG);
+    if (threadIdx.x < 2 * Seg::SEG) (&stats[buf][0][0])[threadIdx.x] = st;
+  };
+  f32x4 dk[2 * KS2], dv[2 * KS2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        next[r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, boff + (uint32_t)((q0 + (r & 3) + 8 * (r >> 2)) * p.ldb) * 4, 0, 0));
+  for (int eb = 0; eb < 2 * KS2; ++eb) dk[eb] = dv[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (nseg > 0) {
+    bf16x8 kf[KS2], vf[KS2];
+    fetch(0);
+#pragma unroll
+    for (int ks = 0; ks < KS2; ++ks) {
+      const int c = 32 * ks + 8 * g;
+      kf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)key * ld2 + d2 + hcol + 2 * c : OUTSIDE));
+      vf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)key * ld2 + 2 * d2 + hcol + 2 * c : OUTSIDE));
+    }
+    f32x4 sc[T];
+    auto load_bias = [&](int t, int q0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rb, boff + (uint32_t)(q0 + r) * brow, 0, 0));
     };
-    load_bias(0);
-    sg.put(smem);
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_bias(t, 16 * t);
+    put(0);
     __syncthreads();
     for (int s = 0; s < nseg; ++s) {
       const bool more = s + 1 < nseg;
-      if (more) sg.fetch(rs, (uint32_t)p.ld * 2, cq, rd, (uint32_t)p.d * 2, cq, (s + 1) * Seg::SEG, len);
+      const int q0 = s * Seg::SEG;
+      if (more) fetch(q0 + Seg::SEG);
       const char* imgQ = smem + (s & 1) * 2 * Seg::IMG;
       const char* imgD = imgQ + Seg::IMG;
 #pragma unroll
-      for (int t = 0; t < Seg::SEG / 32; ++t) {
-        const int q0 = s * Seg::SEG + 32 * t;
-        if (q0 >= len) break;
-        f32x4 nl[4], dl[4];
+      for (int t = 0; t < T; t += 2) {
+        if (q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries' statistics say -inf)
+          union { uint32_t u[4]; bf16x8 v; } pf, df;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          nl[g] = load4f(rt, (uint32_t)(4 * L.half + q0 + 8 * g) * 4);
-          dl[g] = load4f(rt, (uint32_t)(4 * L.half + p.Np + q0 + 8 * g) * 4);
-        }
-        f32x16 sc = next;
-        load_bias(q0 + 32);
-        f32x16 dp = zero16();
-        tile_product<KS>(sc, imgQ, 32 * t + L.ql, kf, L.half);
-        tile_product<KS>(dp, imgD, 32 * t + L.ql, vf, L.half);
+          for (int k = 0; k < 2; ++k) {
+            f32x4 dp = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, nl[r >> 2][r & 3]));
-          dp[r] = sc[r] * (dp[r] - dl[r >> 2][r & 3]);
+            for (int ks = 0; ks < KS2; ++ks) {
+              sc[t + k] = mfma16(lds_row_frag(imgQ, 16 * (t + k) + ql, 4 * ks + g), kf[ks], sc[t + k]);
+              dp = mfma16(lds_row_frag(imgD, 16 * (t + k) + ql, 4 * ks + g), vf[ks], dp);
+            }
+            const f32x4 nl = *reinterpret_cast<const f32x4*>(&stats[s & 1][0][16 * (t + k) + 4 * g]);
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][1][16 * (t + k) + 4 * g]);
+            float pr[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t + k][r], LOG2E_F, nl[r]));
+              dp[r] = pr[r] * (dp[r] - dl[r]);
+            }
+            pf.u[2 * k] = pack_bf16x2(pr[0], pr[1]);
+            pf.u[2 * k + 1] = pack_bf16x2(pr[2], pr[3]);
+            df.u[2 * k] = pack_bf16x2(dp[0], dp[1]);
+            df.u[2 * k + 1] = pack_bf16x2(dp[2], dp[3]);
+            if (more) load_bias(t + k, q0 + Seg::SEG + 16 * (t + k));
+          }
+#pragma unroll
+          for (int eb = 0; eb < 2 * KS2; ++eb) {
+            dv[eb] = mfma16(lds_tr_pair(imgD, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dv[eb]);
+            dk[eb] = mfma16(lds_tr_pair(imgQ, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), df.v, dk[eb]);
+          }
         }
-        tile_accumulate<KS>(dv, imgD, 32 * t, sc, L);
-        tile_accumulate<KS>(dk, imgQ, 32 * t, dp, L);
       }
       if (more) {
-        sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
+        put((s + 1) & 1);
         __syncthreads();
       }
     }
   }
   if (key < p.N) {
-    if (!ok) dk[0] = dk[1] = dv[0] = dv[1] = zero16();
-    bf16_t* row = p.dqkv + ((size_t)b * p.N + key) * p.ld + p.d + h * hd;
-    store_row_tile(row, dk, L.half, hd, 1.0f);
-    store_row_tile(row + p.d, dv, L.half, hd, 1.0f);
+    if (!ok) {
+#pragma unroll
+      for (int eb = 0; eb < 2 * KS2; ++eb) dk[eb] = dv[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bf16_t* row = p.dqkv + ((size_t)b * p.N + key) * p.ld + p.d + h * p.hd;
+    store_row16<KS2>(row, dk, g, p.hd, 1.0f);
+    store_row16<KS2>(row + p.d, dv, g, p.hd, 1.0f);
   }
 }
 
 // dbias of a tile of 32 W queries x SEG keys of one head, summed over the images of a part
-template <int W, int KS>
-__global__ __launch_bounds__(64 * W, 2) void bias_attn_db_kernel(const BiasAttnParams p) {
+template <int KS>
+__global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnParams p) {
+  constexpr int W = 4;
   typedef Segment<W, KS> Seg;
   constexpr int T = Seg::SEG / 32;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
@@ -511,22 +685,6 @@ __global__ __launch_bounds__(64 * W, 2) void bias_attn_db_kernel(const BiasAttnP
 // Persistent over the images of one head, with two K / V image pairs: the next image's rows are fetched into registers (in groups where they are many) while this one is
 // computed, and put into the other pair half an image later; the only barrier is the one between images.  The score tiles are independent
 // accumulators: every LDS and MFMA latency is covered by the other tiles of the same wave.
-
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-// rows row0 .. row0 + 3 and row0 + 16 .. + 19 (row0 = 4 (lane / 16)) of columns col0 .. + 15: A operand whose k order is that of two stacked 16 x 16
-// accumulators
-__device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
-  const int o = img_off(row, col >> 3) + ((col & 7) << 1);  // (16 rows on: the same swizzle)
-  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o));
-  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o + 16 * ROWB));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-// sum over lanes l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ float quarters_sum(float v) {
-  float a = v, b = v;
-  permlane16_swap(a, b);
-  return half_sum(a + b);
-}
 
 template <int KT, int KS2, bool DB>
 __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_kernel(const BiasAttnParams p) {
@@ -668,14 +826,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
         if (t == KT / 4 * 2) load_queries(bn, lenn);
       }
     }
-    if (q < p.N) {
-      bf16_t* row = p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd + 4 * g;
-#pragma unroll
-      for (int eb = 0; eb < 2 * KS2; ++eb)
-        if (16 * eb < p.hd)
-          *reinterpret_cast<uint2*>(row + 16 * eb) = make_uint2(pack_bf16x2(dq[eb][0] * p.dq_scale, dq[eb][1] * p.dq_scale),
-                                                                pack_bf16x2(dq[eb][2] * p.dq_scale, dq[eb][3] * p.dq_scale));
-    }
+    if (q < p.N) store_row16<KS2>(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd, dq, g, p.hd, p.dq_scale);
     {  // statistics of the queries, and of the padding up to Np (fewer than three times the rows here) that the dK / dV kernel's tiles read
       const int row = q + g * (int)(blockDim.x >> 6) * 16 * p.blocks;
       if (row < p.Np) {
@@ -717,7 +868,6 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
   }
 }
 
-int waves_of(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : 4; }
 int padded(int N) { return (N + 63) / 64 * 64; }
 
 // Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel
@@ -755,18 +905,17 @@ bool size_ok(int B, int N, int H, int hd, int ld, int ldb) {
 }
 bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
-#define BIAS_ATTN_KS(KERNEL, WV, GRID)                                                                                                              \
-  switch (head_dim / 16) {                                                                                                                          \
-    case 1: hipLaunchKernelGGL((KERNEL<WV, 1>), dim3((unsigned)(GRID)), dim3(64 * WV), 0, st, p); break;                                              \
-    case 2: hipLaunchKernelGGL((KERNEL<WV, 2>), dim3((unsigned)(GRID)), dim3(64 * WV), 0, st, p); break;                                              \
-    case 3: hipLaunchKernelGGL((KERNEL<WV, 3>), dim3((unsigned)(GRID)), dim3(64 * WV), 0, st, p); break;                                              \
-    default: hipLaunchKernelGGL((KERNEL<WV, 4>), dim3((unsigned)(GRID)), dim3(64 * WV), 0, st, p); break;                                             \
-  }
-#define BIAS_ATTN_LAUNCH(KERNEL, GRID)                                                                                                              \
-  do {                                                                                                                                              \
-    if (W == 1) { BIAS_ATTN_KS(KERNEL, 1, GRID) } else if (W == 2) { BIAS_ATTN_KS(KERNEL, 2, GRID) } else { BIAS_ATTN_KS(KERNEL, 4, GRID) }           \
-    const hipError_t e_ = hipGetLastError();                                                                                                        \
-    if (e_ != hipSuccess) return (int)e_;                                                                                                           \
+#define BIAS_ATTN_LAUNCH(KERNEL, GRID)                                                              \
+  do {                                                                                              \
+    const dim3 g_((unsigned)(GRID)), t_(256);                                                       \
+    switch (head_dim / 16) {                                                                        \
+      case 1: hipLaunchKernelGGL((KERNEL<1>), g_, t_, 0, st, p); break;                             \
+      case 2: hipLaunchKernelGGL((KERNEL<2>), g_, t_, 0, st, p); break;                             \
+      case 3: hipLaunchKernelGGL((KERNEL<3>), g_, t_, 0, st, p); break;                             \
+      default: hipLaunchKernelGGL((KERNEL<4>), g_, t_, 0, st, p); break;                            \
+    }                                                                                               \
+    const hipError_t e_ = hipGetLastError();                                                        \
+    if (e_ != hipSuccess) return (int)e_;                                                           \
   } while (0)
 
 template <int KT, int KS2, bool DB>
@@ -793,6 +942,38 @@ int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
   }
 }
 
+// waves a workgroup: as many as a short sequence has tiles, four at the most
+int waves_for(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+template <typename F>
+int launch_waves(BiasAttnParams& p, int W, int rows, F kfn, hipStream_t st) {  // rows: of a wave
+  p.blocks = (p.N + rows * W - 1) / (rows * W);
+  const long grid = (long)p.B * p.H * p.blocks;
+  SAVIT_CHECK_ARG(grid <= 0x7fffffffL);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)grid), dim3(64 * W), 0, st, p);
+  SAVIT_LAUNCH_RET();
+}
+int launch_fwd(BiasAttnParams p, hipStream_t st) {
+  const int W = waves_for(p.N);
+  // 32 queries a wave where heads are wide, sequences long and the grid is two workgroups a CU or more, else 16 (heads of 64; 32 against 16 a wave:
+  // [128 x 12 x 197] 54.5 against 62.8 us, [16 x 12 x 197] 11.9 / 11.7, [8 x 16 x 577] 31.4 / 33.9, [4 x 16 x 577] 22.1 / 21.6, [2 x 8 x 1500] 39.7 / 34.6,
+  // [1024 x 12 x 49] 85.2 / 64.1)
+  if (p.N > 64 && p.hd > 32 && (long)p.B * p.H * ((p.N + 127) / 128) >= 2L * CUS)
+    return p.hd == 48 ? launch_waves(p, 4, 32, bias_attn_fwd_kernel<3>, st) : launch_waves(p, 4, 32, bias_attn_fwd_kernel<4>, st);
+  if (p.hd <= 32)
+    return W == 1 ? launch_waves(p, 1, 16, bias_attn_fwd16_kernel<1, 1>, st)
+                  : W == 2 ? launch_waves(p, 2, 16, bias_attn_fwd16_kernel<2, 1>, st) : launch_waves(p, 4, 16, bias_attn_fwd16_kernel<4, 1>, st);
+  return W == 1 ? launch_waves(p, 1, 16, bias_attn_fwd16_kernel<1, 2>, st)
+                : W == 2 ? launch_waves(p, 2, 16, bias_attn_fwd16_kernel<2, 2>, st) : launch_waves(p, 4, 16, bias_attn_fwd16_kernel<4, 2>, st);
+}
+int launch_dkv(BiasAttnParams p, hipStream_t st) {
+  const int W = waves_for(p.N);
+  if (p.hd <= 32)
+    return W == 1 ? launch_waves(p, 1, 16, bias_attn_dkv_kernel<1, 1>, st)
+                  : W == 2 ? launch_waves(p, 2, 16, bias_attn_dkv_kernel<2, 1>, st) : launch_waves(p, 4, 16, bias_attn_dkv_kernel<4, 1>, st);
+  return W == 1 ? launch_waves(p, 1, 16, bias_attn_dkv_kernel<1, 2>, st)
+                : W == 2 ? launch_waves(p, 2, 16, bias_attn_dkv_kernel<2, 2>, st) : launch_waves(p, 4, 16, bias_attn_dkv_kernel<4, 2>, st);
+}
+
 }  // namespace
 
 extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
@@ -802,11 +983,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.o = (bf16_t*)o; p.lse = lse;
   p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias;
-  const int W = waves_of(N);
-  const hipStream_t st = (hipStream_t)stream;
-  p.blocks = (N + 32 * W - 1) / (32 * W);
-  BIAS_ATTN_LAUNCH(bias_attn_fwd_kernel, (long)B * H * p.blocks);
-  return SAVIT_OK;
+  return launch_fwd(p, (hipStream_t)stream);
 }
 
 extern "C" long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, int ld_bias, int want_dbias) {
@@ -834,19 +1011,16 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   p.dbias = slab;
   if (resident(N)) {
     p.blocks = resident_blocks(N);
-    const int rc = launch_resident(p, dbias != nullptr, st);
-    if (rc != SAVIT_OK) return rc;
+    const int rr = launch_resident(p, dbias != nullptr, st);
+    if (rr != SAVIT_OK) return rr;
   } else {
-    constexpr int W = 4;
     p.blocks = (N + 127) / 128;
     BIAS_ATTN_LAUNCH(bias_attn_dq_kernel, (long)B * H * p.blocks);
   }
-  const int W = waves_of(N);
-  p.blocks = (N + 32 * W - 1) / (32 * W);
-  BIAS_ATTN_LAUNCH(bias_attn_dkv_kernel, (long)B * H * p.blocks);
+  const int rc = launch_dkv(p, st);
+  if (rc != SAVIT_OK) return rc;
   if (dbias) {
     if (!resident(N)) {
-      constexpr int W = 4;
       p.key_blocks = (N + 63) / 64;
       const long grid = (long)p.parts * H * p.blocks * p.key_blocks;
       SAVIT_CHECK_ARG(grid <= 0x7fffffffL);
