@@ -377,100 +377,110 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
   }
 }
 
-// dQ, and the statistics the other two kernels read.  Two loops over the keys: delta, then dQ.
-template <int KS>
-__global__ __launch_bounds__(256, 2) void bias_attn_dq_kernel(const BiasAttnParams p) {
+// dQ, and the statistics the other two kernels read.  Two loops over the keys: delta, then dQ.  16 queries a wave.
+template <int KS2>
+__global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnParams p) {
   constexpr int W = 4;
-  typedef Segment<W, KS> Seg;
+  typedef Segment<W, 2 * KS2> Seg;
+  constexpr int T = Seg::SEG / 16;
   __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
-  constexpr int hd = 16 * KS;
-  const Lane L;
+  const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
   item_of(p, h, b, blk);
   const int len = length_of(p, b);
-  const int q = (blk * W + wave) * 32 + L.ql;
-  const bool ok = q < len;
-  const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
-  const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
+  const int q = (blk * W + wave) * 16 + ql;
+  const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, hcol = (uint32_t)(h * p.hd) * 2;
+  const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2);
+  const auto ro = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
-  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : BEYOND;
-  const uint32_t ck = (uint32_t)(p.d + h * hd) * 2, cv = ck + (uint32_t)p.d * 2;
-  const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
+  const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * g) * 4 : BEYOND;
+  const int nseg = blk * W * 16 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
   float nl = -INFINITY, delta = 0.f;
-  if (ok) {
+  if (q < len) {
     const float v = p.lse[((size_t)b * p.H + h) * p.N + q];
     nl = v == -INFINITY ? -INFINITY : -LOG2E_F * v;
   }
-  constexpr int T = Seg::SEG / 32;
   Seg sg;
-  f32x16 dq[2] = {zero16(), zero16()};
-  if (nseg > 0) {
-    bf16x8 qf[KS], df[KS];
-    sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, 0, len);
-    load_frags<KS>(qf, img, q, p.ld, h * hd, L.half, ok);
-    load_frags<KS>(df, p.d_o, (size_t)b * p.N + q, p.d, h * hd, L.half, ok);
-    f32x16 next[T];
+  f32x4 dq[2 * KS2];
 #pragma unroll
-    for (int t = 0; t < T; ++t) load_bias_t(next[t], rb, boff, 32 * t);
+  for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (nseg > 0) {
+    bf16x8 qf[KS2], df[KS2];
+    sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, 0, len, p.hd / 8);
+#pragma unroll
+    for (int ks = 0; ks < KS2; ++ks) {
+      const int c = 32 * ks + 8 * g;
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
+      df[ks] = __builtin_bit_cast(bf16x8, load16(ro, c < p.hd ? (uint32_t)q * d2 + hcol + 2 * c : OUTSIDE));
+    }
+    f32x4 next[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) next[t] = load4f(rb, boff + 64 * t);
     sg.put(smem);
     __syncthreads();
     for (int s2 = 0; s2 < 2 * nseg; ++s2) {
       const bool second = s2 >= nseg, more = s2 + 1 < 2 * nseg;
       const int k0 = (second ? s2 - nseg : s2) * Seg::SEG, kn = k0 + Seg::SEG < len ? k0 + Seg::SEG : 0;
-      if (more) sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, kn, len);
-      if (s2 == nseg) delta = half_sum(delta);
+      if (more) sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, kn, len, p.hd / 8);
+      if (s2 == nseg) delta = quarters_sum(delta);
       const char* imgK = smem + (s2 & 1) * 2 * Seg::IMG;
       const char* imgV = imgK + Seg::IMG;
-      auto tiles = [&](auto count) {
-        constexpr int M = decltype(count)::value;
-        f32x16 sc[M], dp[M];
+      f32x4 sc[T], dp[T];
 #pragma unroll
-        for (int t = 0; t < M; ++t) {
-          sc[t] = next[t];
-          dp[t] = zero16();
+      for (int t = 0; t < T; ++t) {
+        sc[t] = next[t];
+        dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (more) next[t] = load4f(rb, boff + (uint32_t)(kn + 16 * t) * 4);
+#pragma unroll
+        for (int ks = 0; ks < KS2; ++ks) {
+          sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+          dp[t] = mfma16(lds_row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
         }
-        if (more) {
+      }
 #pragma unroll
-          for (int t = 0; t < T; ++t) load_bias_t(next[t], rb, boff, kn + 32 * t);
-        }
+      for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int t = 0; t < M; ++t) {
-          tile_product<KS>(sc[t], imgK, 32 * t + L.ql, qf, L.half);
-          tile_product<KS>(dp[t], imgV, 32 * t + L.ql, df, L.half);
-        }
+        for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+      if (k0 + Seg::SEG > len) {
 #pragma unroll
-        for (int t = 0; t < M; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
-        if (k0 + 32 * M > len) mask_keys(sc[M - 1], k0 + 32 * (M - 1), len, L, 0.f);
-        if (!second) {
+          for (int r = 0; r < 4; ++r)
+            if (k0 + 16 * t + 4 * g + r >= len) sc[t][r] = 0.f;
+      }
+      if (!second) {
 #pragma unroll
-          for (int t = 0; t < M; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) delta += sc[t][r] * dp[t][r];
-        } else {
+          for (int r = 0; r < 4; ++r) delta += sc[t][r] * dp[t][r];
+      } else {
 #pragma unroll
-          for (int t = 0; t < M; ++t) {
+        for (int t = 0; t < T; t += 2) {
+          union { uint32_t u[4]; bf16x8 v; } pf;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[t][r] *= dp[t][r] - delta;
-            tile_accumulate<KS>(dq, imgK, 32 * t, sc[t], L);
+          for (int k = 0; k < 2; ++k) {
+            f32x4 x = sc[t + k] * (dp[t + k] - delta);
+            pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
+            pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
           }
+#pragma unroll
+          for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dq[eb]);
         }
-      };
-      if (T == 2 && k0 + 32 < len) tiles(std::integral_constant<int, T>{});
-      else tiles(std::integral_constant<int, 1>{});
+      }
       if (more) {
         sg.put(smem + ((s2 + 1) & 1) * 2 * Seg::IMG);
         __syncthreads();
       }
     }
   }
-  if (q < p.N) {
-    if (!ok) dq[0] = dq[1] = zero16();
-    store_row_tile(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * hd, dq, L.half, hd, p.dq_scale);
+  if (q >= len) {
+    delta = 0.f;
+#pragma unroll
+    for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (L.half == 0 && q < p.Np) {
+  if (q < p.N) store_row16<KS2>(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd, dq, g, p.hd, p.dq_scale);
+  if (g == 0 && q < p.Np) {
     float* st = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + q;
     st[0] = nl;
     st[p.Np] = delta;
@@ -558,6 +568,11 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
             for (int r = 0; r < 4; ++r) {
               pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t + k][r], LOG2E_F, nl[r]));
               dp[r] = pr[r] * (dp[r] - dl[r]);
+            }
+            if (q0 + 16 * (t + k) + 16 > len) {  // whatever the bias holds there
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (q0 + 16 * (t + k) + 4 * g + r >= len) pr[r] = dp[r] = 0.f;
             }
             pf.u[2 * k] = pack_bf16x2(pr[0], pr[1]);
             pf.u[2 * k + 1] = pack_bf16x2(pr[2], pr[3]);
@@ -659,8 +674,10 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl)) * (dp[t][r] - delta);
       if (k0 + 32 * t + 32 > len) mask_keys(sc[t], k0 + 32 * t, len, L, 0.f);
+      if (q < len) {  // (whatever the bias holds in other rows)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[t][r] += sc[t][r];
+        for (int r = 0; r < 16; ++r) acc[t][r] += sc[t][r];
+      }
     }
     if (more) {
       sg.put(smem + ((b - b0 + 1) & 1) * 2 * Seg::IMG);
@@ -792,7 +809,12 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
 #pragma unroll
       for (int r = 0; r < 4; ++r) d[r] += sc[t][r] * dp[t][r];
     }
-    const float delta = quarters_sum((d[0] + d[1]) + (d[2] + d[3]));
+    float delta = quarters_sum((d[0] + d[1]) + (d[2] + d[3]));
+    if (q >= len) {  // whatever the bias holds in such a row
+      delta = 0.f;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     if constexpr (RES_GROUPS >= 2) {
       put(0, buf ^ 1);
       fetch(rn, 1);
@@ -1014,13 +1036,14 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
     const int rr = launch_resident(p, dbias != nullptr, st);
     if (rr != SAVIT_OK) return rr;
   } else {
-    p.blocks = (N + 127) / 128;
-    BIAS_ATTN_LAUNCH(bias_attn_dq_kernel, (long)B * H * p.blocks);
+    const int rq = head_dim <= 32 ? launch_waves(p, 4, 16, bias_attn_dq_kernel<1>, st) : launch_waves(p, 4, 16, bias_attn_dq_kernel<2>, st);
+    if (rq != SAVIT_OK) return rq;
   }
   const int rc = launch_dkv(p, st);
   if (rc != SAVIT_OK) return rc;
   if (dbias) {
     if (!resident(N)) {
+      p.blocks = (N + 127) / 128;
       p.key_blocks = (N + 63) / 64;
       const long grid = (long)p.parts * H * p.blocks * p.key_blocks;
       SAVIT_CHECK_ARG(grid <= 0x7fffffffL);

@@ -296,6 +296,29 @@ def test_bias_attention_padded_batch(ops, N, lens):
     assert torch.equal(again[0], dqkv) and torch.equal(again[1], dbias)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("N,lens,hd", [(20, [3, 0, 9], 32), (64, [47, 33], 16), (130, [100, 128], 48), (224, [197, 1], 64), (300, [7, 290, 257], 64), (330, [129, 0], 32)])
+def test_bias_attention_rows_behind_every_sequence(ops, N, lens, hd, bad):
+    """Bias rows and columns that no sequence reaches hold anything: no gradient reads them, theirs is zero."""
+    B, H, top = len(lens), 2, max(lens)
+    g = gen(N + hd)
+    lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qkv = randn(g, B * N, 3 * H * hd, dtype=torch.bfloat16, scale=0.6)
+    d_o = randn(g, B * N, H * hd, dtype=torch.bfloat16)
+    clean = ops.relpos_bias_empty(H, N)
+    clean.copy_(randn(g, H, N, N))
+    o, lse = ops.bias_attention_fwd(qkv, clean, B, N, H, head_dim=hd, lens=lens)
+    want = ops.bias_attention_bwd(qkv, clean, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd, lens=lens)
+    dirty = ops.relpos_bias_empty(H, N)
+    dirty.copy_(clean)
+    dirty[:, top:], dirty[:, :, top:] = bad, bad
+    o2, lse2 = ops.bias_attention_fwd(qkv, dirty, B, N, H, head_dim=hd, lens=lens)
+    got = ops.bias_attention_bwd(qkv, dirty, d_o, lse2, B, N, H, dq_scale=1.0, head_dim=hd, lens=lens)
+    assert torch.equal(o2, o) and torch.equal(lse2, lse)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert bool((got[1][:, top:] == 0).all()) and bool((got[1][:, :, top:] == 0).all())
+
+
 @pytest.mark.parametrize("N", [3, 40, 64, 197])
 @pytest.mark.parametrize("masked", [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min])
 def test_bias_attention_masks_in_the_bias(ops, N, masked):
