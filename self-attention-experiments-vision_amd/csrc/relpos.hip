@@ -15,15 +15,16 @@ namespace {
 
 constexpr int RB_HEADS = 4;
 
+// A thread takes four columns of four heads; G threads in a row take 4 G heads of the same columns, so that they read one bucket's heads from the same
+// cache line and the 64 / G column groups of a wave still store 1 KB / G in a row.
 // VEC: H % 4 == 0 and the table 16-byte aligned - a bucket's four heads are one load (four times fewer gathers)
-template <bool VEC>
+template <bool VEC, int G>
 __global__ __launch_bounds__(256) void relpos_bias_kernel(const float* __restrict__ table, const int* __restrict__ index, float* __restrict__ bias, int N,
                                                           int H, int nb, int ld) {
-  const int quads = ld / 4;
-  const long t = (long)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (long)N * quads) return;
-  const int i = (int)(t / quads), j0 = (int)(t - (long)i * quads) * 4;
-  const int h0 = blockIdx.y * RB_HEADS;
+  const unsigned quads = ld / 4, t = blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int h0 = (blockIdx.y * G + threadIdx.x % G) * RB_HEADS;
+  if (t >= N * quads || h0 >= H) return;
+  const int i = (int)(t / quads), j0 = (int)(t - i * quads) * 4;
   const int* row = index + (size_t)i * N;
   int b[4];
 #pragma unroll
@@ -158,13 +159,15 @@ int chunks_of(int N) { return (int)(((long)N * N + RB_CHUNK - 1) / RB_CHUNK); }
 
 extern "C" int savit_relpos_bias_fwd(const float* table, const int* index, float* bias, int N, int H, int buckets, int ld_bias, void* stream) {
   SAVIT_CHECK_ARG(table && index && bias && size_ok(N, H, buckets, ld_bias) && ((uintptr_t)bias % 16) == 0);
-  const long blocks = ((long)N * (ld_bias / 4) + 255) / 256;
-  SAVIT_CHECK_ARG(blocks <= 0x7fffffffL && H <= 4 * 65535);
-  const dim3 grid((unsigned)blocks, (unsigned)((H + RB_HEADS - 1) / RB_HEADS));
+  const int groups = (H + RB_HEADS - 1) / RB_HEADS, G = groups == 1 ? 1 : groups == 2 ? 2 : 4;
+  const long blocks = ((long)N * (ld_bias / 4) + 256 / G - 1) / (256 / G);
+  SAVIT_CHECK_ARG(blocks <= 0xffffffL);  // (32-bit thread numbers)
+  const dim3 grid((unsigned)blocks, (unsigned)((groups + G - 1) / G));
+  auto launch = [&](auto kfn) { hipLaunchKernelGGL(kfn, grid, dim3(256), 0, (hipStream_t)stream, table, index, bias, N, H, buckets, ld_bias); };
   if (H % RB_HEADS == 0 && ((uintptr_t)table % 16) == 0)
-    hipLaunchKernelGGL(relpos_bias_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, table, index, bias, N, H, buckets, ld_bias);
+    G == 1 ? launch(relpos_bias_kernel<true, 1>) : G == 2 ? launch(relpos_bias_kernel<true, 2>) : launch(relpos_bias_kernel<true, 4>);
   else
-    hipLaunchKernelGGL(relpos_bias_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, table, index, bias, N, H, buckets, ld_bias);
+    G == 1 ? launch(relpos_bias_kernel<false, 1>) : G == 2 ? launch(relpos_bias_kernel<false, 2>) : launch(relpos_bias_kernel<false, 4>);
   SAVIT_LAUNCH_RET();
 }
 
