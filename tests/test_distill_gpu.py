@@ -259,3 +259,43 @@ def test_distill_captured(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((loss, dz, db), want[k]))
         eager(z)
+
+
+def test_distill_through_a_model(ops):
+    """The loss on an engine's logits, its gradient through the engine's custom-loss entry: the hard term alone gives loss_backward's gradients; with a
+    teacher the head's gradients are those of the 64-bit loss gradient.  200 classes: the engine's gradient rows are padded."""
+    from oracle import vit_ref
+    from savit_amd.config import ModelConfig
+    from savit_amd.engine import ViTEngine
+
+    kw = dict(kind="vit", num_layers=2, num_heads=3, embed_dim=192, patch=16, num_classes=200, img_size=64)
+    B, C, K = 6, 200, 9
+    eng = ViTEngine(ModelConfig(**kw), B)
+    eng.load_params(vit_ref.init_params(vit_ref.Cfg(**kw), seed=1, randomize=True))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    images = torch.randn(B, 64, 64, 3, generator=g, device="cuda")
+    _, top, at, lse, labels = make(B, C, K, 11, torch.float32, lse=True, T=2.0)
+    eng.forward(images)
+    eng.loss_backward(labels, 0.1)
+    want = eng.grads.double()
+
+    def backward(**loss):
+        db = torch.zeros(C, device="cuda")
+        rows = ops.distill_xent(eng.logits, top, at, labels=labels, label_smoothing=0.1, dlogits=eng.dlogits[:, :C], dbias=db, **loss)
+        eng.backward_from_dlogits()
+        off = eng.layout.off["bh"][0]
+        eng.grads[off : off + C] += db
+        return rows, db
+
+    backward(distill_weight=0.0, hard_weight=1.0)
+    # the two kernels' logit gradients may round to neighbours, and so may what follows: a few steps of 2^-8 at random signs
+    assert float((eng.grads.double() - want).norm() / want.norm()) < 2 * U
+    rows, db = backward(temperature=2.0, distill_weight=0.7, teacher_lse=lse, hard_weight=0.3)
+    loss, grad, tol_loss, tol_grad = ref_distill(eng.logits, top, at, 2.0, 0.7, lse, labels, 0.3, 0.1, None, 1.0 / B)
+    assert bool(((rows.double() - loss).abs() <= tol_loss).all())
+    tol = tol_grad + U * grad.abs()
+    off, d = eng.layout.off["Wh"][0], kw["embed_dim"]
+    z = eng.zcls.double()
+    dwh = eng.grads[off : off + d * C].view(d, C).double()
+    assert bool(((dwh - z.T @ grad).abs() <= z.abs().T @ tol * 1.01 + 1e-30).all())  # (a sum of six products in fp32: 2^-21 of them, inside the hundredth)
+    assert bool(((db.double() - grad.sum(0)).abs() <= tol.sum(0) * 1.01 + 1e-30).all())
