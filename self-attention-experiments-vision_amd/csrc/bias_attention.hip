@@ -60,6 +60,16 @@ __device__ __forceinline__ int length_of(const BiasAttnParams& p, int b) {
   return l < 0 ? 0 : l > p.N ? p.N : l;
 }
 
+// Byte offset of 16-byte chunk c of an image's row (ROWB bytes).  The XOR by row bits 1..3 serves both shapes without bank conflicts: row fragments of
+// 16 rows x 4 chunks (a pass of ds_read_b128 takes rows 0-3 and 12-15 of one chunk with rows 4-11 of its neighbour) or 32 rows x 2, and transposed reads
+// of 16 rows x 2 chunks or 4 rows x 4.  (attention.hip's order of the bits is made for its 32-row tiles; 16 rows of it conflict: 22 % of dK / dV's LDS time.)
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1 & 1) << 2 | ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); }
+__device__ __forceinline__ int at_chunk(int row, int c) { return row * ROWB + ((c ^ swizzle(row)) << 4); }
+__device__ __forceinline__ bf16x8 row_frag(const char* img, int row, int c) { return *reinterpret_cast<const bf16x8*>(img + at_chunk(row, c)); }
+__device__ __forceinline__ bf16x4 read_tr(const char* img, int row, int col) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + at_chunk(row, col >> 3) + ((col & 7) << 1)));
+}
+
 // two images (64 columns a row, SEG rows) of a segment: registers on their way from memory to LDS
 template <int W, int KS>
 struct Segment {
@@ -80,7 +90,7 @@ struct Segment {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int i = threadIdx.x + k * 64 * W;
-      const int off = img_off(i >> 3, i & 7);
+      const int off = at_chunk(i >> 3, i & 7);
       *reinterpret_cast<u32x4*>(img + off) = a[k];
       *reinterpret_cast<u32x4*>(img + IMG + off) = b[k];
     }
@@ -120,7 +130,7 @@ __device__ __forceinline__ void load_frags(bf16x8 (&f)[KS], const bf16_t* base, 
 template <int KS>
 __device__ __forceinline__ void tile_product(f32x16& s, const char* img, int row, const bf16x8 (&f)[KS], int half) {
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_row_frag(img, row, 2 * ks + half), f[ks], s, 0, 0, 0);
+  for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag(img, row, 2 * ks + half), f[ks], s, 0, 0, 0);
 }
 // out^T[e][lane] += sum over the tile's 32 rows of image[row][e] * a[row][lane]
 template <int KS>
@@ -129,8 +139,11 @@ __device__ __forceinline__ void tile_accumulate(f32x16 (&out)[2], const char* im
   for (int s2 = 0; s2 < 2; ++s2) {
     const bf16x8 af = acc_to_frag(a, s2);
 #pragma unroll
-    for (int eb = 0; eb < (KS > 2 ? 2 : 1); ++eb)
-      out[eb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_tr_frag(img, row0 + 16 * s2 + L.trow, 32 * eb + L.tcol), af, out[eb], 0, 0, 0);
+    for (int eb = 0; eb < (KS > 2 ? 2 : 1); ++eb) {
+      const int row = row0 + 16 * s2 + L.trow, col = 32 * eb + L.tcol;
+      const bf16x8 vf = __builtin_shufflevector(read_tr(img, row, col), read_tr(img, row + 8, col), 0, 1, 2, 3, 4, 5, 6, 7);
+      out[eb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, af, out[eb], 0, 0, 0);
+    }
   }
 }
 __device__ __forceinline__ f32x16 zero16() {
@@ -151,9 +164,7 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __
 // rows row0 .. row0 + 3 and row0 + 16 .. + 19 (row0 = 4 (lane / 16)) of columns col0 .. + 15: A operand whose k order is that of two stacked 16 x 16
 // accumulators
 __device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
-  const int o = img_off(row, col >> 3) + ((col & 7) << 1);  // (16 rows on: the same swizzle)
-  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o));
-  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(img + o + 16 * ROWB));
+  const bf16x4 lo = read_tr(img, row, col), hi = read_tr(img + 16 * ROWB, row, col);  // (16 rows on: the same swizzle)
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -205,7 +216,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
   item_of(p, h, b, blk);
   const int len = length_of(p, b);
   const int q = (blk * W + wave) * 32 + L.ql;
-  const bool ok = q < len;
+  const bool ok = q < len, live = (blk * W + wave) * 32 < len;  // live: some query of the wave is
   const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
   const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
@@ -231,7 +242,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
 #pragma unroll
       for (int t = 0; t < Seg::SEG / 32; ++t) {
         const int k0 = s * Seg::SEG + 32 * t;
-        if (k0 >= len) break;
+        if (!live || k0 >= len) break;
         f32x16 sc = next;
         load_bias_t(next, rb, boff, k0 + 32);
         tile_product<KS>(sc, imgK, 32 * t + L.ql, qf, L.half);
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int ks = 0; ks < KS2; ++ks) sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+        for (int ks = 0; ks < KS2; ++ks) sc[t] = mfma16(row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
       if (k0 + Seg::SEG > len) {
 #pragma unroll
         for (int t = 0; t < T; ++t)
@@ -434,8 +445,8 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
         if (more) next[t] = load4f(rb, boff + (uint32_t)(kn + 16 * t) * 4);
 #pragma unroll
         for (int ks = 0; ks < KS2; ++ks) {
-          sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
-          dp[t] = mfma16(lds_row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
+          sc[t] = mfma16(row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+          dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
         }
       }
 #pragma unroll
@@ -501,7 +512,7 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   item_of(p, h, b, blk);
   const int len = length_of(p, b);
   const int key = (blk * W + wave) * 16 + ql;
-  const bool ok = key < len;
+  const bool ok = key < len, live = (blk * W + wave) * 16 < len;  // live: some key of the wave is
   const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, hcol = (uint32_t)(h * p.hd) * 2;
   const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2);
   const auto rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
@@ -551,15 +562,15 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
       const char* imgD = imgQ + Seg::IMG;
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
-        if (q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries' statistics say -inf)
+        if (live && q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries' statistics say -inf)
           union { uint32_t u[4]; bf16x8 v; } pf, df;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             f32x4 dp = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS2; ++ks) {
-              sc[t + k] = mfma16(lds_row_frag(imgQ, 16 * (t + k) + ql, 4 * ks + g), kf[ks], sc[t + k]);
-              dp = mfma16(lds_row_frag(imgD, 16 * (t + k) + ql, 4 * ks + g), vf[ks], dp);
+              sc[t + k] = mfma16(row_frag(imgQ, 16 * (t + k) + ql, 4 * ks + g), kf[ks], sc[t + k]);
+              dp = mfma16(row_frag(imgD, 16 * (t + k) + ql, 4 * ks + g), vf[ks], dp);
             }
             const f32x4 nl = *reinterpret_cast<const f32x4*>(&stats[s & 1][0][16 * (t + k) + 4 * g]);
             const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][1][16 * (t + k) + 4 * g]);
@@ -725,21 +736,28 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
   constexpr int LEAST = 64 * (KT <= 8 ? KT - 1 : KT / 2), MAXL = (PIECES / RES_GROUPS + LEAST - 1) / LEAST;  // threads, pieces a thread and group
   u32x4 st[MAXL];
   const int chunks = p.hd / 8;
+  auto thread = [] {  // opaque: the offsets below are computed where they are used, 16 of them held over the loop are 16 registers too many
+    int i = threadIdx.x;
+    if constexpr (RES_GROUPS == 4) asm volatile("" : "+v"(i));
+    return i;
+  };
   auto fetch = [&](__amdgpu_buffer_rsrc_t rs, int grp) {
+    const int i0 = thread();
 #pragma unroll
     for (int k = 0; k < MAXL; ++k) {
-      const int u = grp * (PIECES / RES_GROUPS) + threadIdx.x + k * blockDim.x;
+      const int u = grp * (PIECES / RES_GROUPS) + i0 + k * blockDim.x;
       const int t = (u >> 4), c = (u & 7) < chunks ? (u & 7) : 0;
-      const bool in = threadIdx.x + k * blockDim.x < PIECES / RES_GROUPS;
+      const bool in = i0 + k * (int)blockDim.x < PIECES / RES_GROUPS;
       st[k] = load16(rs, in ? (uint32_t)t * ld2 + ((u & 8) ? 2 * d2 : d2) + hcol + 16 * c : OUTSIDE);
     }
   };
   auto put = [&](int grp, int buf) {
+    const int i0 = thread();
 #pragma unroll
     for (int k = 0; k < MAXL; ++k) {
-      const int u = grp * (PIECES / RES_GROUPS) + threadIdx.x + k * blockDim.x;
-      if (threadIdx.x + k * blockDim.x < PIECES / RES_GROUPS)
-        *reinterpret_cast<u32x4*>(smem + buf * 2 * IMG + ((u & 8) ? IMG : 0) + img_off(u >> 4, u & 7)) = st[k];
+      const int u = grp * (PIECES / RES_GROUPS) + i0 + k * blockDim.x;
+      if (i0 + k * (int)blockDim.x < PIECES / RES_GROUPS)
+        *reinterpret_cast<u32x4*>(smem + buf * 2 * IMG + ((u & 8) ? IMG : 0) + at_chunk(u >> 4, u & 7)) = st[k];
     }
   };
   auto image = [&](int b, int len) { return rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2); };
@@ -791,8 +809,8 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
       dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS2; ++ks) {
-        sc[t] = mfma16(lds_row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
-        dp[t] = mfma16(lds_row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
+        sc[t] = mfma16(row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+        dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
       }
     }
     const float nl = q < len && lse != -INFINITY ? -LOG2E_F * lse : -INFINITY;
