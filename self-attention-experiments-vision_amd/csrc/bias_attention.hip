@@ -54,6 +54,16 @@ constexpr uint32_t BEYOND = 0xfff00000u;   // the same for an offset that someth
 __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
 __device__ __forceinline__ f32x4 load4f(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_bit_cast(f32x4, load16(r, off)); }
 
+__device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t r, uint32_t off, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0); }
+// off, or beyond every range.  Opaque: the compiler makes two loads in two branches of a plain choice.  (What is in flight is counted: behind a
+// branch with a load or store in it, the count is not known and every wait is for everything - the segment just asked for included.  The kernels here
+// therefore fetch unconditionally, out of range where there is nothing to fetch.)
+__device__ __forceinline__ uint32_t only(bool in, uint32_t off) {
+  uint32_t m = in ? 0u : OUTSIDE;
+  asm("" : "+v"(m));
+  return off | m;
+}
+
 __device__ __forceinline__ int length_of(const BiasAttnParams& p, int b) {
   if (p.lens == nullptr) return p.N;
   const int l = __builtin_amdgcn_readfirstlane(p.lens[b]);
@@ -118,12 +128,6 @@ __device__ __forceinline__ void load_bias_t(f32x16& s, __amdgpu_buffer_rsrc_t r,
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[4 * g + i] = v[i];
   }
-}
-
-template <int KS>
-__device__ __forceinline__ void load_frags(bf16x8 (&f)[KS], const bf16_t* base, size_t row, int ld, int col, int half, bool ok) {
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) f[ks] = load_row_frag_global(base, row, ld, col + 16 * ks + 8 * half, ok);
 }
 
 // S^T (or dP^T) tile: rows of the image against the lane's fragments
@@ -217,8 +221,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
   const int len = length_of(p, b);
   const int q = (blk * W + wave) * 32 + L.ql;
   const bool ok = q < len, live = (blk * W + wave) * 32 < len;  // live: some query of the wave is
-  const bf16_t* img = p.qkv + (size_t)b * p.N * p.ld;
-  const auto rs = rsrc_of(img, (size_t)p.N * p.ld * 2);
+  const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)p.N * p.ld * 2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
   const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * L.half) * 4 : BEYOND;
   const uint32_t ck = (uint32_t)(p.d + h * hd) * 2, cv = ck + (uint32_t)p.d * 2;
@@ -229,24 +232,24 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
   if (nseg > 0) {
     bf16x8 qf[KS];
     sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, 0, len);
-    load_frags<KS>(qf, img, q, p.ld, h * hd, L.half, ok);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(ok, (uint32_t)q * p.ld * 2 + (h * hd + 16 * ks + 8 * L.half) * 2)));
     f32x16 next;
     load_bias_t(next, rb, boff, 0);
     sg.put(smem);
     __syncthreads();
-    for (int s = 0; s < nseg; ++s) {
-      const bool more = s + 1 < nseg;
-      if (more) sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, (s + 1) * Seg::SEG, len);
+    auto segment = [&](int s, auto more) {
       const char* imgK = smem + (s & 1) * 2 * Seg::IMG;
       const char* imgV = imgK + Seg::IMG;
 #pragma unroll
       for (int t = 0; t < Seg::SEG / 32; ++t) {
         const int k0 = s * Seg::SEG + 32 * t;
-        if (!live || k0 >= len) break;
         f32x16 sc = next;
-        load_bias_t(next, rb, boff, k0 + 32);
+        if (more || t == 0) load_bias_t(next, rb, boff, k0 + 32);
+        if (more && t == 0) sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, (s + 1) * Seg::SEG, len);  // (behind the bias: loads arrive in order)
+        if (!live || (!more && k0 >= len)) continue;
         tile_product<KS>(sc, imgK, 32 * t + L.ql, qf, L.half);
-        if (k0 + 32 > len) mask_keys(sc, k0, len, L, -INFINITY);
+        if (!more && k0 + 32 > len) mask_keys(sc, k0, len, L, -INFINITY);
         float top = sc[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
@@ -270,11 +273,13 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
         }
         tile_accumulate<KS>(oacc, imgV, 32 * t, sc, L);
       }
-      if (more) {
+      if constexpr (more) {
         sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
         __syncthreads();
       }
-    }
+    };
+    for (int s = 0; s + 1 < nseg; ++s) segment(s, std::true_type{});
+    segment(nseg - 1, std::false_type{});
   }
   l = half_sum(l);
   if (q < p.N) {
@@ -285,13 +290,13 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
   }
 }
 
-// The same with 16 queries a wave: twice the waves of half the registers, for narrow heads, short sequences and grids that leave SIMDs empty.  What
+// The same with 16 queries a wave (ONE: and no more keys than a segment; else the last segment asks for one that is out of range): twice the waves of half the registers, for narrow heads, short sequences and grids that leave SIMDs empty.  What
 // it reads from LDS serves half as many queries.
-template <int W, int KS2>
+template <int W, int KS2, bool ONE>
 __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel(const BiasAttnParams p) {
   typedef Segment<W, 2 * KS2> Seg;
   constexpr int T = Seg::SEG / 16;
-  __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
+  __shared__ __attribute__((aligned(16))) char smem[(ONE ? 2 : 4) * Seg::IMG];
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
@@ -314,17 +319,19 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
 #pragma unroll
     for (int ks = 0; ks < KS2; ++ks) {
       const int c = 32 * ks + 8 * g;
-      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(c < p.hd, (uint32_t)q * ld2 + hcol + 2 * c)));
     }
     f32x4 sc[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) sc[t] = load4f(rb, boff + 64 * t);
     sg.put(smem);
     __syncthreads();
-    for (int s = 0; s < nseg; ++s) {
-      const bool more = s + 1 < nseg;
+    for (int s = 0; s < (ONE ? 1 : nseg); ++s) {
       const int k0 = s * Seg::SEG;
-      if (more) sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, k0 + Seg::SEG, len, p.hd / 8);
+      if constexpr (!ONE) {
+        sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, k0 + Seg::SEG, len, p.hd / 8);
+        __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to their use)
+      }
       const char* imgK = smem + (s & 1) * 2 * Seg::IMG;
       const char* imgV = imgK + Seg::IMG;
 #pragma unroll
@@ -365,12 +372,12 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
           }
           pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
           pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
-          if (more) x = load4f(rb, boff + (uint32_t)(k0 + Seg::SEG + 16 * (t + k)) * 4);
+          if constexpr (!ONE) x = load4f(rb, boff + (uint32_t)(k0 + Seg::SEG + 16 * (t + k)) * 4);
         }
 #pragma unroll
         for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = mfma16(lds_tr_pair(imgV, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, o[eb]);
       }
-      if (more) {
+      if (!ONE && s + 1 < nseg) {
         sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
         __syncthreads();
       }
@@ -422,68 +429,75 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
 #pragma unroll
     for (int ks = 0; ks < KS2; ++ks) {
       const int c = 32 * ks + 8 * g;
-      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
-      df[ks] = __builtin_bit_cast(bf16x8, load16(ro, c < p.hd ? (uint32_t)q * d2 + hcol + 2 * c : OUTSIDE));
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(c < p.hd, (uint32_t)q * ld2 + hcol + 2 * c)));
+      df[ks] = __builtin_bit_cast(bf16x8, load16(ro, only(c < p.hd, (uint32_t)q * d2 + hcol + 2 * c)));
     }
-    f32x4 next[T];
+    f32x4 sc[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) next[t] = load4f(rb, boff + 64 * t);
+    for (int t = 0; t < T; ++t) sc[t] = load4f(rb, boff + 64 * t);
     sg.put(smem);
     __syncthreads();
-    for (int s2 = 0; s2 < 2 * nseg; ++s2) {
-      const bool second = s2 >= nseg, more = s2 + 1 < 2 * nseg;
-      const int k0 = (second ? s2 - nseg : s2) * Seg::SEG, kn = k0 + Seg::SEG < len ? k0 + Seg::SEG : 0;
-      if (more) sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, kn, len, p.hd / 8);
-      if (s2 == nseg) delta = quarters_sum(delta);
-      const char* imgK = smem + (s2 & 1) * 2 * Seg::IMG;
-      const char* imgV = imgK + Seg::IMG;
-      f32x4 sc[T], dp[T];
+    int buf = 0;
+    auto pass = [&](auto second) {
+      for (int k0 = 0; k0 < len; k0 += Seg::SEG) {
+        const bool last = k0 + Seg::SEG >= len, more = !last || !second;
+        const int kn = last && !second ? 0 : k0 + Seg::SEG;
+        sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, kn, len, p.hd / 8);
+        __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to their use)
+        const char* imgK = smem + buf * 2 * Seg::IMG;
+        const char* imgV = imgK + Seg::IMG;
+        f32x4 dp[T];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        sc[t] = next[t];
-        dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (more) next[t] = load4f(rb, boff + (uint32_t)(kn + 16 * t) * 4);
+        for (int t = 0; t < T; ++t) {
+          dp[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS2; ++ks) {
-          sc[t] = mfma16(row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
-          dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
+          for (int ks = 0; ks < KS2; ++ks) {
+            sc[t] = mfma16(row_frag(imgK, 16 * t + ql, 4 * ks + g), qf[ks], sc[t]);
+            dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
+          }
         }
-      }
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
-      if (k0 + Seg::SEG > len) {
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (k0 + 16 * t + 4 * g + r >= len) sc[t][r] = 0.f;
-      }
-      if (!second) {
+          for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+        if (last) {
 #pragma unroll
-        for (int t = 0; t < T; ++t)
+          for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) delta += sc[t][r] * dp[t][r];
-      } else {
+            for (int r = 0; r < 4; ++r)
+              if (k0 + 16 * t + 4 * g + r >= len) sc[t][r] = 0.f;
+        }
 #pragma unroll
         for (int t = 0; t < T; t += 2) {
           union { uint32_t u[4]; bf16x8 v; } pf;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            f32x4 x = sc[t + k] * (dp[t + k] - delta);
-            pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
-            pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
-          }
+            f32x4& x = sc[t + k];
+            if constexpr (second) {
+              x = x * (dp[t + k] - delta);
+              pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
+              pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
+            } else {
 #pragma unroll
-          for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dq[eb]);
+              for (int r = 0; r < 4; ++r) delta += x[r] * dp[t + k][r];
+            }
+            x = load4f(rb, boff + (uint32_t)(kn + 16 * (t + k)) * 4);
+          }
+          if constexpr (second) {
+#pragma unroll
+            for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dq[eb]);
+          }
+        }
+        if (more) {
+          buf ^= 1;
+          sg.put(smem + buf * 2 * Seg::IMG);
+          __syncthreads();
         }
       }
-      if (more) {
-        sg.put(smem + ((s2 + 1) & 1) * 2 * Seg::IMG);
-        __syncthreads();
-      }
-    }
+    };
+    pass(std::false_type{});
+    delta = quarters_sum(delta);
+    pass(std::true_type{});
   }
   if (q >= len) {
     delta = 0.f;
@@ -500,12 +514,12 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
 
 // dK and dV: a wave owns 16 keys (on the lane; queries in registers), Q and dO stream.  16 and not 32 keys a wave: 64 accumulators fewer leave room for four waves
 // a SIMD instead of two, which is worth more than the LDS reads that 32 keys would share
-template <int W, int KS2>
+template <int W, int KS2, bool ONE>
 __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(const BiasAttnParams p) {
   typedef Segment<W, 2 * KS2> Seg;
   constexpr int T = Seg::SEG / 16;
-  __shared__ __attribute__((aligned(16))) char smem[4 * Seg::IMG];
-  __shared__ float stats[2][2][Seg::SEG];  // of the two buffers: -lse log2 e, delta
+  __shared__ __attribute__((aligned(16))) char smem[(ONE ? 2 : 4) * Seg::IMG];
+  __shared__ float stats[ONE ? 1 : 2][64 * W];  // of the two buffers: SEG times -lse log2 e, SEG times delta (and what the other threads write)
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
@@ -524,14 +538,12 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   float st = 0.f;
   auto fetch = [&](int q0) {
     sg.fetch(rs, ld2, hcol, rd, d2, hcol, q0, len, p.hd / 8);
-    if (threadIdx.x < 2 * Seg::SEG) {
-      const int i = threadIdx.x % Seg::SEG;
-      st = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, (uint32_t)(q0 + i + (threadIdx.x < Seg::SEG ? 0 : p.Np)) * 4, 0, 0));
-    }
+    const uint32_t row = q0 + threadIdx.x % Seg::SEG + (threadIdx.x < Seg::SEG ? 0 : p.Np);
+    st = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, threadIdx.x < 2 * Seg::SEG ? row * 4 : OUTSIDE, 0, 0));
   };
   auto put = [&](int buf) {
     sg.put(smem + buf * 2 * Seg::IMG);
-    if (threadIdx.x < 2 * Seg::SEG) (&stats[buf][0][0])[threadIdx.x] = st;
+    stats[buf][threadIdx.x] = st;
   };
   f32x4 dk[2 * KS2], dv[2 * KS2];
 #pragma unroll
@@ -542,8 +554,8 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
 #pragma unroll
     for (int ks = 0; ks < KS2; ++ks) {
       const int c = 32 * ks + 8 * g;
-      kf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)key * ld2 + d2 + hcol + 2 * c : OUTSIDE));
-      vf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)key * ld2 + 2 * d2 + hcol + 2 * c : OUTSIDE));
+      kf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(c < p.hd, (uint32_t)key * ld2 + d2 + hcol + 2 * c)));
+      vf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(c < p.hd, (uint32_t)key * ld2 + 2 * d2 + hcol + 2 * c)));
     }
     f32x4 sc[T];
     auto load_bias = [&](int t, int q0) {
@@ -554,10 +566,9 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
     for (int t = 0; t < T; ++t) load_bias(t, 16 * t);
     put(0);
     __syncthreads();
-    for (int s = 0; s < nseg; ++s) {
-      const bool more = s + 1 < nseg;
+    for (int s = 0; s < (ONE ? 1 : nseg); ++s) {
       const int q0 = s * Seg::SEG;
-      if (more) fetch(q0 + Seg::SEG);
+      if constexpr (!ONE) fetch(q0 + Seg::SEG);
       const char* imgQ = smem + (s & 1) * 2 * Seg::IMG;
       const char* imgD = imgQ + Seg::IMG;
 #pragma unroll
@@ -572,8 +583,8 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
               sc[t + k] = mfma16(row_frag(imgQ, 16 * (t + k) + ql, 4 * ks + g), kf[ks], sc[t + k]);
               dp = mfma16(row_frag(imgD, 16 * (t + k) + ql, 4 * ks + g), vf[ks], dp);
             }
-            const f32x4 nl = *reinterpret_cast<const f32x4*>(&stats[s & 1][0][16 * (t + k) + 4 * g]);
-            const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][1][16 * (t + k) + 4 * g]);
+            const f32x4 nl = *reinterpret_cast<const f32x4*>(&stats[s & 1][16 * (t + k) + 4 * g]);
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][Seg::SEG + 16 * (t + k) + 4 * g]);
             float pr[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -589,7 +600,6 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
             pf.u[2 * k + 1] = pack_bf16x2(pr[2], pr[3]);
             df.u[2 * k] = pack_bf16x2(dp[0], dp[1]);
             df.u[2 * k + 1] = pack_bf16x2(dp[2], dp[3]);
-            if (more) load_bias(t + k, q0 + Seg::SEG + 16 * (t + k));
           }
 #pragma unroll
           for (int eb = 0; eb < 2 * KS2; ++eb) {
@@ -597,8 +607,12 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
             dk[eb] = mfma16(lds_tr_pair(imgQ, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), df.v, dk[eb]);
           }
         }
+        if constexpr (!ONE) {
+          load_bias(t, q0 + Seg::SEG + 16 * t);
+          load_bias(t + 1, q0 + Seg::SEG + 16 * (t + 1));
+        }
       }
-      if (more) {
+      if (!ONE && s + 1 < nseg) {
         put((s + 1) & 1);
         __syncthreads();
       }
@@ -646,13 +660,17 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
   float nln, deltan;
   auto fetch = [&](int b) {  // an image's operands, one image ahead
     const int len = length_of(p, b);
-    const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)p.N * p.ld * 2);
-    sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, k0, len);
-    load_frags<KS>(qn, p.qkv, (size_t)b * p.N + q, p.ld, h * hd, L.half, q < len);
-    load_frags<KS>(dn, p.d_o, (size_t)b * p.N + q, p.d, h * hd, L.half, q < len);
-    const float* st = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + q;
-    nln = q < len ? st[0] : -INFINITY;
-    deltan = q < len ? st[p.Np] : 0.f;
+    const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, col = (uint32_t)(h * hd + 8 * L.half) * 2;
+    const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2), rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
+    const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
+    sg.fetch(rs, ld2, ck, rs, ld2, cv, k0, len);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qn[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(q < len, (uint32_t)q * ld2 + col + 32 * ks)));
+      dn[ks] = __builtin_bit_cast(bf16x8, load16(rd, only(q < len, (uint32_t)q * d2 + col + 32 * ks)));
+    }
+    nln = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)q * 4), 0, 0));
+    deltan = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)(q + p.Np) * 4), 0, 0));
   };
   if (b0 < b1) {
     fetch(b0);
@@ -669,7 +687,8 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
       df[ks] = dn[ks];
     }
     const float nl = nln, delta = deltan;
-    if (more) fetch(b + 1);
+    fetch(more ? b + 1 : b);  // (the last one again)
+    __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to their use)
     const char* imgK = smem + ((b - b0) & 1) * 2 * Seg::IMG;
     const char* imgV = imgK + Seg::IMG;
     f32x16 sc[T], dp[T];
@@ -768,8 +787,8 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
 #pragma unroll
     for (int ks = 0; ks < KS2; ++ks) {
       const int c = 32 * ks + 8 * g;
-      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, c < p.hd ? (uint32_t)q * ld2 + hcol + 2 * c : OUTSIDE));
-      df[ks] = __builtin_bit_cast(bf16x8, load16(rd, c < p.hd ? (uint32_t)q * d2 + hcol + 2 * c : OUTSIDE));
+      qf[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(c < p.hd, (uint32_t)q * ld2 + hcol + 2 * c)));
+      df[ks] = __builtin_bit_cast(bf16x8, load16(rd, only(c < p.hd, (uint32_t)q * d2 + hcol + 2 * c)));
     }
     lse = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rl, (uint32_t)q * 4, 0, 0));
   };
@@ -982,37 +1001,33 @@ int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
   }
 }
 
-// waves a workgroup: as many as a short sequence has tiles, four at the most
-int waves_for(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 template <typename F>
-int launch_waves(BiasAttnParams& p, int W, int rows, F kfn, hipStream_t st) {  // rows: of a wave
+int launch_waves(BiasAttnParams p, int W, int rows, F kfn, hipStream_t st) {  // rows: of a wave
   p.blocks = (p.N + rows * W - 1) / (rows * W);
   const long grid = (long)p.B * p.H * p.blocks;
   SAVIT_CHECK_ARG(grid <= 0x7fffffffL);
   hipLaunchKernelGGL(kfn, dim3((unsigned)grid), dim3(64 * W), 0, st, p);
   SAVIT_LAUNCH_RET();
 }
+// kernels with 16 rows a wave: as many waves as a short sequence has tiles, four at the most
+template <typename A, typename B, typename C, typename D>
+int launch_sixteen(const BiasAttnParams& p, A one_wave, B two, C segment, D many, hipStream_t st) {
+  if (p.N <= 16) return launch_waves(p, 1, 16, one_wave, st);
+  if (p.N <= 32) return launch_waves(p, 2, 16, two, st);
+  return p.N <= 64 ? launch_waves(p, 4, 16, segment, st) : launch_waves(p, 4, 16, many, st);
+}
+#define BIAS_ATTN_SIXTEEN(K)                                                                        \
+  (p.hd <= 32 ? launch_sixteen(p, K<1, 1, true>, K<2, 1, true>, K<4, 1, true>, K<4, 1, false>, st)  \
+              : launch_sixteen(p, K<1, 2, true>, K<2, 2, true>, K<4, 2, true>, K<4, 2, false>, st))
 int launch_fwd(BiasAttnParams p, hipStream_t st) {
-  const int W = waves_for(p.N);
   // 32 queries a wave where heads are wide, sequences long and the grid is two workgroups a CU or more, else 16 (heads of 64; 32 against 16 a wave:
   // [128 x 12 x 197] 54.5 against 62.8 us, [16 x 12 x 197] 11.9 / 11.7, [8 x 16 x 577] 31.4 / 33.9, [4 x 16 x 577] 22.1 / 21.6, [2 x 8 x 1500] 39.7 / 34.6,
   // [1024 x 12 x 49] 85.2 / 64.1)
   if (p.N > 64 && p.hd > 32 && (long)p.B * p.H * ((p.N + 127) / 128) >= 2L * CUS)
     return p.hd == 48 ? launch_waves(p, 4, 32, bias_attn_fwd_kernel<3>, st) : launch_waves(p, 4, 32, bias_attn_fwd_kernel<4>, st);
-  if (p.hd <= 32)
-    return W == 1 ? launch_waves(p, 1, 16, bias_attn_fwd16_kernel<1, 1>, st)
-                  : W == 2 ? launch_waves(p, 2, 16, bias_attn_fwd16_kernel<2, 1>, st) : launch_waves(p, 4, 16, bias_attn_fwd16_kernel<4, 1>, st);
-  return W == 1 ? launch_waves(p, 1, 16, bias_attn_fwd16_kernel<1, 2>, st)
-                : W == 2 ? launch_waves(p, 2, 16, bias_attn_fwd16_kernel<2, 2>, st) : launch_waves(p, 4, 16, bias_attn_fwd16_kernel<4, 2>, st);
+  return BIAS_ATTN_SIXTEEN(bias_attn_fwd16_kernel);
 }
-int launch_dkv(BiasAttnParams p, hipStream_t st) {
-  const int W = waves_for(p.N);
-  if (p.hd <= 32)
-    return W == 1 ? launch_waves(p, 1, 16, bias_attn_dkv_kernel<1, 1>, st)
-                  : W == 2 ? launch_waves(p, 2, 16, bias_attn_dkv_kernel<2, 1>, st) : launch_waves(p, 4, 16, bias_attn_dkv_kernel<4, 1>, st);
-  return W == 1 ? launch_waves(p, 1, 16, bias_attn_dkv_kernel<1, 2>, st)
-                : W == 2 ? launch_waves(p, 2, 16, bias_attn_dkv_kernel<2, 2>, st) : launch_waves(p, 4, 16, bias_attn_dkv_kernel<4, 2>, st);
-}
+int launch_dkv(const BiasAttnParams& p, hipStream_t st) { return BIAS_ATTN_SIXTEEN(bias_attn_dkv_kernel); }
 
 }  // namespace
 
