@@ -185,17 +185,21 @@ __device__ __forceinline__ float quarters_max(float v) {
 }
 // Columns of the 2 KS2 accumulators of a lane's row (16 eb + 4 (lane / 16) ..), scaled, rounded and stored 16 bytes at a time: lanes 16 apart trade pieces of
 // two accumulators first.  Columns >= hd are skipped.
-template <int KS2>
-__device__ __forceinline__ void store_row16(bf16_t* row, const f32x4 (&o)[2 * KS2], int g, int hd, float sc) {
+template <int KS2, typename F>
+__device__ __forceinline__ void pieces_of_row16(const f32x4 (&o)[2 * KS2], int g, float sc, F store) {
 #pragma unroll
   for (int eb = 0; eb < 2 * KS2; eb += 2) {
     uint32_t a0 = pack_bf16x2(o[eb][0] * sc, o[eb][1] * sc), a1 = pack_bf16x2(o[eb][2] * sc, o[eb][3] * sc);
     uint32_t b0 = pack_bf16x2(o[eb + 1][0] * sc, o[eb + 1][1] * sc), b1 = pack_bf16x2(o[eb + 1][2] * sc, o[eb + 1][3] * sc);
     const auto r0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false), r1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
-    const unsigned x0 = r0[0], y0 = r0[1], x1 = r1[0], y1 = r1[1];
-    const int col = (g & 1) ? 16 * (eb + 1) + 4 * (g - 1) : 16 * eb + 4 * g;
-    if (col < hd) *reinterpret_cast<uint4*>(row + col) = make_uint4(x0, x1, y0, y1);
+    store((g & 1) ? 16 * (eb + 1) + 4 * (g - 1) : 16 * eb + 4 * g, u32x4{(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]});
   }
+}
+template <int KS2>
+__device__ __forceinline__ void store_row16(bf16_t* row, const f32x4 (&o)[2 * KS2], int g, int hd, float sc) {
+  pieces_of_row16<KS2>(o, g, sc, [&](int col, u32x4 v) {
+    if (col < hd) *reinterpret_cast<u32x4*>(row + col) = v;
+  });
 }
 
 // workgroup -> (head, image, block): all blocks and images of a head in a row, and consecutive numbers on one XCD, so that its L2 holds the
@@ -736,8 +740,8 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
 template <int KT, int KS2, bool DB>
 __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_kernel(const BiasAttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int IMG = KT * 16 * ROWB, PIECES = KT * 16 * 8 * 2, RES_GROUPS = KT <= 6 ? 1 : KT <= 8 ? 2 : 4;
-  constexpr bool AHEAD = KT <= 8;  // the next image's bias and queries ahead too: longer rows leave no registers for them (14 tiles: 93 spills, twice the time)
+  constexpr int KE = KT + KT % 2, IMG = KE * 16 * ROWB, PIECES = KE * 16 * 8 * 2, RES_GROUPS = KT <= 6 ? 1 : KT <= 8 ? 2 : 4;
+  constexpr bool AHEAD = KT <= 8;  // the next image's bias ahead too: longer rows leave no registers for them (14 tiles: 93 spills, twice the time)
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int t0 = xcd_remap(blockIdx.x, gridDim.x);
@@ -752,7 +756,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
 
   // the next image's K and V rows: PIECES 16-byte pieces in RES_GROUPS groups ; rows at and beyond its length are out of the descriptor's range (zero),
   // columns at and beyond hd repeat others (they meet zeros of the query fragments, or output rows that are not stored)
-  constexpr int LEAST = 64 * (KT <= 8 ? KT - 1 : KT / 2), MAXL = (PIECES / RES_GROUPS + LEAST - 1) / LEAST;  // threads, pieces a thread and group
+  constexpr int LEAST = 64 * (KE <= 8 ? KE - 1 : KE / 2), MAXL = (PIECES / RES_GROUPS + LEAST - 1) / LEAST;  // threads, pieces a thread and group
   u32x4 st[MAXL];
   const int chunks = p.hd / 8;
   auto thread = [] {  // opaque: the offsets below are computed where they are used, 16 of them held over the loop are 16 registers too many
@@ -864,6 +868,10 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
       union { uint32_t u[4]; bf16x8 v; } f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        if (t + k == KT) {
+          f.u[2] = f.u[3] = 0;
+          break;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           sc[t + k][r] *= dp[t + k][r] - delta;
@@ -876,23 +884,23 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
       for (int eb = 0; eb < 2 * KS2; ++eb)
         dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), f.v, dq[eb]);
       if constexpr (RES_GROUPS == 4) {
-        if (t == KT / 6 * 2) { put(1, buf ^ 1); fetch(rn, 2); }
-        if (t == KT / 6 * 4) { put(2, buf ^ 1); fetch(rn, 3); }
+        if (t == KE / 6 * 2) { put(1, buf ^ 1); fetch(rn, 2); }
+        if (t == KE / 6 * 4) { put(2, buf ^ 1); fetch(rn, 3); }
       }
       if constexpr (AHEAD) {  // into registers that have just become free
 #pragma unroll
         for (int k = 0; k < 2; ++k) sc[t + k] = load4f(rb, boff + 64 * (t + k));
-        if (t == KT / 4 * 2) load_queries(bn, lenn);
       }
+      if (AHEAD && t == KT / 4 * 2) load_queries(bn, lenn);
     }
-    if (q < p.N) store_row16<KS2>(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd, dq, g, p.hd, p.dq_scale);
+    const auto ro = rsrc_of(p.dqkv + (size_t)b * p.N * p.ld, (size_t)p.N * ld2);
+    pieces_of_row16<KS2>(dq, g, p.dq_scale, [&](int col, u32x4 v) { store16(ro, only(q < p.N && col < p.hd, (uint32_t)q * ld2 + hcol + 2 * col), v); });
     {  // statistics of the queries, and of the padding up to Np (fewer than three times the rows here) that the dK / dV kernel's tiles read
       const int row = q + g * (int)(blockDim.x >> 6) * 16 * p.blocks;
-      if (row < p.Np) {
-        float* s = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + row;
-        s[0] = g == 0 ? nl : -INFINITY;
-        s[p.Np] = g == 0 ? delta : 0.f;
-      }
+      const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
+      const uint32_t off = only(row < p.Np, (uint32_t)row * 4), off2 = only(row < p.Np, (uint32_t)(row + p.Np) * 4);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, g == 0 ? nl : -INFINITY), rt, off, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, g == 0 ? delta : 0.f), rt, off2, 0, 0);
     }
     put(RES_GROUPS - 1, buf ^ 1);
     if constexpr (!AHEAD) load_queries(bn, lenn);
@@ -981,7 +989,7 @@ template <int KT, int KS2, bool DB>
 int launch_resident_k(const BiasAttnParams& p, hipStream_t st) {
   auto kfn = bias_attn_dq_resident_kernel<KT, KS2, DB>;
   SAVIT_LDS_ONCE(kfn);
-  hipLaunchKernelGGL(kfn, dim3((unsigned)(p.parts * p.H * p.blocks)), dim3(64 * resident_waves(p.N)), (size_t)4 * KT * 16 * ROWB, st, p);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)(p.parts * p.H * p.blocks)), dim3(64 * resident_waves(p.N)), (size_t)4 * (KT + KT % 2) * 16 * ROWB, st, p);
   SAVIT_LAUNCH_RET();
 }
 template <int KT>
@@ -990,13 +998,17 @@ int launch_resident_kt(const BiasAttnParams& p, bool db, hipStream_t st) {
   return db ? launch_resident_k<KT, 2, true>(p, st) : launch_resident_k<KT, 2, false>(p, st);
 }
 int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
-  switch ((p.N + 31) / 32) {
-    case 1: return launch_resident_kt<2>(p, db, st);
-    case 2: return launch_resident_kt<4>(p, db, st);
-    case 3: return launch_resident_kt<6>(p, db, st);
-    case 4: return launch_resident_kt<8>(p, db, st);
-    case 5: return launch_resident_kt<10>(p, db, st);
-    case 6: return launch_resident_kt<12>(p, db, st);
+  const int nq = (p.N + 15) / 16;  // to an even number up to eight (2 % of the time); beyond, a tile less is 12 registers less, where some are spilled
+  switch (nq) {
+    case 1: case 2: return launch_resident_kt<2>(p, db, st);
+    case 3: case 4: return launch_resident_kt<4>(p, db, st);
+    case 5: case 6: return launch_resident_kt<6>(p, db, st);
+    case 7: case 8: return launch_resident_kt<8>(p, db, st);
+    case 9: return launch_resident_kt<9>(p, db, st);
+    case 10: return launch_resident_kt<10>(p, db, st);
+    case 11: return launch_resident_kt<11>(p, db, st);
+    case 12: return launch_resident_kt<12>(p, db, st);
+    case 13: return launch_resident_kt<13>(p, db, st);
     default: return launch_resident_kt<14>(p, db, st);
   }
 }
