@@ -10,6 +10,13 @@
 // in-register reductions plus an exchange between the lanes of a query, and the score tile is the next product's operand without an LDS round trip.
 // The bias tile is fetched one tile ahead and is the INITIAL value of the score accumulators: adding it costs nothing.  W = 1, 2 or 4 by the sequence
 // length, so that short sequences leave no wave idle.
+// Rounded to bf16: P and dS as operands of the matrix instructions (O, dQ, dK, dV are bf16 themselves; P stays below 2^8 and is divided by its fp32 sum at
+// the end), O and the gradients when stored.  Scores, statistics, delta, sums and dbias are fp32.
+//
+// What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (55 measured) and 55 backward (99 dQ and dbias, 94 dK and dV), the
+// products 13 and 31: with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
+// goes into (dK / dV: vector issue 39 %, LDS 27 %, matrix pipe 17 % busy).  One segment or long rows come nearer: [2048 x 4 x 49], heads of 32,
+// 27 us forward (bytes 21), 37 dK and dV (31).
 //
 // delta is summed from the fp32 probabilities, in a loop of its own over the keys, not taken as rowsum(dO . O): O is rounded to bf16, and the table
 // gradient that dS feeds is an fp32 parameter gradient (2^-9 of O in delta is 1e-4 of the gradient; this way it is 1e-6).
@@ -72,7 +79,7 @@ __device__ __forceinline__ int length_of(const BiasAttnParams& p, int b) {
 
 // Byte offset of 16-byte chunk c of an image's row (ROWB bytes).  The XOR by row bits 1..3 serves both shapes without bank conflicts: row fragments of
 // 16 rows x 4 chunks (a pass of ds_read_b128 takes rows 0-3 and 12-15 of one chunk with rows 4-11 of its neighbour) or 32 rows x 2, and transposed reads
-// of 16 rows x 2 chunks or 4 rows x 4.  (attention.hip's order of the bits is made for its 32-row tiles; 16 rows of it conflict: 22 % of dK / dV's LDS time.)
+// of 16 rows x 2 chunks or 4 rows x 4.  (attention.hip's order of the bits is made for its 32-row tiles; 16 rows of it conflict: 38 % of dK / dV's LDS cycles.)
 __device__ __forceinline__ int swizzle(int row) { return (row >> 1 & 1) << 2 | ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); }
 __device__ __forceinline__ int at_chunk(int row, int c) { return row * ROWB + ((c ^ swizzle(row)) << 4); }
 __device__ __forceinline__ bf16x8 row_frag(const char* img, int row, int c) { return *reinterpret_cast<const bf16x8*>(img + at_chunk(row, c)); }
@@ -937,7 +944,9 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
 
 int padded(int N) { return (N + 63) / 64 * 64; }
 
-// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel
+// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 182 us against 273 of the
+// streaming kernels at [128 x 12 x 197], 82 / 122 at [2048 x 4 x 49], 80 / 118 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 165 /
+// 194, 76 / 82, 67 / 80, 18 / 17.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
 constexpr int RESIDENT_N = 224;
 bool resident(int N) { return N <= RESIDENT_N; }
 constexpr int CUS = 256;  // not the device's or a budget's: the parts set the order of the bias gradient's sum
@@ -998,7 +1007,7 @@ int launch_resident_kt(const BiasAttnParams& p, bool db, hipStream_t st) {
   return db ? launch_resident_k<KT, 2, true>(p, st) : launch_resident_k<KT, 2, false>(p, st);
 }
 int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
-  const int nq = (p.N + 15) / 16;  // to an even number up to eight (2 % of the time); beyond, a tile less is 12 registers less, where some are spilled
+  const int nq = (p.N + 15) / 16;  // rounded to an even number up to eight; beyond, a tile less is 12 registers less, where they are all in use (197 tokens: 119 us with 14, 99 with 13)
   switch (nq) {
     case 1: case 2: return launch_resident_kt<2>(p, db, st);
     case 3: case 4: return launch_resident_kt<4>(p, db, st);
@@ -1033,8 +1042,8 @@ int launch_sixteen(const BiasAttnParams& p, A one_wave, B two, C segment, D many
               : launch_sixteen(p, K<1, 2, true>, K<2, 2, true>, K<4, 2, true>, K<4, 2, false>, st))
 int launch_fwd(BiasAttnParams p, hipStream_t st) {
   // 32 queries a wave where heads are wide, sequences long and the grid is two workgroups a CU or more, else 16 (heads of 64; 32 against 16 a wave:
-  // [128 x 12 x 197] 54.5 against 62.8 us, [16 x 12 x 197] 11.9 / 11.7, [8 x 16 x 577] 31.4 / 33.9, [4 x 16 x 577] 22.1 / 21.6, [2 x 8 x 1500] 39.7 / 34.6,
-  // [1024 x 12 x 49] 85.2 / 64.1)
+  // [128 x 12 x 197] 52 against 66 us, [32 x 12 x 197] 17.4 / 20.3, [16 x 12 x 197] 11.7 / 11.4, [8 x 16 x 577] 32 / 33, [4 x 16 x 577] 22.9 / 21.2,
+  // [8 x 8 x 1500] 80 / 94, [1 x 8 x 1500] 32 / 24.5; up to 64 tokens one segment is all there is and 16 are never slower)
   if (p.N > 64 && p.hd > 32 && (long)p.B * p.H * ((p.N + 127) / 128) >= 2L * CUS)
     return p.hd == 48 ? launch_waves(p, 4, 32, bias_attn_fwd_kernel<3>, st) : launch_waves(p, 4, 32, bias_attn_fwd_kernel<4>, st);
   return BIAS_ATTN_SIXTEEN(bias_attn_fwd16_kernel);

@@ -8,6 +8,8 @@
 //
 // Bound by HBM: forward reads and writes a row once, backward reads the cotangent row and the saved queries and keys and writes a row;
 // statistics are recomputed from x, which is cheaper than to store and load them.  All arithmetic is in fp32, one rounding at the store.
+// Measured, bf16: [128 x 197 rows, 3 x 12 heads of 64] forward 48 us (232 MB: 4.8 TB/s, a large copy reaches 5.0), backward 71 us (310 MB, 4.4 TB/s) and
+// 5 us for the weights' sums; [16384 rows, 3 x 8 heads of 48] 19 us (75 MB, 4.0 TB/s); 4 rows: one launch.
 //
 // Layout: G = 1..16 lanes per head, each with 8 columns of the head's lower half and the 8 columns hd/2 above them, so that both
 // kinds of pairs lie in one lane and a reduction takes log2 G lane exchanges.  A group of G lanes owns a fixed chunk of HS heads and walks over rows:
