@@ -266,7 +266,8 @@ int savit_attention_bwd(const void* qkv, const void* o, const void* d_o, const f
  *   (NULL: no rotation); pairs are (e, e + head_dim/2), or (2e, 2e+1) when interleaved; angle 0 leaves a pair alone (a class token, a partial
  *   rotation).  positions int32 [rows] (NULL: row mod N); a position outside [0, table_rows) makes its row NaN.  head_dim % 16 == 0, <= 256.
  * savit_qk_norm_rope_bwd: dqkv = cotangent of the output, qkv = the forward's INPUT; out receives the gradient of that input (value columns
- *   copied; out == dqkv: in place, values left alone; out must not be qkv); dwq, dwk fp32 [head_dim] are ACCUMULATED, in a fixed order.
+ *   copied; out == dqkv: in place, values left alone; out must not be qkv); dwq, dwk fp32 [head_dim] are ACCUMULATED, in a fixed order
+ *   (two buffers, also where wq == wk).
  *   workspace: savit_qk_norm_rope_bwd_workspace_bytes(H, Hk, head_dim). */
 int savit_qk_norm_rope_fwd(const void* qkv, long ld, const float* wq, const float* wk, const float* table, int table_rows, const int* positions,
                            void* out, long ld_out, int rows, int N, int H, int Hk, int head_dim, int is_bf16, float eps, float q_scale, int center,
@@ -288,7 +289,7 @@ long savit_relpos_bias_bwd_workspace_bytes(int N, int H, int buckets);
  *   lens int32 [B] (NULL: all N): keys and queries at or beyond lens[b] (clamped to [0, N]) take no part; their rows of o are zero, their lse is
  *   -inf - as those of a query whose bias masks every key.  A bias of -inf masks; so does float's or bfloat16's lowest value.  lse is required.
  * savit_bias_attention_bwd: dqkv as in savit_attention_bwd (rows of padding are zero); dbias fp32 [H, N, ld_bias] (nullable) = the sum of dS over
- *   the batch, in a fixed order.  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
+ *   the batch, in a fixed order (not in bias's place: later kernels read that).  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
  *   head_dim 16, 32, 48 or 64; N <= 32 768, and one image's rows and one head's bias each below 4 GiB; d_o, o compact [B*N, H*head_dim]. */
 int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
                              int ld_bias, void* stream);

@@ -1054,7 +1054,7 @@ int launch_dkv(const BiasAttnParams& p, hipStream_t st) { return BIAS_ATTN_SIXTE
 
 extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
                                         int ld_bias, void* stream) {
-  SAVIT_CHECK_ARG(qkv && bias && o && lse && size_ok(B, N, H, head_dim, ld_qkv, ld_bias) && aligned16(qkv) && aligned16(bias) && aligned16(o));
+  SAVIT_CHECK_ARG(qkv && bias && o && lse && size_ok(B, N, H, head_dim, ld_qkv, ld_bias) && o != qkv && aligned16(qkv) && aligned16(bias) && aligned16(o));
   if (B == 0) return SAVIT_OK;
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.o = (bf16_t*)o; p.lse = lse;
@@ -1071,7 +1071,7 @@ extern "C" long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, in
 extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, const int* lens, const void* d_o, const float* lse, void* dqkv, float* dbias, int B,
                                         int N, int H, int head_dim, int ld_qkv, int ld_bias, float dq_scale, void* workspace, long workspace_bytes,
                                         void* stream) {
-  SAVIT_CHECK_ARG(qkv && bias && d_o && lse && dqkv && size_ok(B, N, H, head_dim, ld_qkv, ld_bias) && dqkv != qkv);
+  SAVIT_CHECK_ARG(qkv && bias && d_o && lse && dqkv && size_ok(B, N, H, head_dim, ld_qkv, ld_bias) && dqkv != qkv && dqkv != d_o && dbias != bias);
   SAVIT_CHECK_ARG(aligned16(qkv) && aligned16(bias) && aligned16(d_o) && aligned16(dqkv) && aligned16(dbias));
   const hipStream_t st = (hipStream_t)stream;
   if (B == 0) return dbias ? (int)SAVIT_EINVAL : SAVIT_OK;  // no image: there is no gradient to write

@@ -494,6 +494,7 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
                                       int head_dim, int is_bf16, float eps, float q_scale, int center, int interleaved, void* workspace,
                                       long workspace_bytes, void* stream) {
   SAVIT_CHECK_ARG(dqkv && qkv && wq && wk && out && dwq && dwk && geometry_ok(rows, N, H, Hk, head_dim) && eps >= 0.f && out != qkv);
+  SAVIT_CHECK_ARG((uintptr_t)dwq >= (uintptr_t)(dwk + head_dim) || (uintptr_t)dwk >= (uintptr_t)(dwq + head_dim));  // each is added to by its own blocks
   const long cols = (long)(H + 2 * Hk) * head_dim;
   const int q16 = is_bf16 ? 8 : 4;
   SAVIT_CHECK_ARG(ld >= cols && ld_out >= cols && ld_dqkv >= cols && ld % q16 == 0 && ld_out % q16 == 0 && ld_dqkv % q16 == 0);

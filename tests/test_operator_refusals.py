@@ -20,7 +20,7 @@ def L():
 
 def qkn(L, bwd=False, **kw):
     a = dict(x=P, ld=192, wq=P, wk=P, table=P, T=50, pos=None, out=2 * P, ldo=192, rows=50, N=50, H=1, Hk=1, hd=64, bf16=1, eps=1e-6, dq=3 * P, ldd=192,
-             dwq=P, dwk=P, ws=P, bytes=1 << 30)
+             dwq=P, dwk=P + 256, ws=P, bytes=1 << 30)
     a.update(kw)
     if bwd:
         return L.savit_qk_norm_rope_bwd(a["dq"], a["ldd"], a["x"], a["ld"], a["wq"], a["wk"], a["table"], a["T"], a["pos"], a["out"], a["ldo"], a["dwq"], a["dwk"], a["rows"],
@@ -37,7 +37,7 @@ def test_qk_norm_rope(L, bad):
     assert qkn(L, bwd=True, **bad) == EINVAL
 
 
-@pytest.mark.parametrize("bad", [dict(dq=None), dict(ldd=100), dict(ldd=196), dict(dwq=None), dict(dwk=None), dict(dq=3 * P + 2), dict(ws=P + 1), dict(out=P, dq=3 * P),
+@pytest.mark.parametrize("bad", [dict(dq=None), dict(ldd=100), dict(ldd=196), dict(dwq=None), dict(dwk=None), dict(dq=3 * P + 2), dict(ws=P + 1), dict(out=P, dq=3 * P), dict(dwk=P), dict(dwk=P + 252),
                                  dict(ws=None, rows=1 << 20, N=1 << 20, T=1 << 20)])
 def test_qk_norm_rope_bwd(L, bad):
     assert qkn(L, bwd=True, **bad) == EINVAL
@@ -70,7 +70,7 @@ def test_relpos(L):
 
 
 def attn(L, bwd=False, **kw):
-    a = dict(qkv=P, bias=P, lens=None, o=P, lse=P, do=P, dqkv=2 * P, dbias=P, B=2, N=50, H=3, hd=64, ld=576, ldb=52, ws=P, n=1 << 30)
+    a = dict(qkv=P, bias=P, lens=None, o=3 * P, lse=P, do=P, dqkv=2 * P, dbias=3 * P, B=2, N=50, H=3, hd=64, ld=576, ldb=52, ws=P, n=1 << 30)
     a.update(kw)
     if bwd:
         return L.savit_bias_attention_bwd(a["qkv"], a["bias"], a["lens"], a["do"], a["lse"], a["dqkv"], a["dbias"], a["B"], a["N"], a["H"], a["hd"], a["ld"], a["ldb"], 1.0, a["ws"],
@@ -85,17 +85,17 @@ def test_bias_attention(L, bad):
     assert attn(L, bwd=True, **bad) == EINVAL
 
 
-@pytest.mark.parametrize("bad", [dict(do=None), dict(dqkv=None), dict(dqkv=P), dict(ws=None), dict(ws=P + 4), dict(do=P + 2), dict(dqkv=2 * P + 8), dict(dbias=P + 8), dict(B=0)])
+@pytest.mark.parametrize("bad", [dict(do=None), dict(dqkv=None), dict(dqkv=P), dict(ws=None), dict(ws=P + 4), dict(do=P + 2), dict(dqkv=2 * P + 8), dict(dbias=3 * P + 8), dict(dbias=P), dict(do=2 * P), dict(B=0)])
 def test_bias_attention_bwd(L, bad):
     assert attn(L, bwd=True, **bad) == EINVAL
 
 
 def test_bias_attention_workspace(L):
-    assert attn(L, o=None) == EINVAL and attn(L, o=P + 2) == EINVAL and attn(L, B=0) == 0
+    assert attn(L, o=None) == EINVAL and attn(L, o=P + 2) == EINVAL and attn(L, o=P) == EINVAL and attn(L, B=0) == 0
     for want in (0, 1):
         need = L.savit_bias_attention_bwd_workspace_bytes(128, 197, 12, 200, want)
         assert need >= 128 * 12 * 2 * 256 * 4
-        assert attn(L, bwd=True, B=128, N=197, H=12, ld=2304, ldb=200, n=need - 1, dbias=P if want else None) == EINVAL
+        assert attn(L, bwd=True, B=128, N=197, H=12, ld=2304, ldb=200, n=need - 1, dbias=3 * P if want else None) == EINVAL
 
 
 def distill(L, **kw):
