@@ -669,8 +669,8 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
   Seg sg;
   bf16x8 qn[KS], dn[KS];
   float nln, deltan;
-  auto fetch = [&](int b) {  // an image's operands, one image ahead
-    const int len = length_of(p, b);
+  auto fetch = [&](int b, bool any) {  // an image's operands, one image ahead (any: or nothing, out of range)
+    const int len = any ? length_of(p, b) : 0;
     const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, col = (uint32_t)(h * hd + 8 * L.half) * 2;
     const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2), rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
     const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
     deltan = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)(q + p.Np) * 4), 0, 0));
   };
   if (b0 < b1) {
-    fetch(b0);
+    fetch(b0, true);
     sg.put(smem);
     __syncthreads();
   }
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
       df[ks] = dn[ks];
     }
     const float nl = nln, delta = deltan;
-    fetch(more ? b + 1 : b);  // (the last one again)
+    fetch(more ? b + 1 : b, more);
     __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to their use)
     const char* imgK = smem + ((b - b0) & 1) * 2 * Seg::IMG;
     const char* imgV = imgK + Seg::IMG;
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
   // the next image's K and V rows: PIECES 16-byte pieces in RES_GROUPS groups ; rows at and beyond its length are out of the descriptor's range (zero),
   // columns at and beyond hd repeat others (they meet zeros of the query fragments, or output rows that are not stored)
   constexpr int LEAST = 64 * (KE <= 8 ? KE - 1 : KE / 2), MAXL = (PIECES / RES_GROUPS + LEAST - 1) / LEAST;  // threads, pieces a thread and group
-  u32x4 st[MAXL];
+  u32x4 st[RES_GROUPS][MAXL];  // (the first image's all at once; then a group at a time)
   const int chunks = p.hd / 8;
   auto thread = [] {  // opaque: the offsets below are computed where they are used, 16 of them held over the loop are 16 registers too many
     int i = threadIdx.x;
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
       const int u = grp * (PIECES / RES_GROUPS) + i0 + k * blockDim.x;
       const int t = (u >> 4), c = (u & 7) < chunks ? (u & 7) : 0;
       const bool in = i0 + k * (int)blockDim.x < PIECES / RES_GROUPS;
-      st[k] = load16(rs, in ? (uint32_t)t * ld2 + ((u & 8) ? 2 * d2 : d2) + hcol + 16 * c : OUTSIDE);
+      st[grp][k] = load16(rs, in ? (uint32_t)t * ld2 + ((u & 8) ? 2 * d2 : d2) + hcol + 16 * c : OUTSIDE);
     }
   };
   auto put = [&](int grp, int buf) {
@@ -787,7 +787,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
     for (int k = 0; k < MAXL; ++k) {
       const int u = grp * (PIECES / RES_GROUPS) + i0 + k * blockDim.x;
       if (i0 + k * (int)blockDim.x < PIECES / RES_GROUPS)
-        *reinterpret_cast<u32x4*>(smem + buf * 2 * IMG + ((u & 8) ? IMG : 0) + at_chunk(u >> 4, u & 7)) = st[k];
+        *reinterpret_cast<u32x4*>(smem + buf * 2 * IMG + ((u & 8) ? IMG : 0) + at_chunk(u >> 4, u & 7)) = st[grp][k];
     }
   };
   auto image = [&](int b, int len) { return rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2); };
@@ -812,10 +812,10 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
   int len = length_of(p, b0);
   {
     const auto rs = image(b0, len);
-    for (int i = 0; i < RES_GROUPS; ++i) {
-      fetch(rs, i);
-      put(i, 0);
-    }
+#pragma unroll
+    for (int i = 0; i < RES_GROUPS; ++i) fetch(rs, i);
+#pragma unroll
+    for (int i = 0; i < RES_GROUPS; ++i) put(i, 0);
   }
   load_queries(b0, len);
   f32x4 sc[KT], dp[KT];
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_
     for (int t = 0; t < KT; ++t) sc[t] = load4f(rb, boff + 64 * t);
   }
   for (int b = b0; b < b1; ++b) {
-    const int buf = (b - b0) & 1, bn = b + 1 < b1 ? b + 1 : b, lenn = length_of(p, bn);  // (the last image fetches itself again)
+    const int buf = (b - b0) & 1, bn = b + 1 < b1 ? b + 1 : b, lenn = b + 1 < b1 ? length_of(p, bn) : 0;  // (behind the last one nothing is in range)
     const auto rn = image(bn, lenn);
     const char* imgK = smem + buf * 2 * IMG;
     const char* imgV = imgK + IMG;
