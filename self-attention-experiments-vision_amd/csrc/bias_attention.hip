@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
 // accumulators: every LDS and MFMA latency is covered by the other tiles of the same wave.
 
 template <int KT, int KS2, bool DB>
-__global__ __launch_bounds__(512, (KT <= 4 ? 3 : 2)) void bias_attn_dq_resident_kernel(const BiasAttnParams p) {
+__global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const BiasAttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int KE = KT + KT % 2, IMG = KE * 16 * ROWB, PIECES = KE * 16 * 8 * 2, RES_GROUPS = KT <= 6 ? 1 : KT <= 8 ? 2 : 4;
   constexpr bool AHEAD = KT <= 8;  // the next image's bias ahead too: longer rows leave no registers for them (14 tiles: 93 spills, twice the time)
@@ -958,10 +958,11 @@ int resident_waves(int N) {
   return nq > 8 ? (nq + 1) / 2 : nq;
 }
 int resident_blocks(int N) { return (N + 15) / 16 > 8 ? 2 : 1; }
-// parts of the batch, a workgroup each: the persistent kernel's fill the chip once (160 KB of LDS a CU; 8, 12 or 16 waves by its registers) ...
+// parts of the batch, a workgroup each: the persistent kernel's fill the chip once with 8 waves a CU (160 KB of LDS a CU; 12 and 16 waves, more than fit at once,
+// take 205 and 231 us against 200 at [1024 x 12 x 49], heads of 64) ...
 int resident_parts(int B, int N, int H) {
   const int kt = (N + 31) / 32 * 2, W = resident_waves(N);
-  int per_cu = (kt <= 4 ? 16 : kt <= 8 ? 12 : 8) / W;
+  int per_cu = 8 / W;
   if (per_cu > 160 / (8 * kt)) per_cu = 160 / (8 * kt);
   return clamp_parts((long)CUS * (per_cu < 1 ? 1 : per_cu) / ((long)H * resident_blocks(N)), B);
 }
