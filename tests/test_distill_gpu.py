@@ -299,3 +299,17 @@ def test_distill_through_a_model(ops):
     dwh = eng.grads[off : off + d * C].view(d, C).double()
     assert bool(((dwh - z.T @ grad).abs() <= z.abs().T @ tol * 1.01 + 1e-30).all())  # (a sum of six products in fp32: 2^-21 of them, inside the hundredth)
     assert bool(((db.double() - grad.sum(0)).abs() <= tol.sum(0) * 1.01 + 1e-30).all())
+
+
+def test_distill_offsets_beyond_32_bits(ops):
+    """The last rows of logits of more than 4 GiB come out as they do alone."""
+    C, K = 131072, 8
+    z, top, at, _, labels = make(16, C, K, 5, torch.bfloat16)
+    kw = dict(temperature=2.0, hard_weight=0.5, label_smoothing=0.1, grad_scale=1.0)
+    n = 1040  # times 16 rows of 256 KiB
+    big = z.repeat(n, 1)
+    assert big.numel() * 2 > 1 << 32
+    want = torch.empty_like(z)
+    rows = ops.distill_xent(z, top, at, labels=labels, dlogits=want, **kw)
+    got = ops.distill_xent(big, top.repeat(n, 1), at.repeat(n, 1), labels=labels.repeat(n), dlogits=big, **kw)
+    assert torch.equal(got[-16:], rows) and torch.equal(big[-16:], want) and torch.equal(big[:16], want)

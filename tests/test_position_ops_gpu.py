@@ -446,3 +446,46 @@ def test_attention_step_captured_and_on_another_stream(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for _, out in graphs for x, y in zip(out, eager[k % 2])), k
         step(ops, **src)  # eager work between the replays
+
+
+def test_offsets_beyond_32_bits(ops):
+    """The last head (image, rows) of tensors of more than 4 GiB comes out as it does alone, bit by bit."""
+    g = gen(77)
+    H, N, hd = 17, 8192, 16  # a bias of 4.25 GiB
+    index = ((torch.arange(N, device="cuda")[:, None] * 31 + torch.arange(N, device="cuda")[None, :] * 7) % 97).int()
+    table = randn(g, 97, H)
+    bias = ops.relpos_bias_fwd(table, index)
+    assert bias.numel() * 4 > 1 << 32
+    last = ops.relpos_bias_fwd(table[:, -1:].contiguous(), index)
+    assert torch.equal(bias[-1], last[0])
+    qkv = randn(g, N, 3 * H * hd, dtype=torch.bfloat16)
+    d_o = randn(g, N, H * hd, dtype=torch.bfloat16)
+    o, lse = ops.bias_attention_fwd(qkv, bias, 1, N, H, head_dim=hd)
+    dqkv, dbias = ops.bias_attention_bwd(qkv, bias, d_o, lse, 1, N, H, dq_scale=1.0, head_dim=hd)
+    one = qkv.view(N, 3, H, hd)[:, :, -1].reshape(N, 3 * hd).contiguous()
+    d_one = d_o[:, -hd:].contiguous()
+    o1, lse1 = ops.bias_attention_fwd(one, last, 1, N, 1, head_dim=hd)
+    g1, b1 = ops.bias_attention_bwd(one, last, d_one, lse1, 1, N, 1, dq_scale=1.0, head_dim=hd)
+    assert torch.equal(o[:, -hd:], o1) and torch.equal(lse[:, -1:], lse1)
+    assert torch.equal(dqkv.view(N, 3, H, hd)[:, :, -1].reshape(N, -1), g1) and torch.equal(dbias[-1], b1[0])
+    del bias, dbias, last, b1
+    B, N, H, hd = 4800, 197, 12, 64  # packed rows of 4.06 GiB
+    small = randn(g, 8 * N, 3 * H * hd, dtype=torch.bfloat16, scale=0.5)
+    qkv = small.repeat(B // 8, 1)
+    assert qkv.numel() * 2 > 1 << 32
+    w = 1 + randn(g, 2, hd, scale=0.1)
+    tab = ops.rope_table(ops.rope_angles_1d(N, hd))
+    y = ops.qk_norm_rope_fwd(qkv, w[0], w[1], tab, N, H)
+    assert torch.equal(y[-8 * N :], ops.qk_norm_rope_fwd(small, w[0], w[1], tab, N, H))
+    dw = torch.zeros(2, 2, hd, device="cuda")
+    dx = ops.qk_norm_rope_bwd(qkv, qkv, w[0], w[1], tab, dw[0, 0], dw[0, 1], N, H, out=y)
+    assert torch.equal(dx[-8 * N :], ops.qk_norm_rope_bwd(small, small, w[0], w[1], tab, dw[1, 0], dw[1, 1], N, H, out=torch.empty_like(small)))
+    bias = ops.relpos_bias_empty(H, N)
+    bias.copy_(randn(g, H, N, N))
+    d_small = randn(g, 8 * N, H * hd, dtype=torch.bfloat16)
+    o, lse = ops.bias_attention_fwd(qkv, bias, B, N, H)
+    o1, lse1 = ops.bias_attention_fwd(small[-N:], bias, 1, N, H)
+    assert float((o[-N:].double() - o1.double()).norm() / o1.double().norm()) < 2 * U  # (another tile shape for one image)
+    dqkv, _ = ops.bias_attention_bwd(qkv, bias, d_small.repeat(B // 8, 1), lse, B, N, H, dq_scale=1.0, want_dbias=False, dqkv=y)
+    g1, _ = ops.bias_attention_bwd(small[-N:], bias, d_small[-N:], lse[-1:].contiguous(), 1, N, H, dq_scale=1.0, want_dbias=False)
+    assert torch.equal(dqkv[-N:], g1)
