@@ -16,7 +16,7 @@
 // What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (55 measured) and 55 backward (99 dQ and dbias, 94 dK and dV), the
 // products 13 and 31: with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
 // goes into (dK / dV: vector issue 39 %, LDS 27 %, matrix pipe 17 % busy).  One segment or long rows come nearer: [2048 x 4 x 49], heads of 32,
-// 27 us forward (bytes 21), 37 dK and dV (31).
+// 25 us forward (bytes 21), 28 dK and dV (31 from memory; some of it is still in the caches), 32 dQ and dbias.
 //
 // delta is summed from the fp32 probabilities, in a loop of its own over the keys, not taken as rowsum(dO . O): O is rounded to bf16, and the table
 // gradient that dS feeds is an fp32 parameter gradient (2^-9 of O in delta is 1e-4 of the gradient; this way it is 1e-6).
@@ -48,6 +48,7 @@ struct BiasAttnParams {
   int hd;
   int blocks;          // query (key) blocks of a sequence
   int key_blocks, parts;
+  int image_major;     // workgroups: all heads of an image in a row, or all images of a head
   float dq_scale;
 };
 
@@ -209,14 +210,15 @@ __device__ __forceinline__ void store_row16(bf16_t* row, const f32x4 (&o)[2 * KS
   });
 }
 
-// workgroup -> (head, image, block): all blocks and images of a head in a row, and consecutive numbers on one XCD, so that its L2 holds the
-// head's bias for every image
+// workgroup -> (head, image, block), consecutive numbers on one XCD.  All images of a head in a row: the L2 holds the head's bias for every image.
+// All heads of an image in a row: the L2 holds every head's bias, and the heads' pieces of a row, which lie next to each other in memory, are read
+// together (many_heads)
 __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b, int& blk) {
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   blk = t % p.blocks;
   const int r = t / p.blocks;
-  b = r % p.B;
-  h = r / p.B;
+  b = p.image_major ? r / p.H : r % p.B;
+  h = p.image_major ? r % p.H : r / p.B;
 }
 
 template <int KS>
@@ -751,10 +753,17 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
   constexpr bool AHEAD = KT <= 8;  // the next image's bias ahead too: longer rows leave no registers for them (14 tiles: 93 spills, twice the time)
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int t0 = xcd_remap(blockIdx.x, gridDim.x);
-  const int part = t0 % p.parts;
-  t0 /= p.parts;
-  const int blk = t0 % p.blocks, h = t0 / p.blocks;
+  const int t0 = xcd_remap(blockIdx.x, gridDim.x);
+  int part, h, blk;
+  if (p.image_major) {
+    blk = t0 % p.blocks;
+    h = t0 / p.blocks % p.H;
+    part = t0 / p.blocks / p.H;
+  } else {
+    part = t0 % p.parts;
+    blk = t0 / p.parts % p.blocks;
+    h = t0 / p.parts / p.blocks;
+  }
   const int b0 = (int)((long)p.B * part / p.parts), b1 = (int)((long)p.B * (part + 1) / p.parts);
   const int q = (blk * (int)(blockDim.x >> 6) + wave) * 16 + ql;
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
@@ -945,7 +954,7 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
 int padded(int N) { return (N + 63) / 64 * 64; }
 
 // Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 182 us against 273 of the
-// streaming kernels at [128 x 12 x 197], 82 / 122 at [2048 x 4 x 49], 80 / 118 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 165 /
+// streaming kernels at [128 x 12 x 197], 60 / 102 at [2048 x 4 x 49], 80 / 118 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 165 /
 // 194, 76 / 82, 67 / 80, 18 / 17.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
 constexpr int RESIDENT_N = 224;
 bool resident(int N) { return N <= RESIDENT_N; }
@@ -972,6 +981,12 @@ int db_parts(int B, int N, int H) {
   return clamp_parts(4L * CUS / tiles, B);
 }
 int dbias_parts(int B, int N, int H) { return resident(N) ? resident_parts(B, N, H) : db_parts(B, N, H); }
+
+// All heads of an image in a row where their biases fit an XCD's L2 (4 MB) beside the rows: half of it where heads end inside a cache line of a row, a
+// quarter where they are whole lines and less is won.  Against all images of a head in a row, forward and backward: [2048 x 4 x 49], heads of 32,
+// 23 and 60 us against 27 and 80; [128 x 12 x 197], heads of 48 (1.9 MB), forward 48 / 56; heads of 64: [1024 x 8 x 128] forward 152 / 162, [1024 x 8 x 64]
+// backward 181 / 187, but [128 x 12 x 197] (1.9 MB) forward 54.5 / 51.7 and [16 x 16 x 577] (21 MB) 78 / 51
+bool many_heads(int N, int H, int hd, int ldb) { return (long)H * N * ldb * 4 <= (hd == 64 ? 1L << 20 : 2L << 20); }
 
 bool size_ok(int B, int N, int H, int hd, int ld, int ldb) {
   if (!(B >= 0 && N > 0 && N <= 32768 && H > 0 && (hd == 16 || hd == 32 || hd == 48 || hd == 64))) return false;
@@ -1060,6 +1075,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.o = (bf16_t*)o; p.lse = lse;
   p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias;
+  p.image_major = many_heads(N, H, head_dim, ld_bias);
   return launch_fwd(p, (hipStream_t)stream);
 }
 
@@ -1080,6 +1096,7 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.d_o = (const bf16_t*)d_o; p.lse = const_cast<float*>(lse); p.dqkv = (bf16_t*)dqkv;
   p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias; p.dq_scale = dq_scale;
+  p.image_major = many_heads(N, H, head_dim, ld_bias);
   p.Np = padded(N);
   p.stat = (float*)workspace;
   const int parts = dbias_parts(B, N, H);
