@@ -953,9 +953,9 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
 
 int padded(int N) { return (N + 63) / 64 * 64; }
 
-// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 182 us against 273 of the
-// streaming kernels at [128 x 12 x 197], 60 / 102 at [2048 x 4 x 49], 80 / 118 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 165 /
-// 194, 76 / 82, 67 / 80, 18 / 17.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
+// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 173 us against 265 of the
+// streaming kernels at [128 x 12 x 197], 60 / 110 at [2048 x 4 x 49], 80 / 117 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 163 /
+// 192, 56 / 70, 65 / 79, 17 / 17.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
 constexpr int RESIDENT_N = 224;
 bool resident(int N) { return N <= RESIDENT_N; }
 constexpr int CUS = 256;  // not the device's or a budget's: the parts set the order of the bias gradient's sum

@@ -8,7 +8,7 @@
 // an atomic per position would make the gradient depend on scheduling, and the few buckets that far positions share would serialise.
 // A wave takes one bucket's list for 4 heads (the list is read once for them); where lists are long it takes a fixed number of entries instead,
 // and a second launch adds the pieces of a bucket.
-// Measured: [8 x 1500 x 1500] forward 15 us (72 MB, 4.8 TB/s), table gradient of 32 buckets 24 + 5 us (72 MB read through the list);
+// Measured: [8 x 1500 x 1500] forward 15 us (72 MB, 4.8 TB/s), table gradient of 32 buckets 23 + 5 us (72 MB read through the list);
 // [16 x 577 x 577] 9.6 us (21 MB; bound by the gathers from 2212 buckets), [12 x 197 x 197] 5 us and 9 us.
 #include "common.h"
 #include "savit.h"
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void relpos_grad_kernel(const float* __restric
 
 // long lists: a wave RB_CHUNK entries, whatever buckets they belong to; the piece of bucket b in chunk c goes to slab row c + b (every new piece
 // is a new chunk, a new bucket or both, so rows are not shared)
-constexpr int RB_CHUNK = 256;  // 1024: 36 us against 24 at 1500 tokens and 8 heads (a wave's few loads in flight are all latency)
+constexpr int RB_CHUNK = 256;  // four entries a lane, all under way at once: 23 us at 1500 tokens and 8 heads (longer chunks, a loop of such loads: 36)
 __global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __restrict__ dbias, const int* __restrict__ order, const int* __restrict__ start,
                                                                  float* __restrict__ slab, int N, int H, int nb, int ld, int chunks) {
   const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -111,6 +111,23 @@ __global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __
   const int h0 = blockIdx.y * RB_HEADS, nh = (H - h0) < RB_HEADS ? H - h0 : RB_HEADS;
   const unsigned total = (unsigned)N * (unsigned)N;
   const unsigned c0 = (unsigned)c * RB_CHUNK, c1 = c0 + RB_CHUNK < total ? c0 + RB_CHUNK : total;
+  constexpr int U = RB_CHUNK / 64;
+  float v[U][RB_HEADS];  // all of the chunk, under way while its buckets are looked for (an entry outside reads position 0 and is dropped)
+  bool in[U];
+  {
+    unsigned e[U];
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = c0 + lane + 64 * u < c1 ? (unsigned)order[c0 + lane + 64 * u] : 0xffffffffu;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      in[u] = e[u] < total;
+      const unsigned x = in[u] ? e[u] : 0, r = x / (unsigned)N;
+      const size_t at = (size_t)r * ld + (x - r * (unsigned)N);
+#pragma unroll
+      for (int k = 0; k < RB_HEADS; ++k) v[u][k] = dbias[(size_t)(h0 + (k < nh ? k : 0)) * N * ld + at];
+    }
+  }
   int lo = 0, hi = nb;  // first bucket whose list ends behind c0
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -122,12 +139,17 @@ __global__ __launch_bounds__(256) void relpos_grad_chunks_kernel(const float* __
     if (l0 >= c1) break;
     const unsigned p0 = l0 > c0 ? l0 : c0, p1 = l1 < c1 ? l1 : c1;
     if (p0 >= p1) continue;
-    float s[RB_HEADS];
-    sum_list(dbias, order, p0, p1, N, ld, h0, nh, total, s);
-    if ((threadIdx.x & 63) == 0) {
+    float s[RB_HEADS] = {};
 #pragma unroll
-      for (int k = 0; k < RB_HEADS; ++k)
-        if (k < nh) slab[((size_t)c + b) * H + h0 + k] = s[k];
+    for (int u = 0; u < U; ++u) {
+      const unsigned q = c0 + (threadIdx.x & 63) + 64 * u;
+#pragma unroll
+      for (int k = 0; k < RB_HEADS; ++k) s[k] += in[u] && q >= p0 && q < p1 ? v[u][k] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < RB_HEADS; ++k) {
+      const float sum = wave_sum(s[k]);
+      if ((threadIdx.x & 63) == 0 && k < nh) slab[((size_t)c + b) * H + h0 + k] = sum;
     }
   }
 }
