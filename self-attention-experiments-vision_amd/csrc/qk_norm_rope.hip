@@ -12,7 +12,7 @@
 // 5 us for the weights' sums; [16384 rows, 3 x 8 heads of 48] 19 us (75 MB, 4.0 TB/s); 4 rows: one launch.
 //
 // Layout: G = 1..16 lanes per head, each with 8 columns of the head's lower half and the 8 columns hd/2 above them, so that both
-// kinds of pairs lie in one lane and a reduction takes log2 G lane exchanges.  A group of G lanes owns a fixed chunk of HS heads and walks over rows:
+// kinds of pairs lie in one lane and a reduction takes log2 G lane exchanges.  A group of G lanes owns a fixed chunk of HS heads (backward: one) and walks over rows:
 // its weights stay in registers (in backward its weight gradients too), the table row is fetched once for HS heads, and neighbouring
 // groups read neighbouring chunks of the same row.
 #include "common.h"
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void qkn_fwd_kernel(const QknParams p) {
 
 constexpr int QKN_BWD_THREADS = 256;
 
-template <typename T, int G, int HS>
+template <typename T, int G>
 __global__ __launch_bounds__(QKN_BWD_THREADS, sizeof(T) == 2 ? 4 : 3) void qkn_bwd_kernel(const QknParams p) {
   constexpr int GPB = QKN_BWD_THREADS / G;
   __shared__ float red[QKN_BWD_THREADS * 16];
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(QKN_BWD_THREADS, sizeof(T) == 2 ? 4 : 3) void qkn_b
   for (int i = 0; i < 8; ++i) da[i] = db[i] = 0.f;
   if (grp < step * chunks) {
     int sec, col0, heads;
-    chunk_of<HS>(p, grp % chunks, sec, col0, heads);
+    chunk_of<1>(p, grp % chunks, sec, col0, heads);
     const int lo = col0 + 8 * l, hi = lo + p.hd / 2;
     float wa[8], wb[8];
     const float sc = sec == 0 ? p.q_scale : 1.0f;
@@ -252,83 +252,77 @@ __global__ __launch_bounds__(QKN_BWD_THREADS, sizeof(T) == 2 ? 4 : 3) void qkn_b
       const T* x = reinterpret_cast<const T*>(p.x) + (size_t)row * p.ldx;
       const T* g = reinterpret_cast<const T*>(p.g) + (size_t)row * p.ldg;
       T* y = reinterpret_cast<T*>(p.y) + (size_t)row * p.ldy;
-      Vec8<T> ga[HS], gb[HS], va[HS], vb[HS];
-#pragma unroll
-      for (int h = 0; h < HS; ++h)
-        if (on && h < heads) {
-          ga[h].load(g + lo + h * p.hd);
-          gb[h].load(g + hi + h * p.hd);
-          if (sec < 2) {
-            va[h].load(x + lo + h * p.hd);
-            vb[h].load(x + hi + h * p.hd);
-          }
+      Vec8<T> ga, gb, va, vb;
+      if (on) {
+        ga.load(g + lo);
+        gb.load(g + hi);
+        if (sec < 2) {
+          va.load(x + lo);
+          vb.load(x + hi);
         }
+      }
       float cs[8], sn[8];
       if (sec < 2 && p.table && on) load_angles(p, row, l, cs, sn);
-#pragma unroll
-      for (int h = 0; h < HS; ++h) {
-        if (h >= heads) break;
-        if (sec < 2) {
-          float a[8], b[8], u[8], v[8];
-          if (on) {
-            va[h].get(a);
-            vb[h].get(b);
-            ga[h].get(u);
-            gb[h].get(v);
-            if (p.table) rotate<-1>(u, v, cs, sn, p.inter);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = b[i] = u[i] = v[i] = 0.f;
-          }
-          if (p.center) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += a[i] + b[i];
-            const float mean = group_sum<G>(s) * inv;
-            if (on) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                a[i] -= mean;
-                b[i] -= mean;
-              }
-            }
-          }
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-          const float r = rsqrtf(group_sum<G>(ss) * inv + p.eps);
-          float hn = 0.f, hs = 0.f;
-          if (on) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              a[i] *= r;
-              b[i] *= r;
-              u[i] *= sc;
-              v[i] *= sc;
-              da[i] += u[i] * a[i];
-              db[i] += v[i] * b[i];
-              u[i] *= wa[i];
-              v[i] *= wb[i];
-              hn += u[i] * a[i] + v[i] * b[i];
-              hs += u[i] + v[i];
-            }
-          }
-          hn = group_sum<G>(hn) * inv;
-          hs = p.center ? group_sum<G>(hs) * inv : 0.f;
-          if (on) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              u[i] = r * (u[i] - hs - a[i] * hn);
-              v[i] = r * (v[i] - hs - b[i] * hn);
-            }
-            ga[h].set(u);
-            gb[h].set(v);
-          }
-        }
+      if (sec < 2) {
+        float a[8], b[8], u[8], v[8];
         if (on) {
-          ga[h].store(y + lo + h * p.hd);
-          gb[h].store(y + hi + h * p.hd);
+          va.get(a);
+          vb.get(b);
+          ga.get(u);
+          gb.get(v);
+          if (p.table) rotate<-1>(u, v, cs, sn, p.inter);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] = b[i] = u[i] = v[i] = 0.f;
         }
+        if (p.center) {
+          float s = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s += a[i] + b[i];
+          const float mean = group_sum<G>(s) * inv;
+          if (on) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              a[i] -= mean;
+              b[i] -= mean;
+            }
+          }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+        const float r = rsqrtf(group_sum<G>(ss) * inv + p.eps);
+        float hn = 0.f, hs = 0.f;
+        if (on) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a[i] *= r;
+            b[i] *= r;
+            u[i] *= sc;
+            v[i] *= sc;
+            da[i] += u[i] * a[i];
+            db[i] += v[i] * b[i];
+            u[i] *= wa[i];
+            v[i] *= wb[i];
+            hn += u[i] * a[i] + v[i] * b[i];
+            hs += u[i] + v[i];
+          }
+        }
+        hn = group_sum<G>(hn) * inv;
+        hs = p.center ? group_sum<G>(hs) * inv : 0.f;
+        if (on) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u[i] = r * (u[i] - hs - a[i] * hn);
+            v[i] = r * (v[i] - hs - b[i] * hn);
+          }
+          ga.set(u);
+          gb.set(v);
+        }
+      }
+      if (on) {
+        ga.store(y + lo);
+        gb.store(y + hi);
       }
     }
   }
@@ -404,8 +398,8 @@ int lanes_of(int hd) {
   return g;
 }
 
-// heads a group takes at a time: HS amortises the table row and keeps 2 HS (backward 4 HS) 16-byte loads of a lane in flight; one where
-// that leaves too few groups to fill the chip
+// heads a group takes at a time in forward: HS amortises the table row and keeps 2 HS 16-byte loads of a lane in flight; one where
+// that leaves too few groups to fill the chip, and in backward (four times the operands a head: more waves beat wider chunks, 71 us against 81)
 template <int HS>
 int chunks_of(int H, int Hk, bool values, QknParams* p) {
   const int nq = (H + HS - 1) / HS, nk = (Hk + HS - 1) / HS;
@@ -431,16 +425,16 @@ int launch_fwd(QknParams& p, bool values, hipStream_t st) {
   hipLaunchKernelGGL((qkn_fwd_kernel<T, G, HS>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   SAVIT_LAUNCH_RET();
 }
-template <typename T, int G, int HS>
+template <typename T, int G>
 int launch_bwd(QknParams& p, bool values, long ws_bytes, hipStream_t st) {
   constexpr int GPB = QKN_BWD_THREADS / G;
-  const int chunks = chunks_of<HS>(p.H, p.Hk, values, &p);
+  const int chunks = chunks_of<1>(p.H, p.Hk, values, &p);
   const long want = ((long)p.rows * chunks + GPB - 1) / GPB;
   const long least = (chunks + GPB - 1) / GPB;
   long blocks = want < QKN_BWD_BLOCKS ? want : QKN_BWD_BLOCKS;
   if (blocks < least) blocks = least;
   SAVIT_CHECK_ARG(blocks == 1 || (p.slab && ws_bytes >= blocks * 2 * p.hd * 4));
-  hipLaunchKernelGGL((qkn_bwd_kernel<T, G, HS>), dim3((unsigned)blocks), dim3(QKN_BWD_THREADS), 0, st, p);
+  hipLaunchKernelGGL((qkn_bwd_kernel<T, G>), dim3((unsigned)blocks), dim3(QKN_BWD_THREADS), 0, st, p);
   if (blocks > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
@@ -511,8 +505,8 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
   const int G = lanes_of(head_dim);
 #define QKN_BWD(GV)                                                                                        \
   case GV:                                                                                                 \
-    return is_bf16 ? launch_bwd<bf16_t, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream)             \
-                   : launch_bwd<float, GV, 1>(p, values, workspace_bytes, (hipStream_t)stream);
+    return is_bf16 ? launch_bwd<bf16_t, GV>(p, values, workspace_bytes, (hipStream_t)stream)             \
+                   : launch_bwd<float, GV>(p, values, workspace_bytes, (hipStream_t)stream);
   switch (G) {
     QKN_BWD(1)
     QKN_BWD(2)
