@@ -35,6 +35,7 @@ struct DistillParams {
   long ldz, lddz;
   int R, C, K, slots;
   float soft, hard, smooth, T, c_soft, c_hard, grad_scale;  // c_soft = log2 e / T, c_hard = log2 e
+  double inv_T;
 };
 
 template <typename T>
@@ -118,15 +119,51 @@ struct Seen {
 };
 
 __device__ __forceinline__ unsigned hash_of(int j) { return (unsigned)j * 2654435761u >> 16; }
+// the wave reductions in 64 bits: the same exchanges as wave_sum's, on both halves (a shuffle through LDS takes five times as long)
+struct Halves {
+  unsigned lo, hi;
+};
+template <int CTRL>
+__device__ __forceinline__ double dpp_mov_d(double v) {
+  const Halves a = __builtin_bit_cast(Halves, v);
+  return __builtin_bit_cast(double, Halves{(unsigned)__builtin_amdgcn_update_dpp(0, (int)a.lo, CTRL, 0xf, 0xf, false),
+                                           (unsigned)__builtin_amdgcn_update_dpp(0, (int)a.hi, CTRL, 0xf, 0xf, false)});
+}
+__device__ __forceinline__ double half_row_d(double v, double& other) {  // value and partner 16 lanes away, in either order
+  const Halves a = __builtin_bit_cast(Halves, v);
+  const auto l = __builtin_amdgcn_permlane16_swap(a.lo, a.lo, false, false), h = __builtin_amdgcn_permlane16_swap(a.hi, a.hi, false, false);
+  const unsigned l0 = l[0], l1 = l[1], h0 = h[0], h1 = h[1];
+  other = __builtin_bit_cast(double, Halves{l1, h1});
+  return __builtin_bit_cast(double, Halves{l0, h0});
+}
+__device__ __forceinline__ double half_wave_d(double v, double& other) {  // and 32 lanes away
+  const Halves a = __builtin_bit_cast(Halves, v);
+  const auto l = __builtin_amdgcn_permlane32_swap(a.lo, a.lo, false, false), h = __builtin_amdgcn_permlane32_swap(a.hi, a.hi, false, false);
+  const unsigned l0 = l[0], l1 = l[1], h0 = h[0], h1 = h[1];
+  other = __builtin_bit_cast(double, Halves{l1, h1});
+  return __builtin_bit_cast(double, Halves{l0, h0});
+}
+template <typename F>
+__device__ __forceinline__ double wave_join_d(double v, F f) {
+  v = f(v, dpp_mov_d<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = f(v, dpp_mov_d<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = f(v, dpp_mov_d<0x141>(v));  // row_half_mirror
+  v = f(v, dpp_mov_d<0x140>(v));  // row_mirror
+  double b;
+  v = half_row_d(v, b);
+  v = f(v, b);
+  v = half_wave_d(v, b);
+  return f(v, b);
+}
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return wave_join_d(v, [](double a, double b) { return a + b; });
 }
 __device__ __forceinline__ double wave_max_d(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-  return v;
+  return wave_join_d(v, [](double a, double b) { return fmax(a, b); });
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+  const Halves a = __builtin_bit_cast(Halves, v);
+  return __builtin_bit_cast(double, Halves{(unsigned)__builtin_amdgcn_readlane((int)a.lo, lane), (unsigned)__builtin_amdgcn_readlane((int)a.hi, lane)});
 }
 
 // exp2((z - m) c) as exp2(fma(z, c, -mb)), mb = m c rounded: one instruction less an element (the exponentials are a third of the kernel's
@@ -192,7 +229,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
   const bool first_lane = (tid & 63) == 0;
   const int row = blockIdx.x * RPB + sub;
   const int K = p.K;
-  // LDS of a row: K pairs {logit / T, z at the class, class, what the gradient takes off there}, and a hash table of their classes
+  // LDS of a row: K pairs {logit / T and then its exponential, z at the class, class, what the gradient takes off there}, and a hash table of their classes
   double* tt = reinterpret_cast<double*>(smem) + (size_t)sub * K;
   float* zt = reinterpret_cast<float*>(smem + (size_t)RPB * K * 8) + (size_t)sub * K;
   int* at = reinterpret_cast<int*>(smem + (size_t)RPB * K * 12) + (size_t)sub * K;
@@ -237,7 +274,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     int mine = 0;
     auto pair = [&](int k, int j, float t) {
       const bool ok = (unsigned)j < (unsigned)p.C;
-      const double td = ok ? (double)t / (double)p.T : -__builtin_inf();
+      const double td = ok ? (double)t * p.inv_T : -__builtin_inf();
       at[k] = ok ? j : -1;
       tt[k] = td;
       tm = fmax(tm, td);
@@ -302,7 +339,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     if (64 * wave < K) {
       tm = p.lse ? (live ? (double)p.lse[row] : 0.0) : wave_max_d(tm);  // what this wave's sum is relative to
       if (live)
-        for (int k = tid; k < K; k += TH) ts += exp(tt[k] - tm);
+        for (int k = tid; k < K; k += TH) ts += tt[k] = exp(tt[k] - tm);  // from here on relative to the wave's
       ts = wave_sum_d(ts);
     }
     if (first_lane) {
@@ -385,27 +422,35 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     return s;
   };
   asm volatile("" ::: "memory");
+  double log_s = 0.0, log_h = 0.0;  // of the row's sums
+  if (live && (64 * wave < K || wave == W - 1)) {
+    const bool odd = two && (tid & 1);  // two logarithms for one, on even and odd lanes
+    const double x = log(join(odd ? p.c_hard : p.c_soft, odd));
+    log_s = lane_d(x, 0);
+    log_h = two ? lane_d(x, 1) : log_s;
+  }
   if (live && 64 * wave < K) {
-    double ref = tpart[sub][0][0], inv = 1.0;  // P = exp(t - ref) inv
+    double ref = tpart[sub][0][0], inv = 1.0;  // P = tt inv, and exp(its wave's reference - ref) where that is another
+    auto apart = [&](int w) { return tpart[sub][w][0] == ref ? 1.0 : exp(tpart[sub][w][0] - ref); };
     if (!p.lse) {
       double sum = 0.0;
       for (int w = 1; w < W && 64 * w < K; ++w) ref = fmax(ref, tpart[sub][w][0]);
-      for (int w = 0; w < W && 64 * w < K; ++w) sum += tpart[sub][w][1] == 0.0 ? 0.0 : tpart[sub][w][1] * exp(tpart[sub][w][0] - ref);
+      for (int w = 0; w < W && 64 * w < K; ++w) sum += tpart[sub][w][1] == 0.0 ? 0.0 : tpart[sub][w][1] * apart(w);
       inv = sum == 0.0 ? 0.0 : 1.0 / sum;
     }
-    const double log_s = log(join(p.c_soft, false));
+    const double mine = apart(wave) * inv;
     double kl = 0.0, named = 0.0;
     for (int k = tid; k < K; k += TH) {
       const int j = at[k];
       if (j < 0) continue;
-      double P = exp(tt[k] - ref) * inv;
+      double P = tt[k] * mine;
       bool first = true;
       if (repeated[sub]) {  // a class named more than once has the sum, and counts once
         P = 0.0;
         for (int i = 0; i < K; ++i)
           if (at[i] == j) {
             if (i < k) first = false;
-            P += exp(tt[i] - ref) * inv;
+            P += tt[i] * (apart((i % TH) >> 6) * inv);
           }
       }
       off[k] = (float)(gs * (p.soft * p.T * P + hard * ((j == label ? 1.0 - p.smooth : 0.0) + (double)p.smooth / p.C)));
@@ -416,7 +461,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       }
     }
     kl = wave_sum_d(kl);
-    named = wave_sum_d(named);
+    if (p.lse) named = wave_sum_d(named);  // (asked for where mass is left over)
     if (first_lane) {
       lpart[sub][wave][0] = kl;
       lpart[sub][wave][1] = named;
@@ -447,13 +492,12 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     kl += lpart[sub][w][0];
     named += lpart[sub][w][1];
   }
-  const double log_s = log(join(p.c_soft, false));
   double Z = 0.0;
   for (int w = 0; w < W; ++w) Z += (double)part[sub][w].z;
   if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log_s - named);
   if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
   if (hard != 0.0) {
-    double ce = (two ? log(join(p.c_hard, true)) : log_s) - (1.0 - p.smooth) * ((double)zl - M);
+    double ce = log_h - (1.0 - p.smooth) * ((double)zl - M);
     if (p.smooth != 0.0f) ce -= p.smooth * (Z / p.C - M);
     loss += hard * ce;
   }
@@ -515,6 +559,7 @@ extern "C" int savit_distill_xent(const void* logits, long ld_logits, int logits
   p.soft = distill_weight; p.hard = hard_weight; p.smooth = hard_weight != 0.f ? label_smoothing : 0.f; p.T = temperature;
   p.c_soft = (float)(1.4426950408889634 / (double)temperature);
   p.c_hard = 1.44269504088896340736f;
+  p.inv_T = 1.0 / (double)temperature;
   p.grad_scale = grad_scale;
   for (p.slots = 16; p.slots < 2 * K; p.slots *= 2) {}
   const hipStream_t st = (hipStream_t)stream;
