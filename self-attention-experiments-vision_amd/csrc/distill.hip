@@ -8,8 +8,8 @@
 // Bound by HBM: z is read once and dz written once.  The row stays in registers between the pass that finds the maximum and the sums and the pass
 // that writes the gradient (C 16-byte pieces a thread; what does not fit is read a second time), so there is one block reduction and no re-read.
 // A thread keeps the sums relative to its own maximum and the block joins (maximum, sum) pairs: one barrier instead of two.
-// Measured, with gradient: [2048 x 131072] 260 us (1075 MB, 4.1 TB/s; a copy of the bytes takes 216), [1024 x 21843] 41 us (135 MB, 3.3 TB/s), [128 x 1000]
-// one launch.  What is left above the copy: a row's loads do not overlap the stores of the row before it in the same registers, and the exponentials (10 %).
+// Measured, with gradient: [2048 x 131072] 260 us (1075 MB, 4.1 TB/s; the loss alone 139; a copy of the bytes takes 216), [1024 x 21843] 39 us (135 MB, 3.5 TB/s), [128 x 1000]
+// 7 to 8 us: a launch, and the 64-bit logarithms and exponentials of the pairs one after the other.  What is left above the copy: a row's loads do not overlap the stores of the row before it in the same registers, and the exponentials (10 %).
 // Exponentials are v_exp_f32 on (z - max) * (log2 e / T), per-thread sums fp32; everything that exists once a row - the pairs, the
 // normalisers, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
 // The gradient is written for every class as if no pair named it, then the at most K + 1 classes with a pair or the label are written again.
@@ -530,13 +530,16 @@ int launch_distill(const DistillParams& p, hipStream_t st) {
                      (size_t)RPB * (p.K * 20 + p.slots * 4), st, p);
   SAVIT_LAUNCH_RET();
 }
-// A row's threads grow with its pieces: a wave (no idle wave where rows are short), four, sixteen; two workgroups of sixteen waves share a CU (64
-// registers a thread), so that one row loads while another computes or stores
+// A row's threads, and the pieces a thread keeps, grow with the row: a wave (no idle wave where rows are short), four, eight, sixteen; eight waves and
+// more share a CU with another row's, so that one row loads while another computes or stores.  Two pieces a thread against four: [128 x 1000] fp32 7.1
+// against 7.8 us, [8192 x 4000] bf16 60 / 64; eight waves of four against eight of twelve: [8192 x 8000] fp32 133 / 137, [64 x 8000] 8.5 / 8.9.
 template <typename TI, typename TO>
 int choose_distill(const DistillParams& p, hipStream_t st) {
   const int pieces = (p.C + Piece<TI>::E - 1) / Piece<TI>::E;
   if (pieces <= 64 * 2) return launch_distill<TI, TO, 1, 2, 4>(p, st);
-  if (pieces <= 256 * 4) return launch_distill<TI, TO, 4, 4, 6>(p, st);
+  if (pieces <= 256 * 2) return launch_distill<TI, TO, 4, 2, 5>(p, st);
+  if (pieces <= 256 * 4) return launch_distill<TI, TO, 4, 4, 5>(p, st);
+  if (pieces <= 512 * 4) return launch_distill<TI, TO, 8, 4, 4>(p, st);
   if (pieces <= 512 * 12) return launch_distill<TI, TO, 8, 12, 4>(p, st);
   return launch_distill<TI, TO, 16, 16, 4>(p, st);
 }

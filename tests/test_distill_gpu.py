@@ -106,7 +106,7 @@ def run_and_check(ops, z, top, at, T, soft, lse, labels, hard, smooth, weight, g
     return loss, dz
 
 
-# the kernels' shapes change at 128, 1024, 4096, 8192 and beyond 16384 pieces of 16 bytes (8 bf16 or 4 fp32 logits)
+# the kernels' shapes change at 128, 512, 1024, 2048, 6144 and beyond 16384 pieces of 16 bytes (8 bf16 or 4 fp32 logits)
 CLASSES = [1, 2, 3, 7, 100, 511, 513, 1000, 1025, 4097, 8191, 8200, 16385, 21843, 32769, 70001, 140003]
 
 
