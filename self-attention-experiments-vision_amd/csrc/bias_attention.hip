@@ -10,7 +10,7 @@
 // in-register reductions plus an exchange between the lanes of a query, and the score tile is the next product's operand without an LDS round trip.
 // The bias tile is fetched one tile ahead and is the INITIAL value of the score accumulators: adding it costs nothing.  W = 1, 2 or 4 by the sequence
 // length, so that short sequences leave no wave idle.
-// Rounded to bf16: P and dS as operands of the matrix instructions (O, dQ, dK, dV are bf16 themselves; P stays below 2^8 and is divided by its fp32 sum at
+// Rounded to bf16: P and dS as operands of the matrix instructions, beyond 32 tokens (O, dQ, dK, dV are bf16 themselves: the error is sqrt 2 of theirs; P stays below 2^8 and is divided by its fp32 sum at
 // the end), O and the gradients when stored.  Scores, statistics, delta, sums and dbias are fp32.
 //
 // What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (55 measured) and 55 backward (99 dQ and dbias, 94 dK and dV), the
@@ -178,6 +178,12 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __
 __device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
   const bf16x4 lo = read_tr(img, row, col), hi = read_tr(img + 16 * ROWB, row, col);  // (16 rows on: the same swizzle)
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// what the rounding of (a, b) to the bf16 pair u took off, as another pair: the operand of a second product
+// (Up to 32 tokens, where a few probabilities make a whole row and their roundings do not average out; there it costs 0 to 3 %, at 49 tokens and heads of 32
+// 9 %, and the longer the row the more.)
+__device__ __forceinline__ uint32_t low_parts(uint32_t u, float a, float b) {
+  return pack_bf16x2(a - __builtin_bit_cast(float, u << 16), b - __builtin_bit_cast(float, u & 0xffff0000u));
 }
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float quarters_sum(float v) {
@@ -374,7 +380,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
       }
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
-        union { uint32_t u[4]; bf16x8 v; } pf;
+        union { uint32_t u[4]; bf16x8 v; } pf, pl;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           f32x4& x = sc[t + k];
@@ -385,10 +391,18 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
           }
           pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
           pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
+          if constexpr (W <= 2) {
+            pl.u[2 * k] = low_parts(pf.u[2 * k], x[0], x[1]);
+            pl.u[2 * k + 1] = low_parts(pf.u[2 * k + 1], x[2], x[3]);
+          }
           if constexpr (!ONE) x = load4f(rb, boff + (uint32_t)(k0 + Seg::SEG + 16 * (t + k)) * 4);
         }
 #pragma unroll
-        for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = mfma16(lds_tr_pair(imgV, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, o[eb]);
+        for (int eb = 0; eb < 2 * KS2; ++eb) {
+          const bf16x8 vf = lds_tr_pair(imgV, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+          o[eb] = mfma16(vf, pf.v, o[eb]);
+          if constexpr (W <= 2) o[eb] = mfma16(vf, pl.v, o[eb]);
+        }
       }
       if (!ONE && s + 1 < nseg) {
         sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
@@ -587,7 +601,7 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
         if (live && q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries' statistics say -inf)
-          union { uint32_t u[4]; bf16x8 v; } pf, df;
+          union { uint32_t u[4]; bf16x8 v; } pf, df, pl, sl;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             f32x4 dp = {0.f, 0.f, 0.f, 0.f};
@@ -613,11 +627,22 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
             pf.u[2 * k + 1] = pack_bf16x2(pr[2], pr[3]);
             df.u[2 * k] = pack_bf16x2(dp[0], dp[1]);
             df.u[2 * k + 1] = pack_bf16x2(dp[2], dp[3]);
+            if constexpr (W <= 2) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                pl.u[2 * k + i] = low_parts(pf.u[2 * k + i], pr[2 * i], pr[2 * i + 1]);
+                sl.u[2 * k + i] = low_parts(df.u[2 * k + i], dp[2 * i], dp[2 * i + 1]);
+              }
+            }
           }
 #pragma unroll
           for (int eb = 0; eb < 2 * KS2; ++eb) {
-            dv[eb] = mfma16(lds_tr_pair(imgD, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dv[eb]);
-            dk[eb] = mfma16(lds_tr_pair(imgQ, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), df.v, dk[eb]);
+            const bf16x8 gf = lds_tr_pair(imgD, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+            dv[eb] = mfma16(gf, pf.v, dv[eb]);
+            if constexpr (W <= 2) dv[eb] = mfma16(gf, pl.v, dv[eb]);
+            const bf16x8 qf = lds_tr_pair(imgQ, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+            dk[eb] = mfma16(qf, df.v, dk[eb]);
+            if constexpr (W <= 2) dk[eb] = mfma16(qf, sl.v, dk[eb]);
           }
         }
         if constexpr (!ONE) {
@@ -881,7 +906,7 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
     for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < KT; t += 2) {
-      union { uint32_t u[4]; bf16x8 v; } f;
+      union { uint32_t u[4]; bf16x8 v; } f, fl;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if (t + k == KT) {
@@ -895,10 +920,17 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
         }
         f.u[2 * k] = pack_bf16x2(sc[t + k][0], sc[t + k][1]);
         f.u[2 * k + 1] = pack_bf16x2(sc[t + k][2], sc[t + k][3]);
+        if constexpr (KT == 2) {
+          fl.u[2 * k] = low_parts(f.u[2 * k], sc[t + k][0], sc[t + k][1]);
+          fl.u[2 * k + 1] = low_parts(f.u[2 * k + 1], sc[t + k][2], sc[t + k][3]);
+        }
       }
 #pragma unroll
-      for (int eb = 0; eb < 2 * KS2; ++eb)
-        dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), f.v, dq[eb]);
+      for (int eb = 0; eb < 2 * KS2; ++eb) {
+        const bf16x8 kf = lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+        dq[eb] = mfma16(kf, f.v, dq[eb]);
+        if constexpr (KT == 2) dq[eb] = mfma16(kf, fl.v, dq[eb]);
+      }
       if constexpr (RES_GROUPS == 4) {
         if (t == KE / 6 * 2) { put(1, buf ^ 1); fetch(rn, 2); }
         if (t == KE / 6 * 4) { put(2, buf ^ 1); fetch(rn, 3); }
