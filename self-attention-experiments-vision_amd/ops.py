@@ -1011,8 +1011,19 @@ def relpos_index_1d(N: int, buckets: int = 32, max_distance: int = 128, device="
     d = torch.arange(N)[None, :] - torch.arange(N)[:, None]
     a, half = d.abs(), buckets // 2
     near = half // 2
-    far = near + (torch.log(a.clamp(min=1).double() / near) / math.log(max_distance / near) * (half - near)).long()
-    index = torch.where(a < near, a, far.clamp(max=half - 1)) + half * (d > 0).long()
+    wide = half - near
+    # where bucket near + k begins: the least a with (a / near)^wide >= (max_distance / near)^k, in whole numbers - a logarithm's rounding puts distances
+    # that lie on a border (10, 20 and 80 of 20 buckets up to 160) into the bucket before
+    begin = []
+    for k in range(1, wide):
+        least, x = near ** (wide - k) * max_distance ** k, round(near * (max_distance / near) ** (k / wide))
+        while x ** wide >= least:
+            x -= 1
+        while x ** wide < least:
+            x += 1
+        begin.append(x)
+    far = near + torch.searchsorted(torch.tensor(begin, dtype=torch.long), a, right=True)
+    index = torch.where(a < near, a, far) + half * (d > 0).long()
     return index.to(torch.int32).to(device).contiguous(), buckets
 
 
