@@ -374,11 +374,13 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     a_soft = (float)(gs * p.soft * p.T * mass) / S;
     base = (float)(gs * p.soft * p.T * left) / (float)(left != 0.0 ? p.C - distinct[sub] : 1) + (float)(gs * hard * p.smooth) / (float)p.C;
   }
-  // the gradient but for the target.  FAST: relative to M c rounded, the difference in the factor
+  // the gradient but for the target.  FAST: relative to M c rounded, as the sums were before residue() put them right: the same factor
   const bool fast = in_range(M * p.c_soft) && in_range(M * p.c_hard);
   const float Ms = M * p.c_soft, Mh = M * p.c_hard;
-  a_soft *= 1.f / residue(M, p.c_soft);
-  a_hard *= 1.f / residue(M, p.c_hard);
+  if (fast) {
+    a_soft *= residue(M, p.c_soft);
+    a_hard *= residue(M, p.c_hard);
+  }
   const float a_both = a_soft + a_hard;
   auto gradient = [&](float zj, auto is_fast) {
     constexpr bool FAST = decltype(is_fast)::value;

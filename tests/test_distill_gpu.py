@@ -313,3 +313,39 @@ def test_distill_offsets_beyond_32_bits(ops):
     rows = ops.distill_xent(z, top, at, labels=labels, dlogits=want, **kw)
     got = ops.distill_xent(big, top.repeat(n, 1), at.repeat(n, 1), labels=labels.repeat(n), dlogits=big, **kw)
     assert torch.equal(got[-16:], rows) and torch.equal(big[-16:], want) and torch.equal(big[:16], want)
+
+
+# --------------------------------------------------------------------------------------------- logits far from zero
+def check_shifted(ops, z, top, at, T, soft, lse, labels, hard, smooth, gdtype=torch.float32):
+    """Loss and gradient against 64 bits.  The reference sees the logits less their row's maximum (exact in 64 bits, and neither output changes by it), so
+    that its bounds know nothing of a common offset: the exponents are rounded as numbers of the size of z - max, and so is the sum of the logits."""
+    R, C = z.shape
+    dz = torch.empty(R, C, dtype=gdtype, device="cuda")
+    loss = ops.distill_xent(z, top, at, temperature=T, distill_weight=soft, teacher_lse=lse, labels=labels, hard_weight=hard, label_smoothing=smooth, dlogits=dz)
+    zd = z.double()
+    want, wz, ltol, tol = ref_distill(zd - zd.amax(1, keepdim=True), top, at, T, soft, lse, labels, hard, smooth, None, 1.0 / R)
+    assert bool(((loss.double() - want).abs() <= ltol).all()), float(((loss.double() - want).abs() / ltol).max())
+    u = U if gdtype == torch.bfloat16 else U32
+    err, lim = (dz.double() - wz).abs(), tol * (1 + u) + u * wz.abs() + 1e-40
+    assert bool((err <= lim).all()), float((err / lim).max())
+
+
+OFFSETS = [300.0, -300.0, 5000.0, 40000.0, -40000.0]
+
+
+@pytest.mark.parametrize("offset", OFFSETS)
+@pytest.mark.parametrize("T", [0.5, 1.0, 4.0])
+@pytest.mark.parametrize("C", [100, 1000, 21843])
+def test_distill_gradient_with_a_common_offset(ops, offset, T, C):
+    z, top, at, _, labels = make(4, C, 20, C, torch.float32)
+    z = z + offset
+    check_shifted(ops, z, top, at, T, 1.0, None, None, 0.0, 0.0)
+    check_shifted(ops, z, top, at, T, 0.6, None, labels, 0.4, 0.0)
+    check_shifted(ops, z.bfloat16(), top, at, T, 0.6, None, labels, 0.4, 0.0)
+
+
+@pytest.mark.parametrize("offset", [8e4, -8e4, 2e5, -2e5])
+def test_distill_gradient_with_an_offset_that_one_temperature_stretches(ops, offset):
+    """At temperature 4 the distillation's exponents are those of ordinary logits and the label term's are not."""
+    z, top, at, _, labels = make(4, 1000, 20, 3, torch.float32)
+    check_shifted(ops, z + offset, top, at, 4.0, 0.6, None, labels, 0.4, 0.0)
