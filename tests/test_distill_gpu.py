@@ -349,3 +349,13 @@ def test_distill_gradient_with_an_offset_that_one_temperature_stretches(ops, off
     """At temperature 4 the distillation's exponents are those of ordinary logits and the label term's are not."""
     z, top, at, _, labels = make(4, 1000, 20, 3, torch.float32)
     check_shifted(ops, z + offset, top, at, 4.0, 0.6, None, labels, 0.4, 0.0)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("C", [21843, 140003])
+def test_distill_maximum_across_the_border_of_the_short_form(ops, C, sign):
+    """Exponents beyond 1e5 are taken in another form: a row whose running maximum crosses that (z log2 e = 1e5) between one piece and the next."""
+    z, top, at, _, labels = make(4, C, 20, C, torch.float32, spread=0.5)
+    z = z + sign * 1e5 * math.log(2.0)
+    z[:, : C // 3] -= 1.5
+    check_shifted(ops, z, top, at, 1.0, 0.6, None, labels, 0.4, 0.0)
