@@ -11,7 +11,7 @@
 // Measured, with gradient: [2048 x 131072] 260 us (1075 MB, 4.1 TB/s; the loss alone 139; a copy of the bytes takes 216), [1024 x 21843] 39 us (135 MB, 3.5 TB/s), [128 x 1000]
 // 7 to 8 us: a launch, and the 64-bit logarithms and exponentials of the pairs one after the other.  What is left above the copy: a row's loads do not overlap the stores of the row before it in the same registers, and the exponentials (10 %).
 // Exponentials are v_exp_f32 on (z - max) * (log2 e / T), per-thread sums fp32; everything that exists once a row - the pairs, the
-// normalisers, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
+// normalisers, the sum of the logits, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
 // The gradient is written for every class as if no pair named it, then the at most K + 1 classes with a pair or the label are written again.
 #include <type_traits>
 
@@ -112,11 +112,12 @@ __device__ __forceinline__ void put_piece(bf16_t* p, const float (&v)[E], int n)
   }
 }
 
-// what a thread (a wave, the row) has seen: maximum, sums of exponentials relative to it at temperatures T and 1, sum of z.
+// what a thread (a wave, the row) has seen: maximum, sums of exponentials relative to it at temperatures T and 1.
 // The maximum starts at the lowest finite value: -inf then counts nothing, and a row of lowest values is uniform.
 struct Seen {
-  float m, s, h, z;
+  float m, s, h;
 };
+constexpr float LOW = -1e20f;  // logits below it (masked classes) are too large for a sum in 32 bits beside others
 
 __device__ __forceinline__ unsigned hash_of(int j) { return (unsigned)j * 2654435761u >> 16; }
 // the wave reductions in 64 bits: the same exchanges as wave_sum's, on both halves (a shuffle through LDS takes five times as long)
@@ -215,14 +216,15 @@ __device__ __forceinline__ float waves_max(float v) {
   return v;
 }
 
-// W waves a row (4 / W rows a block where W < 4), C pieces of the row kept by a thread, OCC waves a SIMD.
-template <typename TI, typename TO, int W, int C, int OCC>
+// W waves a row (4 / W rows a block where W < 4), C pieces of the row kept by a thread, OCC waves a SIMD.  SUM: the sum of the logits is needed (mass of the
+// teacher beside its pairs, label smoothing); a kernel of its own, as its registers cost the others 3 % at 131 072 classes.
+template <typename TI, typename TO, int W, int C, int OCC, bool SUM>
 __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(const DistillParams p) {
   constexpr int TH = 64 * W, RPB = W < 4 ? 4 / W : 1, E = Piece<TI>::E, GROUP = C % 4 == 0 ? 4 : 2;
   static_assert(C % GROUP == 0, "whole groups");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ Seen part[RPB][W];
-  __shared__ double tpart[RPB][W][2], lpart[RPB][W][2];
+  __shared__ double tpart[RPB][W][2], lpart[RPB][W][2], zpart[RPB][W];
   __shared__ int distinct[RPB], repeated[RPB];
   const int sub = RPB > 1 ? threadIdx.x / TH : 0;  // row of the block
   const int tid = RPB > 1 ? threadIdx.x - sub * TH : threadIdx.x;
@@ -246,7 +248,6 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
   const bool has_label = p.hard != 0.0f && (unsigned)label < (unsigned)p.C;
   const float zl = tid == TH - 64 && has_label ? to_float(z[label]) : 0.f;  // read before anything is written in z's place
   const bool two = p.hard != 0.0f && p.c_hard != p.c_soft;  // a second sum of exponentials
-  const bool need_z = p.lse != nullptr || p.smooth != 0.0f;
   auto fetch = [&](Piece<TI>& q, int i) {
     if (i < full) q.load(z + (size_t)i * E);
     else q.load_part(z + (size_t)i * E, p.C - i * E);
@@ -292,7 +293,8 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     for (int k = tid + TH; k < K; k += TH) zt[k] = pair(k, p.at[(size_t)row * K + k], p.top[(size_t)row * K + k]);
     if (mine) atomicAdd(&distinct[sub], mine);
   }
-  Seen me{-3.402823466e38f, 0.f, 0.f, 0.f};
+  Seen me{-3.402823466e38f, 0.f, 0.f};
+  double zsum = 0.0;  // of the logits
   if (live) {
     // G pieces at a time: one comparison with the running maximum, then independent exponentials (a piece at a time its short dependent
     // chains left a third of the time idle); pieces beyond the row are -inf and add nothing
@@ -310,13 +312,27 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       }
       me.s += sum_exps<G>(q, m, p.c_soft);
       if (two) me.h += sum_exps<G>(q, m, p.c_hard);
-      if (need_z) {
+      if constexpr (SUM) {  // a group's in 32 bits less the maximum, so that what all logits have in common costs nothing; the groups' in 64
+        float d = 0.f;
+        int count = 0;
 #pragma unroll
         for (int k = 0; k < G; ++k) {
           const int n = p.C - (i0 + k * TH) * E;
+          count += n < 0 ? 0 : n < E ? n : E;
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            if (e < n) me.z += q[k].get(e);
+            if (e < n) d += q[k].get(e) - m;
+        }
+        if (d > LOW && (count == 0 || fabsf(m) < -LOW)) {
+          zsum += (double)d + (double)count * m;
+        } else {
+#pragma unroll
+          for (int k = 0; k < G; ++k) {
+            const int n = p.C - (i0 + k * TH) * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (e < n) zsum += (double)q[k].get(e);
+          }
         }
       }
     };
@@ -335,7 +351,8 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     if (two) me.h *= residue(me.m, p.c_hard);
     const float M = wave_max(me.m);
     const Seen w{M, wave_sum(me.s * __builtin_amdgcn_exp2f((me.m - M) * p.c_soft)),
-                 two ? wave_sum(me.h * __builtin_amdgcn_exp2f((me.m - M) * p.c_hard)) : 0.f, need_z ? wave_sum(me.z) : 0.f};
+                 two ? wave_sum(me.h * __builtin_amdgcn_exp2f((me.m - M) * p.c_hard)) : 0.f};
+    if constexpr (SUM) zsum = wave_sum_d(zsum);
     double ts = 0.0;
     if (64 * wave < K) {
       tm = p.lse ? (live ? (double)p.lse[row] : 0.0) : wave_max_d(tm);  // what this wave's sum is relative to
@@ -345,6 +362,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     }
     if (first_lane) {
       part[sub][wave] = w;
+      if constexpr (SUM) zpart[sub][wave] = zsum;
       tpart[sub][wave][0] = tm;
       tpart[sub][wave][1] = ts;
     }
@@ -496,7 +514,8 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     named += lpart[sub][w][1];
   }
   double Z = 0.0;
-  for (int w = 0; w < W; ++w) Z += (double)part[sub][w].z;
+  if constexpr (SUM)
+    for (int w = 0; w < W; ++w) Z += zpart[sub][w];
   if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log_s - named);
   if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
   if (hard != 0.0) {
@@ -529,8 +548,8 @@ __global__ __launch_bounds__(1024) void distill_colsum_kernel(const T* __restric
 template <typename TI, typename TO, int W, int C, int OCC>
 int launch_distill(const DistillParams& p, hipStream_t st) {
   constexpr int RPB = W < 4 ? 4 / W : 1;
-  hipLaunchKernelGGL((distill_kernel<TI, TO, W, C, OCC>), dim3((unsigned)((p.R + RPB - 1) / RPB)), dim3(W < 4 ? 256 : 64 * W),
-                     (size_t)RPB * (p.K * 20 + p.slots * 4), st, p);
+  auto kfn = p.lse != nullptr || p.smooth != 0.0f ? distill_kernel<TI, TO, W, C, OCC, true> : distill_kernel<TI, TO, W, C, OCC, false>;
+  hipLaunchKernelGGL(kfn, dim3((unsigned)((p.R + RPB - 1) / RPB)), dim3(W < 4 ? 256 : 64 * W), (size_t)RPB * (p.K * 20 + p.slots * 4), st, p);
   SAVIT_LAUNCH_RET();
 }
 // A row's threads, and the pieces a thread keeps, grow with the row: a wave (no idle wave where rows are short), four, eight, sixteen; eight waves and

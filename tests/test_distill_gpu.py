@@ -359,3 +359,42 @@ def test_distill_maximum_across_the_border_of_the_short_form(ops, C, sign):
     z = z + sign * 1e5 * math.log(2.0)
     z[:, : C // 3] -= 1.5
     check_shifted(ops, z, top, at, 1.0, 0.6, None, labels, 0.4, 0.0)
+
+
+@pytest.mark.parametrize("offset", [0.0] + OFFSETS)
+@pytest.mark.parametrize("C,dtype", [(100, torch.float32), (1000, torch.float32), (21843, torch.float32), (70001, torch.float32), (3000, torch.bfloat16)])
+def test_distill_sums_of_logits_with_a_common_offset(ops, offset, C, dtype):
+    """The rest of the teacher's mass and the smoothing need the sum of all logits: it is no worse for an offset that all of them share."""
+    z, top, at, lse, labels = make(4, C, 20, C, dtype, lse=True, T=2.0)
+    z = (z.float() + offset).to(dtype)
+    check_shifted(ops, z, top, at, 2.0, 1.0, lse, None, 0.0, 0.0)
+    check_shifted(ops, z, top, at, 2.0, 0.6, None, labels, 0.4, 0.1)
+    check_shifted(ops, z, top, at, 2.0, 0.6, lse, labels, 0.4, 0.1)
+
+
+def test_distill_small_divergence_with_the_rest_and_an_offset(ops):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.randn(4, 50, generator=g, device="cuda") * 2
+    t = z + 1e-2 * torch.randn(4, 50, generator=g, device="cuda")
+    top, at = t.topk(30, dim=1)
+    lse = torch.logsumexp(t.double() / 4, 1).float()
+    for offset in (0.0, 4096.0):  # (a power of two: the differences of the logits stay what they were to 2^-11)
+        zo = z + offset
+        loss = ops.distill_xent(zo, top.contiguous(), at.int().contiguous(), temperature=4.0, teacher_lse=lse)
+        want, _, _, _ = ref_distill(zo.double() - offset, top, at.int(), 4.0, 1.0, lse, None, 0.0, 0.0, None, 1.0)
+        # as above: the normaliser's error times T^2, and the sum of 50 logits below 8: 50 roundings of 2^-24 of each, over the classes, times T
+        assert bool(((loss.double() - want).abs() < 16 * 8 * U32 + 4 * 50 * 8 * U32).all()), (loss, want)
+
+
+@pytest.mark.parametrize("C", [300, 140003])
+def test_distill_smoothing_over_the_lowest_logits(ops, C):
+    """Several classes at the type's lowest value: their sum passes what fp32 holds, their mean does not."""
+    z, top, at, _, labels = make(4, C, 8, C, torch.float32)
+    z[:, 50:60] = torch.finfo(torch.float32).min
+    labels[:] = 7
+    loss = ops.distill_xent(z, top, at, distill_weight=0.0, labels=labels, hard_weight=1.0, label_smoothing=0.1)
+    want = -0.1 * z.double().mean(1)
+    assert bool(((loss.double() / want - 1).abs() < 1e-5).all()), (loss, want)
+    z[:] = torch.finfo(torch.float32).min  # every class alike: uniform
+    loss = ops.distill_xent(z, top, at, distill_weight=0.0, labels=labels, hard_weight=1.0, label_smoothing=0.1)
+    assert bool(((loss.double() - math.log(C)).abs() < 64 * U32 * math.log(C)).all()), loss
