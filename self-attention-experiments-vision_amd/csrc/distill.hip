@@ -117,7 +117,7 @@ __device__ __forceinline__ void put_piece(bf16_t* p, const float (&v)[E], int n)
 struct Seen {
   float m, s, h;
 };
-constexpr float LOW = -1e20f;  // logits below it (masked classes) are too large for a sum in 32 bits beside others
+constexpr float LOW = -1e20f;  // logits at or below it are masked classes: their sum is one of its own, others would vanish beside it
 
 __device__ __forceinline__ unsigned hash_of(int j) { return (unsigned)j * 2654435761u >> 16; }
 // the wave reductions in 64 bits: the same exchanges as wave_sum's, on both halves (a shuffle through LDS takes five times as long)
@@ -176,21 +176,25 @@ __device__ __forceinline__ float rescale(float from, float to, float c) {
   if (in_range(from * c) && in_range(to * c)) return __builtin_amdgcn_exp2f(from * c - to * c);
   return __builtin_amdgcn_exp2f((from - to) * c) * residue(from, c) / residue(to, c);  // (one of them in range: a sum relative to its rounded product)
 }
-template <int G, typename T>
-__device__ __forceinline__ float sum_exps(const Piece<T>* q, float m, float c) {
+// SUM: and the sums of the exponents, a piece each
+template <int G, bool SUM, typename T>
+__device__ __forceinline__ float sum_exps(const Piece<T>* q, float m, float c, float (&x)[G]) {
   const float mb = m * c;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (in_range(mb)) {
+  auto sums = [&](auto exponent) {
 #pragma unroll
-    for (int k = 0; k < G; ++k)
+    for (int k = 0; k < G; ++k) {
+      x[k] = 0.f;
 #pragma unroll
-      for (int e = 0; e < Piece<T>::E; ++e) s[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(q[k].get(e), c, -mb));
-  } else {
-#pragma unroll
-    for (int k = 0; k < G; ++k)
-#pragma unroll
-      for (int e = 0; e < Piece<T>::E; ++e) s[e & 3] += __builtin_amdgcn_exp2f((q[k].get(e) - m) * c);
-  }
+      for (int e = 0; e < Piece<T>::E; ++e) {
+        const float v = exponent(q[k].get(e));
+        s[e & 3] += __builtin_amdgcn_exp2f(v);
+        if constexpr (SUM) x[k] += v;
+      }
+    }
+  };
+  if (in_range(mb)) sums([&](float z) { return __builtin_fmaf(z, c, -mb); });
+  else sums([&](float z) { return (z - m) * c; });
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
@@ -224,8 +228,9 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
   static_assert(C % GROUP == 0, "whole groups");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ Seen part[RPB][W];
-  __shared__ double tpart[RPB][W][2], lpart[RPB][W][2], zpart[RPB][W];
-  __shared__ int distinct[RPB], repeated[RPB];
+  __shared__ double tpart[RPB][W][2], lpart[RPB][W][2], xpart[RPB][W];
+  __shared__ double mpart[RPB][W][2];
+  __shared__ int distinct[RPB], repeated[RPB], masked[RPB];
   const int sub = RPB > 1 ? threadIdx.x / TH : 0;  // row of the block
   const int tid = RPB > 1 ? threadIdx.x - sub * TH : threadIdx.x;
   const int wave = tid >> 6;
@@ -267,7 +272,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     }
   }
   for (int i = tid; i < p.slots; i += TH) table[i] = -1;
-  if (tid == 0) distinct[sub] = repeated[sub] = 0;
+  if (tid == 0) distinct[sub] = repeated[sub] = masked[sub] = 0;
   __syncthreads();
 
   double tm = -1.7976931348623157e308;
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     if (mine) atomicAdd(&distinct[sub], mine);
   }
   Seen me{-3.402823466e38f, 0.f, 0.f};
-  double zsum = 0.0;  // of the logits
+  double xsum = 0.0;  // of the logits, times log2 e / T
   if (live) {
     // G pieces at a time: one comparison with the running maximum, then independent exponentials (a piece at a time its short dependent
     // chains left a third of the time idle); pieces beyond the row are -inf and add nothing
@@ -310,30 +315,31 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
         if (two) me.h *= rescale(me.m, m, p.c_hard);
         me.m = m;
       }
-      me.s += sum_exps<G>(q, m, p.c_soft);
-      if (two) me.h += sum_exps<G>(q, m, p.c_hard);
-      if constexpr (SUM) {  // a group's in 32 bits less the maximum, so that what all logits have in common costs nothing; the groups' in 64
-        float d = 0.f;
+      float x[G], none[G];
+      me.s += sum_exps<G, SUM>(q, m, p.c_soft, x);
+      if (two) me.h += sum_exps<G, false>(q, m, p.c_hard, none);
+      if constexpr (SUM) {  // the logits' sum, in units of the exponents: what they have in common is not in it, and goes in 64 bits a group
+        const float mb = m * p.c_soft;
+        const bool near = in_range(mb);
         int count = 0;
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const int n = p.C - (i0 + k * TH) * E;
-          count += n < 0 ? 0 : n < E ? n : E;
+          const int i = i0 + k * TH;
+          count += i < full ? E : i < pieces ? p.C - full * E : 0;
+          if (i >= full) {  // (columns beyond the row were -inf)
+            x[k] = 0.f;
+            if (i < pieces) {
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (e < n) d += q[k].get(e) - m;
-        }
-        if (d > LOW && (count == 0 || fabsf(m) < -LOW)) {
-          zsum += (double)d + (double)count * m;
-        } else {
-#pragma unroll
-          for (int k = 0; k < G; ++k) {
-            const int n = p.C - (i0 + k * TH) * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              if (e < n) zsum += (double)q[k].get(e);
+              for (int e = 0; e < E; ++e)
+                if (e < p.C - full * E) x[k] += near ? __builtin_fmaf(q[k].get(e), p.c_soft, -mb) : (q[k].get(e) - m) * p.c_soft;
+            }
           }
         }
+        float d = x[0];
+#pragma unroll
+        for (int k = 1; k < G; ++k) d += x[k];
+        if (d > 0.5f * LOW * p.c_soft && (count == 0 || fabsf(m) < -0.1f * LOW)) xsum += (double)d + (double)count * (near ? (double)mb : (double)m * p.c_soft);
+        else masked[sub] = 1;  // a masked class, perhaps: the row is summed again
       }
     };
 #pragma unroll
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     const float M = wave_max(me.m);
     const Seen w{M, wave_sum(me.s * __builtin_amdgcn_exp2f((me.m - M) * p.c_soft)),
                  two ? wave_sum(me.h * __builtin_amdgcn_exp2f((me.m - M) * p.c_hard)) : 0.f};
-    if constexpr (SUM) zsum = wave_sum_d(zsum);
+    if constexpr (SUM) xsum = wave_sum_d(xsum);
     double ts = 0.0;
     if (64 * wave < K) {
       tm = p.lse ? (live ? (double)p.lse[row] : 0.0) : wave_max_d(tm);  // what this wave's sum is relative to
@@ -362,12 +368,42 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     }
     if (first_lane) {
       part[sub][wave] = w;
-      if constexpr (SUM) zpart[sub][wave] = zsum;
+      if constexpr (SUM) xpart[sub][wave] = xsum;
       tpart[sub][wave][0] = tm;
       tpart[sub][wave][1] = ts;
     }
   }
   __syncthreads();
+
+  auto is_named = [&](int j) {
+    unsigned s = hash_of(j) & mask;
+    while (table[s] != -1 && table[s] != j) s = (s + 1) & mask;
+    return table[s] != -1;
+  };
+  if constexpr (SUM) {
+    if (masked[sub]) {  // in 64 bits; masked classes apart, and those apart that no pair names (a named one of probability 0 takes no part)
+      double all = 0.0, others = 0.0;
+      xsum = 0.0;
+#pragma unroll 1
+      for (int j = tid; j < p.C; j += TH) {
+        const float v = to_float(z[j]);
+        if (v <= LOW) {
+          all += (double)v;
+          if (!is_named(j)) others += (double)v;
+        } else {
+          xsum += (double)v * p.c_soft;
+        }
+      }
+      xsum = wave_sum_d(xsum);
+      all = wave_sum_d(all);
+      others = wave_sum_d(others);
+      if (first_lane) {
+        xpart[sub][wave] = xsum;
+        mpart[sub][wave][0] = all;
+        mpart[sub][wave][1] = others;
+      }
+    }
+  }
 
   // mass of the pairs with what is left over for the classes that no pair names
   auto masses = [&](double& mass, double& left) {
@@ -460,7 +496,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       inv = sum == 0.0 ? 0.0 : 1.0 / sum;
     }
     const double mine = apart(wave) * inv;
-    double kl = 0.0, named = 0.0;
+    double kl = 0.0, named = 0.0;  // (named: the sum of their logits)
     for (int k = tid; k < K; k += TH) {
       const int j = at[k];
       if (j < 0) continue;
@@ -477,7 +513,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       off[k] = (float)(gs * (p.soft * p.T * P + hard * ((j == label ? 1.0 - p.smooth : 0.0) + (double)p.smooth / p.C)));
       if (first) {
         const double lq = (double)(zt[k] - M) * ((double)p.c_soft * LN2) - log_s;
-        named += lq;
+        if (!(zt[k] <= LOW)) named += (double)zt[k];
         if (P != 0.0) kl += P * (log(P) - lq);
       }
     }
@@ -503,9 +539,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
   masses(mass, left);
   const double share = left != 0.0 ? left / (p.C - distinct[sub]) : 0.0;
   if (p.dz && has_label) {  // the label's class, unless a pair names it
-    unsigned s = hash_of(label) & mask;
-    while (table[s] != -1 && table[s] != label) s = (s + 1) & mask;
-    if (table[s] == -1) put(dz + label, gradient_any(zl) - (float)(gs * (p.soft * p.T * share + hard * (1.0 - p.smooth + (double)p.smooth / p.C))));
+    if (!is_named(label)) put(dz + label, gradient_any(zl) - (float)(gs * (p.soft * p.T * share + hard * (1.0 - p.smooth + (double)p.smooth / p.C))));
   }
   if (p.loss_rows == nullptr) return;
   double kl = 0.0, named = 0.0, loss = 0.0;
@@ -513,14 +547,24 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
     kl += lpart[sub][w][0];
     named += lpart[sub][w][1];
   }
-  double Z = 0.0;
+  double Z = 0.0, masked_all = 0.0, masked_others = 0.0;
   if constexpr (SUM)
-    for (int w = 0; w < W; ++w) Z += zpart[sub][w];
-  if (left != 0.0) kl += left * log(share) - share * ((Z - (double)p.C * M) * ((double)p.c_soft * LN2) - p.C * log_s - named);
+    for (int w = 0; w < W; ++w) {
+      Z += xpart[sub][w];
+      if (masked[sub]) {
+        masked_all += mpart[sub][w][0];
+        masked_others += mpart[sub][w][1];
+      }
+    }
+  Z /= (double)p.c_soft;
+  if (left != 0.0) {
+    const double others = p.C - distinct[sub];
+    kl += left * log(share) - share * ((Z - named + masked_others - others * M) * ((double)p.c_soft * LN2) - others * log_s);
+  }
   if (p.soft != 0.0f) loss = (double)p.soft * p.T * p.T * kl;
   if (hard != 0.0) {
     double ce = log_h - (1.0 - p.smooth) * ((double)zl - M);
-    if (p.smooth != 0.0f) ce -= p.smooth * (Z / p.C - M);
+    if (p.smooth != 0.0f) ce -= p.smooth * ((Z + masked_all) / p.C - M);
     loss += hard * ce;
   }
   p.loss_rows[row] = (float)(loss * weight);

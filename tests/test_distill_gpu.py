@@ -398,3 +398,36 @@ def test_distill_smoothing_over_the_lowest_logits(ops, C):
     z[:] = torch.finfo(torch.float32).min  # every class alike: uniform
     loss = ops.distill_xent(z, top, at, distill_weight=0.0, labels=labels, hard_weight=1.0, label_smoothing=0.1)
     assert bool(((loss.double() - math.log(C)).abs() < 64 * U32 * math.log(C)).all()), loss
+
+
+@pytest.mark.parametrize("masked", [-math.inf, torch.finfo(torch.float32).min, -1e30])
+@pytest.mark.parametrize("C", [300, 5000, 140003])
+def test_distill_masked_classes_with_the_rest(ops, C, masked):
+    """Classes that teacher and student both exclude, named by pairs of probability 0: they take no part, and the loss is that of the others."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    z, _, _, _, labels = make(4, C, 8, C, torch.float32)
+    out = torch.tensor([1, 2, 150, C - 1], device="cuda")
+    t = torch.randn(4, C, generator=g, device="cuda") * 3
+    t[:, out] = -math.inf
+    z[:, out] = masked
+    at = torch.cat([out.expand(4, 4), torch.arange(20, 40, device="cuda").expand(4, 20)], 1)
+    at = torch.cat([at, at[:, :2]], 1)  # one of them twice
+    top = t.gather(1, at)
+    top[:, -2:] = -math.inf
+    lse = torch.logsumexp(t.double(), 1).float()
+    dz = torch.empty_like(z)
+    loss = ops.distill_xent(z, top.contiguous(), at.int().contiguous(), teacher_lse=lse, dlogits=dz, grad_scale=1.0)
+    keep = torch.ones(C, dtype=torch.bool, device="cuda")
+    keep[out] = False
+    new = (keep.cumsum(0) - 1)[at[:, 4:24]].int()
+    want, wz, ltol, tol = ref_distill(z[:, keep], top[:, 4:24], new, 1.0, 1.0, lse, None, 0.0, 0.0, None, 1.0)
+    assert bool(((loss.double() - want).abs() <= ltol).all()), (loss, want)
+    assert bool((dz[:, ~keep] == 0).all()) and bool(((dz[:, keep].double() - wz).abs() <= tol + U32 * wz.abs()).all())
+    # excluded by the student alone: the divergence is infinite (or as large as the mask makes it)
+    z[:, 60] = masked
+    loss = ops.distill_xent(z, top.contiguous(), at.int().contiguous(), teacher_lse=lse)
+    if masked == -math.inf:
+        assert bool((loss == math.inf).all())
+    else:
+        share = ((1 - (top[:, 4:24].double() - lse.double()[:, None]).exp().sum(1)) / (C - 24))
+        assert bool(((loss.double() / (share * -masked) - 1).abs() < 1e-4).all()), (loss, share)  # (lse's own rounding, 2^-22 of exp, is in share too)
