@@ -401,9 +401,11 @@ int savit_softmax_xent(const float* logits, int ld_logits, const int* labels, co
  *   dlogits = grad_scale * d loss / d logits
  * logits fp32 or bf16 [R, ld], dlogits (nullable) fp32 or bf16 [R, ld_dlogits] - columns >= C are left alone; dlogits == logits is allowed with
  * equal type and pitch; any alignment of the element type.  teacher_logits fp32, teacher_index int32, both [R, K] compact, K <= 512: an index
- * outside [0, C) is no pair, one class named twice gets both probabilities; a row without pairs has no distillation term.  labels int32 [R]
+ * outside [0, C) is no pair, one class named twice gets both probabilities; a row without pairs has no distillation term, or, with teacher_lse, the
+ * uniform distribution as its target (all of the mass is left).  temperature in [1e-30, 1e30].  labels int32 [R]
  * (nullable when hard_weight == 0): outside [0, C) drops the row's hard term.  row_weight fp32 [R] (nullable = 1): rows of weight 0 are not read,
- * their loss and gradient are zero.  A -inf logit has q = 0; a row of nothing but -inf, or with +inf or NaN, is NaN.
+ * their loss and gradient are zero.  A -inf logit has q = 0: its class takes no part where P is 0 too, else the loss is infinite; a row of nothing but
+ * -inf, or with +inf or NaN, is NaN.
  * loss_rows fp32 [R] (nullable); dbias fp32 [C] (nullable) += column sums of dlogits as stored, in a fixed order. */
 int savit_distill_xent(const void* logits, long ld_logits, int logits_bf16, const float* teacher_logits, const int* teacher_index, int K,
                        const float* teacher_lse, const int* labels, const float* row_weight, float temperature, float distill_weight, float hard_weight,

@@ -617,7 +617,7 @@ extern "C" int savit_distill_xent(const void* logits, long ld_logits, int logits
                                   float hard_weight, float label_smoothing, float grad_scale, float* loss_rows, void* dlogits, long ld_dlogits,
                                   int dlogits_bf16, float* dbias, int R, int C, void* stream) {
   SAVIT_CHECK_ARG(logits && R >= 0 && C > 0 && ld_logits >= C && K >= 0 && K <= DS_MAX_K && (K == 0 || (teacher_logits && teacher_index)));
-  SAVIT_CHECK_ARG(temperature > 0.f && temperature < __builtin_inff() && (hard_weight == 0.f || labels) && label_smoothing >= 0.f && label_smoothing <= 1.f);
+  SAVIT_CHECK_ARG(temperature >= 1e-30f && temperature <= 1e30f && (hard_weight == 0.f || labels) && label_smoothing >= 0.f && label_smoothing <= 1.f);
   SAVIT_CHECK_ARG((dlogits || loss_rows) && (!dlogits || ld_dlogits >= C) && (!dbias || dlogits));
   SAVIT_CHECK_ARG(((uintptr_t)logits % (logits_bf16 ? 2 : 4)) == 0 && ((uintptr_t)dlogits % (dlogits_bf16 ? 2 : 4)) == 0);
   SAVIT_CHECK_ARG(dlogits != logits || (logits_bf16 == dlogits_bf16 && ld_logits == ld_dlogits));

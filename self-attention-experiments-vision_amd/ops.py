@@ -1166,7 +1166,7 @@ def distill_xent(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     hard-label loss beside it: per row
         distill_weight T^2 KL(P || softmax(logits / T)) + hard_weight CE(logits, smoothed label),
     P = softmax(teacher_logits / T) over the pairs, or with teacher_lse [R] (the teacher's log-sum-exp over all classes at temperature T) their
-    true probabilities, the rest spread evenly over the other classes.  logits fp32 / bf16 [R, C]; dlogits (optional, fp32 / bf16, may be logits
+    true probabilities, the rest spread evenly over the other classes (a row without pairs: over all).  logits fp32 / bf16 [R, C]; dlogits (optional, fp32 / bf16, may be logits
     itself) receives grad_scale (1 / R by default) times the gradient; dbias [C] accumulates its column sums.  Returns loss_rows [R].
     savit_distill_xent."""
     dev = _dev(logits)

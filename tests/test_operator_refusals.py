@@ -112,6 +112,12 @@ def test_distill(L, bad):
     assert distill(L, **bad) == EINVAL
 
 
+@pytest.mark.parametrize("T", [1e-39, 1e-31, 1e31, float("nan")])
+def test_distill_temperatures_without_a_scale(L, T):
+    """log2 e / T has to be an ordinary number."""
+    assert distill(L, T=T) == EINVAL
+
+
 def test_distill_nothing_to_do(L):
     assert distill(L, R=0) == 0
 
