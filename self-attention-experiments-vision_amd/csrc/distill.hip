@@ -173,6 +173,7 @@ __device__ __forceinline__ double lane_d(double v, int lane) {
 __device__ __forceinline__ bool in_range(float mb) { return fabsf(mb) < 1e5f; }
 __device__ __forceinline__ float residue(float m, float c) { return in_range(m * c) ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -(m * c))) : 1.f; }
 __device__ __forceinline__ float rescale(float from, float to, float c) {
+#pragma clang fp contract(off)  // both products rounded
   if (in_range(from * c) && in_range(to * c)) return __builtin_amdgcn_exp2f(from * c - to * c);
   return __builtin_amdgcn_exp2f((from - to) * c) * residue(from, c) / residue(to, c);  // (one of them in range: a sum relative to its rounded product)
 }
