@@ -287,7 +287,8 @@ int savit_relpos_bias_bwd(const float* dbias, const int* order, const int* start
 long savit_relpos_bias_bwd_workspace_bytes(int N, int H, int buckets);
 /* savit_bias_attention_fwd: savit_attention_fwd with S = q k^T + bias[h], bias fp32 [H, N, ld_bias] shared by the images (ld_bias % 4 == 0).
  *   lens int32 [B] (NULL: all N): keys and queries at or beyond lens[b] (clamped to [0, N]) take no part; their rows of o are zero, their lse is
- *   -inf - as those of a query whose bias masks every key.  A bias of -inf masks; so does float's or bfloat16's lowest value.  lse is required.
+ *   -inf - as those of a query whose bias masks every key.  Scores below -2^127 are masked (a bias of -inf, or of float's
+ *   or bfloat16's lowest value); any other bias is a number, however low: a row of nothing but -1e9 is uniform.  lse is required.
  * savit_bias_attention_bwd: dqkv as in savit_attention_bwd (rows of padding are zero); dbias fp32 [H, N, ld_bias] (nullable) = the sum of dS over
  *   the batch, in a fixed order (not in bias's place: later kernels read that).  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
  *   head_dim 16, 32, 48 or 64; N <= 32 768, and one image's rows and one head's bias each below 4 GiB; d_o, o compact [B*N, H*head_dim]. */

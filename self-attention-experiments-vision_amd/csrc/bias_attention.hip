@@ -2,7 +2,8 @@
 //   S[b,h,i,j] = q_i . k_j + bias[h,i,j] ;  P = softmax_j(S) ;  O = P V                (queries arrive scaled, as in attention.hip)
 //   dP = dO V^T ;  delta_i = sum_j P_ij dP_ij ;  dS = P (dP - delta) ;  dQ = dS K ;  dK = dS^T Q ;  dV = P^T dO ;  dbias[h] = sum_b dS
 // The batch may be padded: keys and queries at or beyond lens[b] take no part, their rows of O and of the gradients are zero, their
-// log-sum-exp -inf.  So are those of a query whose bias leaves no key (-inf, or the lowest value of float or bfloat16: scaled by log2 e it is -inf).
+// log-sum-exp -inf.  So are those of a query whose bias leaves no key: scores below -2^127 are masked (-inf, the lowest values of float and bfloat16).  Any other
+// mask is a number: among -1e9s alone the weights are uniform, as in a plain softmax.
 //
 // Tiles: a wave owns 16 or 32 queries (forward, dQ) or 16 keys (dK, dV); the other side streams through LDS in segments of 64 rows shared by the
 // W waves of a workgroup, fetched into registers under the arithmetic of the segment before and written to the other of two LDS buffers: one barrier a
@@ -32,7 +33,21 @@
 namespace {
 
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
-constexpr float LOWEST = -3.402823466e38f;
+// A row's exponentials are exp2(s log2 e - r), r = reference(m) of a score m of the row.  One multiply-add an element: its product is exact, so r has to be m log2 e
+// exactly where that is far from zero - rounded to 32 bits it is off by 440 at a mask of -1e10.  r is a pair there; b alone up to |m| = 2^20, where what b
+// was rounded by (2^-4 at the most) is common to the row's sum and its products.
+constexpr float FAR = 1048576.f;
+// Scores below it are masked: -inf, float's and bfloat16's lowest values; a row of nothing else is empty.  (A power of two: its own reference is exact.)
+constexpr float MASKED = -1.7014118346046923e38f;
+struct Reference {
+  float b, lo;  // b + lo
+};
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= FAR && m != MASKED; }
+__device__ __forceinline__ Reference reference(float m) {
+#pragma clang fp contract(off)  // b is the ROUNDED product, wherever it goes
+  const float b = m * LOG2E_F;
+  return {b, fabsf(m) < FAR ? 0.f : __builtin_fmaf(m, LOG2E_F, -b)};
+}
 
 struct BiasAttnParams {
   const bf16_t* qkv;
@@ -227,6 +242,22 @@ __device__ __forceinline__ void item_of(const BiasAttnParams& p, int& h, int& b,
   h = p.image_major ? r % p.H : r / p.B;
 }
 
+// forward: the reference's score follows the maximum once it is 2^8 behind; returns what the sums so far are multiplied by
+constexpr float BEHIND = 5.5f;
+__device__ __forceinline__ float follow(float& m, float top) {
+#pragma clang fp contract(off)
+  const Reference from = reference(m);
+  m = fmaxf(m, top);
+  const Reference to = reference(m);
+  return __builtin_amdgcn_exp2f((from.b - to.b) + (from.lo - to.lo));
+}
+// m + log l: the sum was relative to reference(m), which is m log2 e but for b's rounding
+__device__ __forceinline__ float log_sum(float m, float l) {
+#pragma clang fp contract(off)
+  const Reference rf = reference(m);
+  return __builtin_fmaf(__log2f(l) - (__builtin_fmaf(m, LOG2E_F, -rf.b) - rf.lo), LN2_F, m);
+}
+
 template <int KS>
 __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnParams p) {
   constexpr int W = 4;
@@ -247,7 +278,8 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
   const int nseg = blk * W * 32 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;  // a block beyond the sequence only clears its rows
   Seg sg;
   f32x16 oacc[2] = {zero16(), zero16()};
-  float m = LOWEST, l = 0.f;  // running reference (log2 units) and sum
+  float m = MASKED, l = 0.f;  // score that the reference is made of, and the running sum relative to it
+  bool far = false;           // some query of the wave has one far from zero
   if (nseg > 0) {
     bf16x8 qf[KS];
     sg.fetch(rs, (uint32_t)p.ld * 2, ck, rs, (uint32_t)p.ld * 2, cv, 0, len);
@@ -272,22 +304,29 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
         float top = sc[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
-        top = half_max(top) * LOG2E_F;
+        top = half_max(top);
         // the reference follows the maximum only when it is more than 2^8 behind (P then stays below 2^8, exact in range for fp32 sums and bf16
         // operands alike): most tiles after the first skip the rescaling of the accumulators
-        if (__any(top > m + 8.f)) {
-          const float mn = fmaxf(m, top);
-          const float alpha = __builtin_amdgcn_exp2f(m - mn);
+        if (__any(top > m + BEHIND)) {
+          const float alpha = follow(m, top);
           l *= alpha;
 #pragma unroll
           for (int eb = 0; eb < 2; ++eb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) oacc[eb][r] *= alpha;
-          m = mn;
+          far = __any(is_far(m));
+        }
+        float scale = LOG2E_F, ref = m * LOG2E_F;
+        if (far) {
+          const Reference rf = reference(m);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[r] = __builtin_fmaf(sc[r], LOG2E_F, -rf.b) - rf.lo;
+          scale = 1.f;
+          ref = 0.f;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, -m));
+          sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -ref));
           l += sc[r];
         }
         tile_accumulate<KS>(oacc, imgV, 32 * t, sc, L);
@@ -305,7 +344,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
     const bool some = ok && l != 0.f;
     if (!some) oacc[0] = oacc[1] = zero16();
     store_row_tile(p.o + ((size_t)b * p.N + q) * p.d + h * hd, oacc, L.half, hd, some ? 1.0f / l : 0.f);
-    if (L.half == 0) p.lse[((size_t)b * p.H + h) * p.N + q] = some ? (m + __log2f(l)) * LN2_F : -INFINITY;
+    if (L.half == 0) p.lse[((size_t)b * p.H + h) * p.N + q] = some ? log_sum(m, l) : -INFINITY;
   }
 }
 
@@ -331,7 +370,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
   f32x4 o[2 * KS2];
 #pragma unroll
   for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = LOWEST, l = 0.f;  // running reference (log2 units) and sum
+  float m = MASKED, l = 0.f;  // as above
+  bool far = false;
   if (nseg > 0) {
     bf16x8 qf[KS2];
     sg.fetch(rs, ld2, d2 + hcol, rs, ld2, 2 * d2 + hcol, 0, len, p.hd / 8);
@@ -369,14 +409,23 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
       for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
-      top = quarters_max(top) * LOG2E_F;
-      if (__any(top > m + 8.f)) {  // as above
-        const float mn = fmaxf(m, top);
-        const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      top = quarters_max(top);
+      if (__any(top > m + BEHIND)) {
+        const float alpha = follow(m, top);
         l *= alpha;
 #pragma unroll
         for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] *= alpha;
-        m = mn;
+        far = __any(is_far(m));
+      }
+      float scale = LOG2E_F, ref = m * LOG2E_F;
+      if (far) {
+        const Reference rf = reference(m);
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_fmaf(sc[t][r], LOG2E_F, -rf.b) - rf.lo;
+        scale = 1.f;
+        ref = 0.f;
       }
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
@@ -386,7 +435,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
           f32x4& x = sc[t + k];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], LOG2E_F, -m));
+            x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale, -ref));
             l += x[r];
           }
           pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
@@ -418,7 +467,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
       for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     store_row16<KS2>(p.o + ((size_t)b * p.N + q) * p.d + h * p.hd, o, g, p.hd, some ? 1.0f / l : 0.f);
-    if (g == 0) p.lse[((size_t)b * p.H + h) * p.N + q] = some ? (m + __log2f(l)) * LN2_F : -INFINITY;
+    if (g == 0) p.lse[((size_t)b * p.H + h) * p.N + q] = some ? log_sum(m, l) : -INFINITY;
   }
 }
 
