@@ -34,8 +34,8 @@ namespace {
 
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 // A row's exponentials are exp2(s log2 e - r), r = reference(m) of a score m of the row.  One multiply-add an element: its product is exact, so r has to be m log2 e
-// exactly where that is far from zero - rounded to 32 bits it is off by 440 at a mask of -1e10.  r is a pair there; b alone up to |m| = 2^20, where what b
-// was rounded by (2^-4 at the most) is common to the row's sum and its products.
+// exactly where that is far from zero - rounded to 32 bits it is off by 440 at a mask of -1e10.  It is a pair there, and the exponentials are
+// exp2((s - m) log2 e), an instruction more; b alone up to |m| = 2^20, where what b was rounded by (2^-4 at the most) is common to a row's sum and products.
 constexpr float FAR = 1048576.f;
 // Scores below it are masked: -inf, float's and bfloat16's lowest values; a row of nothing else is empty.  (A power of two: its own reference is exact.)
 constexpr float MASKED = -1.7014118346046923e38f;
@@ -57,7 +57,7 @@ struct BiasAttnParams {
   float* lse;          // [B, H, N]
   const bf16_t* d_o;
   bf16_t* dqkv;
-  float* stat;         // backward: [B, H, 2, Np]: -lse log2 e (-inf where the query takes no part), delta
+  float* stat;         // backward: [B, H, 3, Np]: P = exp2((s - first) log2 e - second); the first is inf where the query takes no part; delta
   float* dbias;        // [H, N, ldb], or the slab [parts][H, N, ldb]
   int B, N, H, ld, d, ldb, Np;
   int hd;
@@ -258,6 +258,26 @@ __device__ __forceinline__ float log_sum(float m, float l) {
   return __builtin_fmaf(__log2f(l) - (__builtin_fmaf(m, LOG2E_F, -rf.b) - rf.lo), LN2_F, m);
 }
 
+// backward: the exponentials are taken relative to a row's log-sum-exp.  That is one 32-bit number: far from zero it holds the row's maximum and little of the
+// sum's logarithm.  The dQ kernels, which see all of a row, therefore sum the exponentials again: P is the forward's whatever the scores have in common (taken
+// from the log-sum-exp alone it was off by 1e-3 at a common bias of 1e4, by a factor of 230 in a row of nothing but -1e8).
+struct RowReference {
+  float less, b;  // exponentials: exp2((s - less) log2 e - b); s - less where some row of the wave is far
+  float shift;    // b + less log2 e - m log2 e
+  bool far;
+  __device__ __forceinline__ RowReference(float m) {
+#pragma clang fp contract(off)
+    far = fabsf(m) >= FAR && m != INFINITY;  // (inf, a row that takes no part: its exponentials are 0)
+    less = far ? m : 0.f;
+    b = far ? 0.f : m * LOG2E_F;
+    shift = far ? 0.f : -__builtin_fmaf(m, LOG2E_F, -b);
+  }
+  // log2 of the sum relative to m log2 e, of one relative to this
+  __device__ __forceinline__ float rest(float sum) const { return sum == 0.f ? 0.f : __log2f(sum) + shift; }
+};
+// a row's log-sum-exp as a reference: inf where it takes no part
+__device__ __forceinline__ float or_none(float lse) { return lse == -INFINITY ? INFINITY : lse; }
+
 template <int KS>
 __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnParams p) {
   constexpr int W = 4;
@@ -316,17 +336,16 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
             for (int r = 0; r < 16; ++r) oacc[eb][r] *= alpha;
           far = __any(is_far(m));
         }
-        float scale = LOG2E_F, ref = m * LOG2E_F;
+        float ref = m * LOG2E_F;
         if (far) {
-          const Reference rf = reference(m);
+          const float less = is_far(m) ? m : 0.f;
+          if (is_far(m)) ref = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[r] = __builtin_fmaf(sc[r], LOG2E_F, -rf.b) - rf.lo;
-          scale = 1.f;
-          ref = 0.f;
+          for (int r = 0; r < 16; ++r) sc[r] -= less;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -ref));
+          sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, -ref));
           l += sc[r];
         }
         tile_accumulate<KS>(oacc, imgV, 32 * t, sc, L);
@@ -417,15 +436,12 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
         for (int eb = 0; eb < 2 * KS2; ++eb) o[eb] *= alpha;
         far = __any(is_far(m));
       }
-      float scale = LOG2E_F, ref = m * LOG2E_F;
+      float ref = m * LOG2E_F;
       if (far) {
-        const Reference rf = reference(m);
+        const float less = is_far(m) ? m : 0.f;
+        if (is_far(m)) ref = 0.f;
 #pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_fmaf(sc[t][r], LOG2E_F, -rf.b) - rf.lo;
-        scale = 1.f;
-        ref = 0.f;
+        for (int t = 0; t < T; ++t) sc[t] -= less;
       }
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
@@ -435,7 +451,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
           f32x4& x = sc[t + k];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale, -ref));
+            x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], LOG2E_F, -ref));
             l += x[r];
           }
           pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
@@ -490,11 +506,10 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
   const uint32_t boff = q < p.N ? (uint32_t)(q * p.ldb + 4 * g) * 4 : BEYOND;
   const int nseg = blk * W * 16 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
-  float nl = -INFINITY, delta = 0.f;
-  if (q < len) {
-    const float v = p.lse[((size_t)b * p.H + h) * p.N + q];
-    nl = v == -INFINITY ? -INFINITY : -LOG2E_F * v;
-  }
+  const float m = or_none(q < len ? p.lse[((size_t)b * p.H + h) * p.N + q] : -INFINITY);
+  const RowReference rf(m);
+  const bool far = __any(rf.far);
+  float delta = 0.f, sum = 0.f, inv = 0.f;
   Seg sg;
   f32x4 dq[2 * KS2];
 #pragma unroll
@@ -532,10 +547,14 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
             dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
           }
         }
+        if (far) {
+#pragma unroll
+          for (int t = 0; t < T; ++t) sc[t] -= rf.less;
+        }
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+          for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, -rf.b));
         if (last) {
 #pragma unroll
           for (int t = 0; t < T; ++t)
@@ -555,7 +574,10 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
               pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
             } else {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) delta += x[r] * dp[t + k][r];
+              for (int r = 0; r < 4; ++r) {
+                sum += x[r];
+                delta += x[r] * dp[t + k][r];
+              }
             }
             x = load4f(rb, boff + (uint32_t)(kn + 16 * (t + k)) * 4);
           }
@@ -572,19 +594,23 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
       }
     };
     pass(std::false_type{});
-    delta = quarters_sum(delta);
+    sum = quarters_sum(sum);
+    inv = sum == 0.f ? 0.f : 1.f / sum;
+    delta = quarters_sum(delta) * inv;
     pass(std::true_type{});
   }
-  if (q >= len) {
-    delta = 0.f;
+  float rest = rf.rest(sum);
+  if (q >= len) {  // whatever the bias holds in such a row
+    delta = rest = inv = 0.f;
 #pragma unroll
     for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (q < p.N) store_row16<KS2>(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd, dq, g, p.hd, p.dq_scale);
+  if (q < p.N) store_row16<KS2>(p.dqkv + ((size_t)b * p.N + q) * p.ld + h * p.hd, dq, g, p.hd, p.dq_scale * inv);
   if (g == 0 && q < p.Np) {
-    float* st = p.stat + ((size_t)b * p.H + h) * 2 * p.Np + q;
-    st[0] = nl;
-    st[p.Np] = delta;
+    float* st = p.stat + ((size_t)b * p.H + h) * 3 * p.Np + q;
+    st[0] = m;
+    st[p.Np] = rest;
+    st[2 * p.Np] = delta;
   }
 }
 
@@ -595,7 +621,8 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   typedef Segment<W, 2 * KS2> Seg;
   constexpr int T = Seg::SEG / 16;
   __shared__ __attribute__((aligned(16))) char smem[(ONE ? 2 : 4) * Seg::IMG];
-  __shared__ float stats[ONE ? 1 : 2][64 * W];  // of the two buffers: SEG times -lse log2 e, SEG times delta (and what the other threads write)
+  constexpr int SL = (3 * Seg::SEG + 64 * W - 1) / (64 * W);
+  __shared__ float stats[ONE ? 1 : 2][64 * W * SL];  // of the two buffers: SEG of each of the three statistics (and what the other threads write)
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
@@ -607,19 +634,23 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2);
   const auto rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
   const auto rb = rsrc_of(p.bias + (size_t)h * p.N * p.ldb, (size_t)p.N * p.ldb * 4);
-  const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
+  const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 3 * p.Np, (size_t)p.Np * 12);
   const uint32_t boff = (uint32_t)(4 * g * p.ldb + key) * 4, brow = (uint32_t)p.ldb * 4;
   const int nseg = blk * W * 16 < len ? (len + Seg::SEG - 1) / Seg::SEG : 0;
   Seg sg;
-  float st = 0.f;
+  float st[SL];
   auto fetch = [&](int q0) {
     sg.fetch(rs, ld2, hcol, rd, d2, hcol, q0, len, p.hd / 8);
-    const uint32_t row = q0 + threadIdx.x % Seg::SEG + (threadIdx.x < Seg::SEG ? 0 : p.Np);
-    st = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, threadIdx.x < 2 * Seg::SEG ? row * 4 : OUTSIDE, 0, 0));
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      const uint32_t i = threadIdx.x + k * 64 * W, row = q0 + i % Seg::SEG + i / Seg::SEG * p.Np;
+      st[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, i < 3 * Seg::SEG ? row * 4 : OUTSIDE, 0, 0));
+    }
   };
   auto put = [&](int buf) {
     sg.put(smem + buf * 2 * Seg::IMG);
-    stats[buf][threadIdx.x] = st;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) stats[buf][threadIdx.x + k * 64 * W] = st[k];
   };
   f32x4 dk[2 * KS2], dv[2 * KS2];
 #pragma unroll
@@ -649,7 +680,7 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
       const char* imgD = imgQ + Seg::IMG;
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
-        if (live && q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries' statistics say -inf)
+        if (live && q0 + 16 * t < len) {  // (uniform; the second tile of a pair may lie beyond: its queries take no part)
           union { uint32_t u[4]; bf16x8 v; } pf, df, pl, sl;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -659,12 +690,13 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
               sc[t + k] = mfma16(row_frag(imgQ, 16 * (t + k) + ql, 4 * ks + g), kf[ks], sc[t + k]);
               dp = mfma16(row_frag(imgD, 16 * (t + k) + ql, 4 * ks + g), vf[ks], dp);
             }
-            const f32x4 nl = *reinterpret_cast<const f32x4*>(&stats[s & 1][16 * (t + k) + 4 * g]);
-            const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][Seg::SEG + 16 * (t + k) + 4 * g]);
+            const f32x4 m = *reinterpret_cast<const f32x4*>(&stats[s & 1][16 * (t + k) + 4 * g]);
+            const f32x4 rest = *reinterpret_cast<const f32x4*>(&stats[s & 1][Seg::SEG + 16 * (t + k) + 4 * g]);
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(&stats[s & 1][2 * Seg::SEG + 16 * (t + k) + 4 * g]);
             float pr[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t + k][r], LOG2E_F, nl[r]));
+              pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t + k][r] - m[r], LOG2E_F, -rest[r]));
               dp[r] = pr[r] * (dp[r] - dl[r]);
             }
             if (q0 + 16 * (t + k) + 16 > len) {  // whatever the bias holds there
@@ -744,20 +776,21 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
   }
   Seg sg;
   bf16x8 qn[KS], dn[KS];
-  float nln, deltan;
+  float mn, restn, deltan;
   auto fetch = [&](int b, bool any) {  // an image's operands, one image ahead (any: or nothing, out of range)
     const int len = any ? length_of(p, b) : 0;
     const uint32_t ld2 = (uint32_t)p.ld * 2, d2 = (uint32_t)p.d * 2, col = (uint32_t)(h * hd + 8 * L.half) * 2;
     const auto rs = rsrc_of(p.qkv + (size_t)b * p.N * p.ld, (size_t)len * ld2), rd = rsrc_of(p.d_o + (size_t)b * p.N * p.d, (size_t)len * d2);
-    const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
+    const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 3 * p.Np, (size_t)p.Np * 12);
     sg.fetch(rs, ld2, ck, rs, ld2, cv, k0, len);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qn[ks] = __builtin_bit_cast(bf16x8, load16(rs, only(q < len, (uint32_t)q * ld2 + col + 32 * ks)));
       dn[ks] = __builtin_bit_cast(bf16x8, load16(rd, only(q < len, (uint32_t)q * d2 + col + 32 * ks)));
     }
-    nln = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)q * 4), 0, 0));
-    deltan = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)(q + p.Np) * 4), 0, 0));
+    mn = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)q * 4), 0, 0));
+    restn = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)(q + p.Np) * 4), 0, 0));
+    deltan = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rt, only(q < p.Np, (uint32_t)(q + 2 * p.Np) * 4), 0, 0));
   };
   if (b0 < b1) {
     fetch(b0, true);
@@ -773,7 +806,7 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
       qf[ks] = qn[ks];
       df[ks] = dn[ks];
     }
-    const float nl = nln, delta = deltan;
+    const float m = mn, rest = restn, delta = deltan;
     fetch(more ? b + 1 : b, more);
     __builtin_amdgcn_sched_barrier(0);  // (else the loads sink to their use)
     const char* imgK = smem + ((b - b0) & 1) * 2 * Seg::IMG;
@@ -789,7 +822,7 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
 #pragma unroll
     for (int t = 0; t < T; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl)) * (dp[t][r] - delta);
+      for (int r = 0; r < 16; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r] - m, LOG2E_F, -rest)) * (dp[t][r] - delta);
       if (k0 + 32 * t + 32 > len) mask_keys(sc[t], k0 + 32 * t, len, L, 0.f);
       if (q < len) {  // (whatever the bias holds in other rows)
 #pragma unroll
@@ -926,23 +959,33 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
         dp[t] = mfma16(row_frag(imgV, 16 * t + ql, 4 * ks + g), df[ks], dp[t]);
       }
     }
-    const float nl = q < len && lse != -INFINITY ? -LOG2E_F * lse : -INFINITY;
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    const float m = or_none(q < len ? lse : -INFINITY);
+    const RowReference rf(m);
+    if (__any(rf.far)) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) sc[t] -= rf.less;
+    }
+    float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, nl));
+      for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], LOG2E_F, -rf.b));
       if (16 * t + 16 > len) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (16 * t + 4 * g + r >= len) sc[t][r] = 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) d[r] += sc[t][r] * dp[t][r];
+      for (int r = 0; r < 4; ++r) {
+        e[r] += sc[t][r];
+        d[r] += sc[t][r] * dp[t][r];
+      }
     }
-    float delta = quarters_sum((d[0] + d[1]) + (d[2] + d[3]));
+    const float sum = quarters_sum((e[0] + e[1]) + (e[2] + e[3]));
+    float inv = sum == 0.f ? 0.f : 1.f / sum, rest = rf.rest(sum);
+    float delta = quarters_sum((d[0] + d[1]) + (d[2] + d[3])) * inv;
     if (q >= len) {  // whatever the bias holds in such a row
-      delta = 0.f;
+      delta = inv = rest = 0.f;
 #pragma unroll
       for (int t = 0; t < KT; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -965,7 +1008,7 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           sc[t + k][r] *= dp[t + k][r] - delta;
-          if constexpr (DB) acc[t + k][r] += sc[t + k][r];
+          if constexpr (DB) acc[t + k][r] = __builtin_fmaf(sc[t + k][r], inv, acc[t + k][r]);
         }
         f.u[2 * k] = pack_bf16x2(sc[t + k][0], sc[t + k][1]);
         f.u[2 * k + 1] = pack_bf16x2(sc[t + k][2], sc[t + k][3]);
@@ -991,13 +1034,16 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
       if (AHEAD && t == KT / 4 * 2) load_queries(bn, lenn);
     }
     const auto ro = rsrc_of(p.dqkv + (size_t)b * p.N * p.ld, (size_t)p.N * ld2);
-    pieces_of_row16<KS2>(dq, g, p.dq_scale, [&](int col, u32x4 v) { store16(ro, only(q < p.N && col < p.hd, (uint32_t)q * ld2 + hcol + 2 * col), v); });
+    pieces_of_row16<KS2>(dq, g, p.dq_scale * inv, [&](int col, u32x4 v) { store16(ro, only(q < p.N && col < p.hd, (uint32_t)q * ld2 + hcol + 2 * col), v); });
     {  // statistics of the queries, and of the padding up to Np (fewer than three times the rows here) that the dK / dV kernel's tiles read
       const int row = q + g * (int)(blockDim.x >> 6) * 16 * p.blocks;
-      const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 2 * p.Np, (size_t)p.Np * 8);
-      const uint32_t off = only(row < p.Np, (uint32_t)row * 4), off2 = only(row < p.Np, (uint32_t)(row + p.Np) * 4);
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, g == 0 ? nl : -INFINITY), rt, off, 0, 0);
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, g == 0 ? delta : 0.f), rt, off2, 0, 0);
+      const auto rt = rsrc_of(p.stat + ((size_t)b * p.H + h) * 3 * p.Np, (size_t)p.Np * 12);
+      auto put_stat = [&](int k, float v) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rt, only(row < p.Np, (uint32_t)(row + k * p.Np) * 4), 0, 0);
+      };
+      put_stat(0, g == 0 ? m : INFINITY);
+      put_stat(1, g == 0 ? rest : 0.f);
+      put_stat(2, g == 0 ? delta : 0.f);
     }
     put(RES_GROUPS - 1, buf ^ 1);
     if constexpr (!AHEAD) load_queries(bn, lenn);
@@ -1163,7 +1209,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
 extern "C" long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, int ld_bias, int want_dbias) {
   if (!(B >= 0 && N > 0 && N <= 32768 && H > 0 && ld_bias >= N)) return 0;
   const int parts = dbias_parts(B, N, H);
-  return (long)B * H * 2 * padded(N) * 4 + (want_dbias && parts > 1 ? (long)parts * H * N * ld_bias * 4 : 0);
+  return (long)B * H * 3 * padded(N) * 4 + (want_dbias && parts > 1 ? (long)parts * H * N * ld_bias * 4 : 0);
 }
 
 extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, const int* lens, const void* d_o, const float* lse, void* dqkv, float* dbias, int B,
@@ -1181,7 +1227,7 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   p.Np = padded(N);
   p.stat = (float*)workspace;
   const int parts = dbias_parts(B, N, H);
-  float* slab = parts == 1 ? dbias : p.stat + (size_t)B * H * 2 * p.Np;
+  float* slab = parts == 1 ? dbias : p.stat + (size_t)B * H * 3 * p.Np;
   p.parts = parts;
   p.dbias = slab;
   if (resident(N)) {

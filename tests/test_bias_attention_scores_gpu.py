@@ -170,3 +170,39 @@ def test_masks_of_several_sizes(ops, B, N, H, hd):
     # u for P and for the output; the exponents of scores below 4 and what follows them, under 200 roundings, and the sum's N
     assert bool(((heads(o, B, N, H, hd) - p @ v).abs() <= (2 * U + (N + 200) * U32) * (p @ v.abs()) + 1e-30).all())
     assert bool((lse[:, :, 7] == -math.inf).all()) and bool(lse[:, :, 8:].isfinite().all())
+
+
+# --------------------------------------------------------------------------------------------- gradients
+@pytest.mark.parametrize("offset", OFFSETS)
+@pytest.mark.parametrize("B,N,H,hd", SIZES + WIDE)
+def test_gradients_of_scores_with_a_common_offset(ops, B, N, H, hd, offset):
+    qkv, bias, d_o = with_offset(ops, B, N, H, hd, offset)
+    check(ops, qkv, bias, B, N, H, hd, d_o, 0.5)
+
+
+@pytest.mark.parametrize("masked", MASKS)
+@pytest.mark.parametrize("B,N,H,hd", SIZES + WIDE)
+def test_gradients_with_large_finite_masks(ops, B, N, H, hd, masked):
+    """Among them rows that are masked all over: their probabilities are uniform in the gradients too."""
+    qkv, bias, d_o, kw = with_mask(ops, B, N, H, hd, masked)
+    check(ops, qkv, bias, B, N, H, hd, d_o, 0.5, **kw)
+
+
+@pytest.mark.parametrize("B,N,H,hd", MANY)
+def test_gradients_with_masks_of_several_sizes(ops, B, N, H, hd):
+    qkv, bias, d_o, p, v = with_masks(ops, B, N, H, hd)
+    d = H * hd
+    _, lse = ops.bias_attention_fwd(qkv, bias, B, N, H, head_dim=hd)
+    dqkv, dbias = ops.bias_attention_bwd(qkv, bias, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd)
+    do = heads(d_o, B, N, H, hd)
+    dv, dva = p.transpose(2, 3) @ do, p.transpose(2, 3) @ do.abs()
+    assert bool(((heads(dqkv[:, 2 * d:3 * d], B, N, H, hd) - dv).abs() <= (2 * U + (N + 200) * U32) * dva + 1e-30).all())
+    assert bool((dbias[:, 7] == 0).all()) and bool(dqkv[:, : 3 * d].isfinite().all()) and bool(dbias.isfinite().all())
+
+
+@pytest.mark.parametrize("B,N,H,hd", [(300, 49, 4, 32), (45, 197, 6, 64), (20, 257, 8, 64)])
+def test_gradients_with_masks_over_many_images(ops, B, N, H, hd):
+    """Several images a workgroup, of different lengths."""
+    qkv, bias, d_o, kw = with_mask(ops, B, N, H, hd, -1e9)
+    lens = torch.randint(0, N + 1, (B,), generator=gen(1), device="cuda", dtype=torch.int32)
+    check(ops, qkv, bias, B, N, H, hd, d_o, 0.5, lens=lens, **kw)
