@@ -290,7 +290,7 @@ long savit_relpos_bias_bwd_workspace_bytes(int N, int H, int buckets);
  *   -inf - as those of a query whose bias masks every key.  Scores below -2^127 are masked (a bias of -inf, or of float's
  *   or bfloat16's lowest value); any other bias is a number, however low: a row of nothing but -1e9 is uniform.  lse is required.
  * savit_bias_attention_bwd: dqkv as in savit_attention_bwd (rows of padding are zero); dbias fp32 [H, N, ld_bias] (nullable) = the sum of dS over
- *   the batch, in a fixed order (not in bias's place: later kernels read that).  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
+ *   the batch, in a fixed order (not in bias's place: later kernels read that); its columns >= N are left as they were.  o is not needed.  workspace: savit_bias_attention_bwd_workspace_bytes(.., dbias != NULL), 16-byte aligned.
  *   head_dim 16, 32, 48 or 64; N <= 32 768, and one image's rows and one head's bias each below 4 GiB; d_o, o compact [B*N, H*head_dim]. */
 int savit_bias_attention_fwd(const void* qkv, const float* bias, const int* lens, void* o, float* lse, int B, int N, int H, int head_dim, int ld_qkv,
                              int ld_bias, void* stream);

@@ -58,8 +58,8 @@ struct BiasAttnParams {
   const bf16_t* d_o;
   bf16_t* dqkv;
   float* stat;         // backward: [B, H, 3, Np]: P = exp2((s - first) log2 e - second); the first is inf where the query takes no part; delta
-  float* dbias;        // [H, N, ldb], or the slab [parts][H, N, ldb]
-  int B, N, H, ld, d, ldb, Np;
+  float* dbias;        // [H, N, lddb], or the slab [parts][H, N, lddb]
+  int B, N, H, ld, d, ldb, lddb, Np;
   int hd;
   int blocks;          // query (key) blocks of a sequence
   int key_blocks, parts;
@@ -748,6 +748,17 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   }
 }
 
+// columns col .. col + 3 of a bias gradient's row; what lies behind column N is the caller's
+__device__ __forceinline__ void store_columns(float* row, int col, int N, f32x4 v) {
+  if (col + 4 <= N) {
+    *reinterpret_cast<f32x4*>(row + col) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (col + i < N) row[col + i] = v[i];
+  }
+}
+
 // dbias of a tile of 32 W queries x SEG keys of one head, summed over the images of a part
 template <int KS>
 __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnParams p) {
@@ -835,13 +846,12 @@ __global__ __launch_bounds__(256, 2) void bias_attn_db_kernel(const BiasAttnPara
     }
   }
   if (q < p.N) {
-    float* out = p.dbias + (((size_t)part * p.H + h) * p.N + q) * p.ldb + k0 + 4 * L.half;
+    float* out = p.dbias + (((size_t)part * p.H + h) * p.N + q) * p.lddb;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (k0 + 32 * t + 8 * g + 4 * L.half < p.N)
-          *reinterpret_cast<float4*>(out + 32 * t + 8 * g) = make_float4(acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]);
+        store_columns(out, k0 + 32 * t + 8 * g + 4 * L.half, p.N, f32x4{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]});
   }
 }
 
@@ -1051,16 +1061,15 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
   }
   if constexpr (DB) {
     if (q < p.N) {
-      float* out = p.dbias + (((size_t)part * p.H + h) * p.N + q) * p.ldb + 4 * g;
+      float* out = p.dbias + (((size_t)part * p.H + h) * p.N + q) * p.lddb;
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
-        if (16 * t + 4 * g < p.N) *reinterpret_cast<f32x4*>(out + 16 * t) = acc[t];
+      for (int t = 0; t < KT; ++t) store_columns(out, 16 * t + 4 * g, p.N, acc[t]);
     }
   }
 }
 
-// out = sum of the parts: 16 16-byte columns a block, 16 strips of parts, fixed order
-__global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __restrict__ slab, float* __restrict__ out, long n4, int parts) {
+// out = sum of the parts (rows of quads 16-byte columns; out's are ld elements apart): 16 columns a block, 16 strips of parts, fixed order
+__global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __restrict__ slab, float* __restrict__ out, long n4, int parts, int N, int quads, int ld) {
   __shared__ f32x4 red[16][16];
   const int c = threadIdx.x & 15, strip = threadIdx.x >> 4;
   const long i = (long)blockIdx.x * 16 + c;
@@ -1074,11 +1083,13 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
   if (strip == 0 && i < n4) {
 #pragma unroll
     for (int k = 1; k < 16; ++k) s += red[k][c];
-    reinterpret_cast<f32x4*>(out)[i] = s;
+    const long row = i / quads;
+    store_columns(out + (size_t)row * ld, (int)(i - row * quads) * 4, N, s);
   }
 }
 
 int padded(int N) { return (N + 63) / 64 * 64; }
+int quads_of(int N) { return (N + 3) / 4; }  // of a row of the slab
 
 // Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 173 us against 265 of the
 // streaming kernels at [128 x 12 x 197], 60 / 110 at [2048 x 4 x 49], 80 / 117 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 163 /
@@ -1209,7 +1220,7 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
 extern "C" long savit_bias_attention_bwd_workspace_bytes(int B, int N, int H, int ld_bias, int want_dbias) {
   if (!(B >= 0 && N > 0 && N <= 32768 && H > 0 && ld_bias >= N)) return 0;
   const int parts = dbias_parts(B, N, H);
-  return (long)B * H * 3 * padded(N) * 4 + (want_dbias && parts > 1 ? (long)parts * H * N * ld_bias * 4 : 0);
+  return (long)B * H * 3 * padded(N) * 4 + (want_dbias && parts > 1 ? (long)parts * H * N * quads_of(N) * 16 : 0);
 }
 
 extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, const int* lens, const void* d_o, const float* lse, void* dqkv, float* dbias, int B,
@@ -1230,6 +1241,7 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   float* slab = parts == 1 ? dbias : p.stat + (size_t)B * H * 3 * p.Np;
   p.parts = parts;
   p.dbias = slab;
+  p.lddb = parts == 1 ? ld_bias : 4 * quads_of(N);
   if (resident(N)) {
     p.blocks = resident_blocks(N);
     const int rr = launch_resident(p, dbias != nullptr, st);
@@ -1249,8 +1261,8 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
       BIAS_ATTN_LAUNCH(bias_attn_db_kernel, grid);
     }
     if (p.parts > 1) {
-      const long n4 = (long)H * N * ld_bias / 4;
-      hipLaunchKernelGGL(bias_attn_parts_kernel, dim3((unsigned)((n4 + 15) / 16)), dim3(256), 0, st, slab, dbias, n4, p.parts);
+      const long n4 = (long)H * N * quads_of(N);
+      hipLaunchKernelGGL(bias_attn_parts_kernel, dim3((unsigned)((n4 + 15) / 16)), dim3(256), 0, st, slab, dbias, n4, p.parts, N, quads_of(N), ld_bias);
       SAVIT_LAUNCH_RET();
     }
   }

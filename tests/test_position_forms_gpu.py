@@ -66,6 +66,20 @@ def test_bias_attention_wide_forward(ops, B, N, H, hd, form):  # noqa: F811
     check_attention(ops, qkv, bias, lens, B, N, H, hd, d_o, 1.0)
 
 
+@pytest.mark.parametrize("B,N,H,hd", [(1, 17, 2, 32), (300, 49, 4, 32), (2, 197, 3, 64), (45, 197, 6, 64), (3, 300, 2, 64), (25, 300, 6, 48), (1, 1, 1, 16)])
+def test_bias_gradient_leaves_what_lies_behind_its_columns(ops, B, N, H, hd):  # noqa: F811
+    """A gradient that is a part of a wider buffer: the columns beside it keep what they hold."""
+    g, qkv, narrow, d_o = attention_inputs(ops, B, N, H, hd, N)
+    ld = (N + 3) // 4 * 4 + 12
+    bias = torch.full((H, N, ld), math.nan, device="cuda")[:, :, :N]
+    bias.copy_(narrow)
+    _, lse = ops.bias_attention_fwd(qkv, bias, B, N, H, head_dim=hd)
+    buf = torch.full((H, N, ld), 7.0, device="cuda")
+    _, db = ops.bias_attention_bwd(qkv, bias, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd, dbias=buf[:, :, :N])
+    _, want = ops.bias_attention_bwd(qkv, narrow, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd)
+    assert torch.equal(db, want) and bool((buf[:, :, N:] == 7.0).all())
+
+
 # --------------------------------------------------------------------------------------------- query / key norm
 # enough rows that a group of lanes takes four heads in bf16 and two in fp32; numbers of heads that leave a last group fewer
 MANY = [(24001, 5, 3, 64), (11000, 7, 1, 256), (33000, 6, 2, 48), (66001, 9, 9, 16)]
