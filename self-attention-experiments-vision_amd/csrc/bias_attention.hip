@@ -11,13 +11,15 @@
 // in-register reductions plus an exchange between the lanes of a query, and the score tile is the next product's operand without an LDS round trip.
 // The bias tile is fetched one tile ahead and is the INITIAL value of the score accumulators: adding it costs nothing.  W = 1, 2 or 4 by the sequence
 // length, so that short sequences leave no wave idle.
-// Rounded to bf16: P and dS as operands of the matrix instructions, beyond 32 tokens (O, dQ, dK, dV are bf16 themselves: the error is sqrt 2 of theirs; P stays below 2^8 and is divided by its fp32 sum at
-// the end), O and the gradients when stored.  Scores, statistics, delta, sums and dbias are fp32.
+// P and dS enter the matrix instructions as two bf16 numbers, the second what the first one's rounding took off (2^-16 of them is lost), in a product of its
+// own: O and the gradients are rounded once, when stored, and are as near to 64 bits as an fp32 form's (0.0017 of their norm; with one number 0.0024).  It
+// costs a tenth: [128 x 12 x 197] forward and backward 250 -> 273 us, [2048 x 4 x 49] 98 -> 107, [16 x 16 x 577] forward 66 -> 76.  Scores, statistics,
+// delta, sums and dbias are fp32.
 //
-// What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (55 measured) and 55 backward (99 dQ and dbias, 94 dK and dV), the
-// products 13 and 31: with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
-// goes into (dK / dV: vector issue 39 %, LDS 27 %, matrix pipe 17 % busy).  One segment or long rows come nearer: [2048 x 4 x 49], heads of 32,
-// 25 us forward (bytes 21), 28 dK and dV (31 from memory; some of it is still in the caches), 32 dQ and dbias.
+// What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (59 measured) and 55 backward (107 dQ and dbias, 104 dK and dV), the
+// products 19 and 44: with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
+// goes into.  One segment or long rows come nearer: [2048 x 4 x 49], heads of 32, 26 us forward (bytes 21), 33 dK and dV (31 from memory; some of it is
+// still in the caches), 37 dQ and dbias.
 //
 // delta is summed from the fp32 probabilities, in a loop of its own over the keys, not taken as rowsum(dO . O): O is rounded to bf16, and the table
 // gradient that dS feeds is an fp32 parameter gradient (2^-9 of O in delta is 1e-4 of the gradient; this way it is 1e-6).
@@ -159,18 +161,31 @@ __device__ __forceinline__ void tile_product(f32x16& s, const char* img, int row
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag(img, row, 2 * ks + half), f[ks], s, 0, 0, 0);
 }
-// out^T[e][lane] += sum over the tile's 32 rows of image[row][e] * a[row][lane]
-template <int KS>
+// what the rounding of (a, b) to the bf16 pair u took off, as another pair: the operand of a second product
+__device__ __forceinline__ uint32_t low_parts(uint32_t u, float a, float b) {
+  return pack_bf16x2(a - __builtin_bit_cast(float, u << 16), b - __builtin_bit_cast(float, u & 0xffff0000u));
+}
+// out^T[e][lane] += sum over the tile's 32 rows of image[row][e] * a[row][lane], a as two bf16 (heads of 48 and 64)
 __device__ __forceinline__ void tile_accumulate(f32x16 (&out)[2], const char* img, int row0, const f32x16& a, const Lane& L) {
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
-    const bf16x8 af = acc_to_frag(a, s2);
+    union { uint32_t u[4]; bf16x8 v; } hi, lo;
 #pragma unroll
-    for (int eb = 0; eb < (KS > 2 ? 2 : 1); ++eb) {
-      const int row = row0 + 16 * s2 + L.trow, col = 32 * eb + L.tcol;
-      const bf16x8 vf = __builtin_shufflevector(read_tr(img, row, col), read_tr(img, row + 8, col), 0, 1, 2, 3, 4, 5, 6, 7);
-      out[eb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, af, out[eb], 0, 0, 0);
+    for (int j = 0; j < 4; ++j) {
+      const float x = a[8 * s2 + 2 * j], y = a[8 * s2 + 2 * j + 1];
+      hi.u[j] = pack_bf16x2(x, y);
+      lo.u[j] = low_parts(hi.u[j], x, y);
     }
+    bf16x8 vf[2];
+#pragma unroll
+    for (int eb = 0; eb < 2; ++eb) {
+      const int row = row0 + 16 * s2 + L.trow, col = 32 * eb + L.tcol;
+      vf[eb] = __builtin_shufflevector(read_tr(img, row, col), read_tr(img, row + 8, col), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int eb = 0; eb < 2; ++eb) out[eb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[eb], hi.v, out[eb], 0, 0, 0);
+#pragma unroll
+    for (int eb = 0; eb < 2; ++eb) out[eb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[eb], lo.v, out[eb], 0, 0, 0);
   }
 }
 __device__ __forceinline__ f32x16 zero16() {
@@ -193,12 +208,6 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __
 __device__ __forceinline__ bf16x8 lds_tr_pair(const char* img, int row, int col) {
   const bf16x4 lo = read_tr(img, row, col), hi = read_tr(img + 16 * ROWB, row, col);  // (16 rows on: the same swizzle)
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-// what the rounding of (a, b) to the bf16 pair u took off, as another pair: the operand of a second product
-// (Up to 32 tokens, where a few probabilities make a whole row and their roundings do not average out; there it costs 0 to 3 %, at 49 tokens and heads of 32
-// 9 %, and the longer the row the more.)
-__device__ __forceinline__ uint32_t low_parts(uint32_t u, float a, float b) {
-  return pack_bf16x2(a - __builtin_bit_cast(float, u << 16), b - __builtin_bit_cast(float, u & 0xffff0000u));
 }
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float quarters_sum(float v) {
@@ -348,7 +357,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_fwd_kernel(const BiasAttnPar
           sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], LOG2E_F, -ref));
           l += sc[r];
         }
-        tile_accumulate<KS>(oacc, imgV, 32 * t, sc, L);
+        tile_accumulate(oacc, imgV, 32 * t, sc, L);
       }
       if constexpr (more) {
         sg.put(smem + ((s + 1) & 1) * 2 * Seg::IMG);
@@ -456,17 +465,15 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 4 : 3) void bias_attn_fwd16_kernel
           }
           pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
           pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
-          if constexpr (W <= 2) {
-            pl.u[2 * k] = low_parts(pf.u[2 * k], x[0], x[1]);
-            pl.u[2 * k + 1] = low_parts(pf.u[2 * k + 1], x[2], x[3]);
-          }
+          pl.u[2 * k] = low_parts(pf.u[2 * k], x[0], x[1]);
+          pl.u[2 * k + 1] = low_parts(pf.u[2 * k + 1], x[2], x[3]);
           if constexpr (!ONE) x = load4f(rb, boff + (uint32_t)(k0 + Seg::SEG + 16 * (t + k)) * 4);
         }
 #pragma unroll
         for (int eb = 0; eb < 2 * KS2; ++eb) {
           const bf16x8 vf = lds_tr_pair(imgV, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
           o[eb] = mfma16(vf, pf.v, o[eb]);
-          if constexpr (W <= 2) o[eb] = mfma16(vf, pl.v, o[eb]);
+          o[eb] = mfma16(vf, pl.v, o[eb]);
         }
       }
       if (!ONE && s + 1 < nseg) {
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
         }
 #pragma unroll
         for (int t = 0; t < T; t += 2) {
-          union { uint32_t u[4]; bf16x8 v; } pf;
+          union { uint32_t u[4]; bf16x8 v; } pf, pl;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             f32x4& x = sc[t + k];
@@ -572,6 +579,8 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
               x = x * (dp[t + k] - delta);
               pf.u[2 * k] = pack_bf16x2(x[0], x[1]);
               pf.u[2 * k + 1] = pack_bf16x2(x[2], x[3]);
+              pl.u[2 * k] = low_parts(pf.u[2 * k], x[0], x[1]);
+              pl.u[2 * k + 1] = low_parts(pf.u[2 * k + 1], x[2], x[3]);
             } else {
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
@@ -583,7 +592,11 @@ __global__ __launch_bounds__(256, 3) void bias_attn_dq_kernel(const BiasAttnPara
           }
           if constexpr (second) {
 #pragma unroll
-            for (int eb = 0; eb < 2 * KS2; ++eb) dq[eb] = mfma16(lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3)), pf.v, dq[eb]);
+            for (int eb = 0; eb < 2 * KS2; ++eb) {
+              const bf16x8 kf = lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+              dq[eb] = mfma16(kf, pf.v, dq[eb]);
+              dq[eb] = mfma16(kf, pl.v, dq[eb]);
+            }
           }
         }
         if (more) {
@@ -708,22 +721,20 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
             pf.u[2 * k + 1] = pack_bf16x2(pr[2], pr[3]);
             df.u[2 * k] = pack_bf16x2(dp[0], dp[1]);
             df.u[2 * k + 1] = pack_bf16x2(dp[2], dp[3]);
-            if constexpr (W <= 2) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                pl.u[2 * k + i] = low_parts(pf.u[2 * k + i], pr[2 * i], pr[2 * i + 1]);
-                sl.u[2 * k + i] = low_parts(df.u[2 * k + i], dp[2 * i], dp[2 * i + 1]);
-              }
+            for (int i = 0; i < 2; ++i) {
+              pl.u[2 * k + i] = low_parts(pf.u[2 * k + i], pr[2 * i], pr[2 * i + 1]);
+              sl.u[2 * k + i] = low_parts(df.u[2 * k + i], dp[2 * i], dp[2 * i + 1]);
             }
           }
 #pragma unroll
           for (int eb = 0; eb < 2 * KS2; ++eb) {
             const bf16x8 gf = lds_tr_pair(imgD, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
-            dv[eb] = mfma16(gf, pf.v, dv[eb]);
-            if constexpr (W <= 2) dv[eb] = mfma16(gf, pl.v, dv[eb]);
             const bf16x8 qf = lds_tr_pair(imgQ, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
+            dv[eb] = mfma16(gf, pf.v, dv[eb]);
             dk[eb] = mfma16(qf, df.v, dk[eb]);
-            if constexpr (W <= 2) dk[eb] = mfma16(qf, sl.v, dk[eb]);
+            dv[eb] = mfma16(gf, pl.v, dv[eb]);
+            dk[eb] = mfma16(qf, sl.v, dk[eb]);
           }
         }
         if constexpr (!ONE) {
@@ -1012,7 +1023,7 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if (t + k == KT) {
-          f.u[2] = f.u[3] = 0;
+          f.u[2] = f.u[3] = fl.u[2] = fl.u[3] = 0;
           break;
         }
 #pragma unroll
@@ -1022,16 +1033,14 @@ __global__ __launch_bounds__(512, 2) void bias_attn_dq_resident_kernel(const Bia
         }
         f.u[2 * k] = pack_bf16x2(sc[t + k][0], sc[t + k][1]);
         f.u[2 * k + 1] = pack_bf16x2(sc[t + k][2], sc[t + k][3]);
-        if constexpr (KT == 2) {
-          fl.u[2 * k] = low_parts(f.u[2 * k], sc[t + k][0], sc[t + k][1]);
-          fl.u[2 * k + 1] = low_parts(f.u[2 * k + 1], sc[t + k][2], sc[t + k][3]);
-        }
+        fl.u[2 * k] = low_parts(f.u[2 * k], sc[t + k][0], sc[t + k][1]);
+        fl.u[2 * k + 1] = low_parts(f.u[2 * k + 1], sc[t + k][2], sc[t + k][3]);
       }
 #pragma unroll
       for (int eb = 0; eb < 2 * KS2; ++eb) {
         const bf16x8 kf = lds_tr_pair(imgK, 16 * t + 4 * g + (ql >> 2), 16 * eb + 4 * (ql & 3));
         dq[eb] = mfma16(kf, f.v, dq[eb]);
-        if constexpr (KT == 2) dq[eb] = mfma16(kf, fl.v, dq[eb]);
+        dq[eb] = mfma16(kf, fl.v, dq[eb]);
       }
       if constexpr (RES_GROUPS == 4) {
         if (t == KE / 6 * 2) { put(1, buf ^ 1); fetch(rn, 2); }
@@ -1091,9 +1100,9 @@ __global__ __launch_bounds__(256) void bias_attn_parts_kernel(const float* __res
 int padded(int N) { return (N + 63) / 64 * 64; }
 int quads_of(int N) { return (N + 3) / 4; }  // of a row of the slab
 
-// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 173 us against 265 of the
-// streaming kernels at [128 x 12 x 197], 60 / 110 at [2048 x 4 x 49], 80 / 117 at [64 x 8 x 224], 25 / 27 at [2 x 12 x 197]; without a bias gradient 163 /
-// 192, 56 / 70, 65 / 79, 17 / 17.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
+// Up to 224 tokens the keys of an (image, head) are resident and the bias gradient is part of the dQ kernel: the backward takes 213 us against 302 of the
+// streaming kernels at [128 x 12 x 197], 71 / 120 at [2048 x 4 x 49], 87 / 125 at [64 x 8 x 224], 27 / 31 at [2 x 12 x 197]; without a bias gradient 188 /
+// 221, 66 / 80, 74 / 88, 20 / 19.  (Beyond, the registers of a wave do not hold a row's P, dP and dS sum.)
 constexpr int RESIDENT_N = 224;
 bool resident(int N) { return N <= RESIDENT_N; }
 constexpr int CUS = 256;  // not the device's or a budget's: the parts set the order of the bias gradient's sum
@@ -1106,7 +1115,7 @@ int resident_waves(int N) {
 }
 int resident_blocks(int N) { return (N + 15) / 16 > 8 ? 2 : 1; }
 // parts of the batch, a workgroup each: the persistent kernel's fill the chip once with 8 waves a CU (160 KB of LDS a CU; 12 and 16 waves, more than fit at once,
-// take 205 and 231 us against 200 at [1024 x 12 x 49], heads of 64) ...
+// take 215 and 216 us against 208 at [1024 x 12 x 49], heads of 64) ...
 int resident_parts(int B, int N, int H) {
   const int kt = (N + 31) / 32 * 2, W = resident_waves(N);
   int per_cu = 8 / W;
@@ -1122,8 +1131,8 @@ int dbias_parts(int B, int N, int H) { return resident(N) ? resident_parts(B, N,
 
 // All heads of an image in a row where their biases fit an XCD's L2 (4 MB) beside the rows: half of it where heads end inside a cache line of a row, a
 // quarter where they are whole lines and less is won.  Against all images of a head in a row, forward and backward: [2048 x 4 x 49], heads of 32,
-// 23 and 60 us against 27 and 80; [128 x 12 x 197], heads of 48 (1.9 MB), forward 48 / 56; heads of 64: [1024 x 8 x 128] forward 152 / 162, [1024 x 8 x 64]
-// backward 181 / 187, but [128 x 12 x 197] (1.9 MB) forward 54.5 / 51.7 and [16 x 16 x 577] (21 MB) 78 / 51
+// 25 and 71 us against 27.5 and 82; [128 x 12 x 197], heads of 48 (1.9 MB), forward 55 / 58; heads of 64: [1024 x 8 x 128] forward 149 / 162, [1024 x 8 x 64]
+// backward 184 / 192, but [128 x 12 x 197] (1.9 MB) forward 63.3 / 62.3 and [16 x 16 x 577] (21 MB) 80 / 59
 bool many_heads(int N, int H, int hd, int ldb) { return (long)H * N * ldb * 4 <= (hd == 64 ? 1L << 20 : 2L << 20); }
 
 bool size_ok(int B, int N, int H, int hd, int ld, int ldb) {
@@ -1161,7 +1170,7 @@ int launch_resident_kt(const BiasAttnParams& p, bool db, hipStream_t st) {
   return db ? launch_resident_k<KT, 2, true>(p, st) : launch_resident_k<KT, 2, false>(p, st);
 }
 int launch_resident(const BiasAttnParams& p, bool db, hipStream_t st) {
-  const int nq = (p.N + 15) / 16;  // rounded to an even number up to eight; beyond, a tile less is 12 registers less, where they are all in use (197 tokens: 119 us with 14, 99 with 13)
+  const int nq = (p.N + 15) / 16;  // rounded to an even number up to eight; beyond, a tile less is 12 registers less, where they are all in use (197 tokens: 110 us with 14, 107 with 13)
   switch (nq) {
     case 1: case 2: return launch_resident_kt<2>(p, db, st);
     case 3: case 4: return launch_resident_kt<4>(p, db, st);
@@ -1196,8 +1205,8 @@ int launch_sixteen(const BiasAttnParams& p, A one_wave, B two, C segment, D many
               : launch_sixteen(p, K<1, 2, true>, K<2, 2, true>, K<4, 2, true>, K<4, 2, false>, st))
 int launch_fwd(BiasAttnParams p, hipStream_t st) {
   // 32 queries a wave where heads are wide, sequences long and the grid is two workgroups a CU or more, else 16 (heads of 64; 32 against 16 a wave:
-  // [128 x 12 x 197] 52 against 66 us, [32 x 12 x 197] 17.4 / 20.3, [16 x 12 x 197] 11.7 / 11.4, [8 x 16 x 577] 32 / 33, [4 x 16 x 577] 22.9 / 21.2,
-  // [8 x 8 x 1500] 80 / 94, [1 x 8 x 1500] 32 / 24.5; up to 64 tokens one segment is all there is and 16 are never slower)
+  // [128 x 12 x 197] 63 against 75 us, [32 x 12 x 197] 20 / 23, [16 x 12 x 197] 14.0 / 13.4, [8 x 16 x 577] 38 / 37, [4 x 16 x 577] 27.5 / 24,
+  // [8 x 8 x 1500] 90 / 98, [1 x 8 x 1500] 40 / 28; up to 64 tokens one segment is all there is and 16 are never slower)
   if (p.N > 64 && p.hd > 32 && (long)p.B * p.H * ((p.N + 127) / 128) >= 2L * CUS)
     return p.hd == 48 ? launch_waves(p, 4, 32, bias_attn_fwd_kernel<3>, st) : launch_waves(p, 4, 32, bias_attn_fwd_kernel<4>, st);
   return BIAS_ATTN_SIXTEEN(bias_attn_fwd16_kernel);
