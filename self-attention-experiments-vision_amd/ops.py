@@ -1059,7 +1059,8 @@ def relpos_bias_empty(H: int, N: int, device="cuda") -> torch.Tensor:
 
 
 def relpos_bias_fwd(table: torch.Tensor, index: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """bias[h, i, j] = table[index[i, j], h]: table fp32 [buckets, H], index int32 [N, N] -> fp32 [H, N, N] (relpos_bias_empty).  savit_relpos_bias_fwd."""
+    """bias[h, i, j] = table[index[i, j], h]: table fp32 [buckets, H], index int32 [N, N] -> fp32 [H, N, N] (relpos_bias_empty; what pads its rows is zeroed).
+    savit_relpos_bias_fwd."""
     dev = _dev(table)
     _chk(table, f32, "table", 2)
     nb, H = table.shape
@@ -1125,8 +1126,8 @@ def bias_attention_fwd(qkv: torch.Tensor, bias: torch.Tensor, B: int, N: int, H:
 def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor, lse: torch.Tensor, B: int, N: int, H: int, dq_scale: float,
                        head_dim: int = 64, lens: Optional[torch.Tensor] = None, dqkv: Optional[torch.Tensor] = None,
                        dbias: Optional[torch.Tensor] = None, want_dbias: bool = True, workspace: Optional[torch.Tensor] = None):
-    """Backward of bias_attention_fwd.  Returns (dqkv bf16 with qkv's row pitch, dbias fp32 [H, N, N] = the bias gradient summed over the batch, or None
-    with want_dbias=False).  savit_bias_attention_bwd."""
+    """Backward of bias_attention_fwd.  Returns (dqkv bf16 [B*N, 3*H*head_dim] with qkv's row pitch, dbias fp32 [H, N, N] = the bias gradient summed over
+    the batch, or None with want_dbias=False).  savit_bias_attention_bwd."""
     dev = _dev(qkv)
     d = H * head_dim
     ld = _packed(qkv, bf16, B * N, 3 * d, "qkv", dev)
@@ -1137,6 +1138,8 @@ def bias_attention_bwd(qkv: torch.Tensor, bias: torch.Tensor, d_o: torch.Tensor,
         _whole(lens, torch.int32, (B,), "lens", dev)
     if dqkv is None:
         dqkv = qkv.new_empty((B * N, ld))
+        if ld != 3 * d:  # (what pads the rows is not written)
+            dqkv = dqkv[:, : 3 * d]
     elif _packed(dqkv, bf16, B * N, 3 * d, "dqkv", dev) != ld and B * N > 1:
         raise ValueError("dqkv must have qkv's row stride")
     if not want_dbias:

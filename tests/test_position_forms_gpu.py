@@ -80,6 +80,20 @@ def test_bias_gradient_leaves_what_lies_behind_its_columns(ops, B, N, H, hd):  #
     assert torch.equal(db, want) and bool((buf[:, :, N:] == 7.0).all())
 
 
+@pytest.mark.parametrize("N", [20, 300])
+def test_bias_attention_gradient_of_wide_rows(ops, N):  # noqa: F811
+    """Rows with columns beside the packed ones: the gradient has those of the packed ones, at the same pitch."""
+    B, H, hd = 2, 2, 32
+    g, qkv, bias, d_o = attention_inputs(ops, B, N, H, hd, N)
+    wide = torch.full((B * N, 3 * H * hd + 24), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, : 3 * H * hd] = qkv
+    _, lse = ops.bias_attention_fwd(wide, bias, B, N, H, head_dim=hd)
+    dqkv, db = ops.bias_attention_bwd(wide, bias, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd)
+    assert dqkv.shape == qkv.shape and dqkv.stride(0) == wide.stride(0)
+    want, wb = ops.bias_attention_bwd(qkv, bias, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd)
+    assert torch.equal(dqkv, want) and torch.equal(db, wb)
+
+
 # --------------------------------------------------------------------------------------------- query / key norm
 # enough rows that a group of lanes takes four heads in bf16 and two in fp32; numbers of heads that leave a last group fewer
 MANY = [(24001, 5, 3, 64), (11000, 7, 1, 256), (33000, 6, 2, 48), (66001, 9, 9, 16)]
