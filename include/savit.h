@@ -534,7 +534,8 @@ int savit_spin(long microseconds, void* stream);
 int savit_hold_cus(int cus, long microseconds, void* stream);
 /* CUs the persistent kernels (attention forward / backward: one workgroup per CU walking over (image, head) items) size their grids
  * for; 0 (default) = every CU of the device.  A data-parallel rank sets its launch plan's budget (device CUs - reserved_cus) so that no
- * persistent workgroup has to wait for a CU that RCCL's channels hold.  Process-wide; results do not depend on it. */
+ * persistent workgroup has to wait for a CU that RCCL's channels hold.  Process-wide; results do not depend on it.  (savit_bias_attention_bwd keeps its
+ * grid: its workgroups are the parts that the bias gradient is summed from, in an order that has to stay.) */
 int savit_set_cu_budget(int cus);
 int savit_zero_bytes(void* dst, long bytes, void* stream);
 
