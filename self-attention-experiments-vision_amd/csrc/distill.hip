@@ -386,13 +386,16 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W, OCC) void distill_kernel(cons
       double all = 0.0, others = 0.0;
       xsum = 0.0;
 #pragma unroll 1
-      for (int j = tid; j < p.C; j += TH) {
-        const float v = to_float(z[j]);
-        if (v <= LOW) {
-          all += (double)v;
-          if (!is_named(j)) others += (double)v;
-        } else {
-          xsum += (double)v * p.c_soft;
+      for (int i = tid; i < pieces; i += TH) {  // a thread its own pieces: nobody else writes a gradient in their place
+#pragma unroll 1
+        for (int j = i * E; j < (i + 1) * E && j < p.C; ++j) {
+          const float v = to_float(z[j]);
+          if (v <= LOW) {
+            all += (double)v;
+            if (!is_named(j)) others += (double)v;
+          } else {
+            xsum += (double)v * p.c_soft;
+          }
         }
       }
       xsum = wave_sum_d(xsum);

@@ -431,3 +431,16 @@ def test_distill_masked_classes_with_the_rest(ops, C, masked):
     else:
         share = ((1 - (top[:, 4:24].double() - lse.double()[:, None]).exp().sum(1)) / (C - 24))
         assert bool(((loss.double() / (share * -masked) - 1).abs() < 1e-4).all()), (loss, share)  # (lse's own rounding, 2^-22 of exp, is in share too)
+
+
+@pytest.mark.parametrize("C,dtype", [(1003, torch.float32), (30011, torch.float32), (140003, torch.bfloat16)])
+def test_distill_masked_classes_in_place(ops, C, dtype):
+    """Rows with masked classes are summed a second time: before any of their logits is replaced by its gradient."""
+    z, top, at, lse, labels = make(32, C, 8, C, dtype, lse=True)
+    z[:, 3::7] = torch.finfo(torch.float32).min if dtype == torch.float32 else -1e30
+    kw = dict(teacher_lse=lse, labels=labels, hard_weight=0.5, distill_weight=0.5, label_smoothing=0.1)
+    dz = torch.empty_like(z)
+    loss = ops.distill_xent(z, top, at, dlogits=dz, **kw)
+    for _ in range(5):
+        place = z.clone()
+        assert torch.equal(ops.distill_xent(place, top, at, dlogits=place, **kw), loss) and torch.equal(place, dz)
