@@ -258,6 +258,7 @@ int savit_attention_bwd(const void* qkv, const void* o, const void* d_o, const f
                         int head_dim, int ld_qkv, float dq_scale, void* stream);
 
 /* ---- Position in attention: per-head normalisation with the rotation, and learned relative biases.
+ * Outputs share no memory with what a call reads, but where it says so (SAVIT_EINVAL; column ranges of one buffer do not).
  * savit_qk_norm_rope_fwd: rows of the packed buffer (H query heads, Hk key heads, Hk value heads of head_dim columns; Hk < H: shared key /
  *   value heads), bf16 (is_bf16) or fp32, row pitches ld / ld_out in elements (16-byte multiples, 16-byte aligned bases).  Per head of the
  *   queries and keys:  n = (x - center * mean x) / sqrt(mean (x - center * mean x)^2 + eps);  out = s * rotate(w * n), s = q_scale for queries
@@ -401,7 +402,7 @@ int savit_softmax_xent(const float* logits, int ld_logits, const int* labels, co
  *   loss = row_weight (distill_weight T^2 sum_j P_j (log P_j - log q_j) + hard_weight CE(logits, smoothed label))
  *   dlogits = grad_scale * d loss / d logits
  * logits fp32 or bf16 [R, ld], dlogits (nullable) fp32 or bf16 [R, ld_dlogits] - columns >= C are left alone; dlogits == logits is allowed with
- * equal type and pitch; any alignment of the element type.  teacher_logits fp32, teacher_index int32, both [R, K] compact, K <= 512: an index
+ * equal type and pitch, any other overlap is SAVIT_EINVAL; any alignment of the element type.  teacher_logits fp32, teacher_index int32, both [R, K] compact, K <= 512: an index
  * outside [0, C) is no pair, one class named twice gets both probabilities; a row without pairs has no distillation term, or, with teacher_lse, the
  * uniform distribution as its target (all of the mass is left).  temperature in [1e-30, 1e30].  labels int32 [R]
  * (nullable when hard_weight == 0): outside [0, C) drops the row's hard term.  row_weight fp32 [R] (nullable = 1): rows of weight 0 are not read,

@@ -1219,6 +1219,8 @@ extern "C" int savit_bias_attention_fwd(const void* qkv, const float* bias, cons
                                         int ld_bias, void* stream) {
   SAVIT_CHECK_ARG(qkv && bias && o && lse && size_ok(B, N, H, head_dim, ld_qkv, ld_bias) && o != qkv && aligned16(qkv) && aligned16(bias) && aligned16(o));
   if (B == 0) return SAVIT_OK;
+  const long d = (long)H * head_dim, rows = (long)B * N;
+  SAVIT_CHECK_ARG(!savit_rows_overlap(o, 2 * d, 2 * d, qkv, 2L * ld_qkv, 6 * d, rows));
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.o = (bf16_t*)o; p.lse = lse;
   p.B = B; p.N = N; p.H = H; p.ld = ld_qkv; p.d = H * head_dim; p.hd = head_dim; p.ldb = ld_bias;
@@ -1239,6 +1241,9 @@ extern "C" int savit_bias_attention_bwd(const void* qkv, const float* bias, cons
   SAVIT_CHECK_ARG(aligned16(qkv) && aligned16(bias) && aligned16(d_o) && aligned16(dqkv) && aligned16(dbias));
   const hipStream_t st = (hipStream_t)stream;
   if (B == 0) return dbias ? (int)SAVIT_EINVAL : SAVIT_OK;  // no image: there is no gradient to write
+  const long d = (long)H * head_dim, rows = (long)B * N;  // later kernels read what the first ones would have overwritten
+  SAVIT_CHECK_ARG(!savit_rows_overlap(dqkv, 2L * ld_qkv, 6 * d, qkv, 2L * ld_qkv, 6 * d, rows) && !savit_rows_overlap(dqkv, 2L * ld_qkv, 6 * d, d_o, 2 * d, 2 * d, rows));
+  SAVIT_CHECK_ARG(!savit_rows_overlap(dbias, 4L * ld_bias, 4L * N, bias, 4L * ld_bias, 4L * N, (long)H * N));
   SAVIT_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= savit_bias_attention_bwd_workspace_bytes(B, N, H, ld_bias, dbias != nullptr));
   BiasAttnParams p{};
   p.qkv = (const bf16_t*)qkv; p.bias = bias; p.lens = lens; p.d_o = (const bf16_t*)d_o; p.lse = const_cast<float*>(lse); p.dqkv = (bf16_t*)dqkv;

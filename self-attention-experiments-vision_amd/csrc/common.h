@@ -41,6 +41,15 @@ __device__ __forceinline__ void nt_store_u4(void* p, uint4 v) {
     if (!(cond)) return SAVIT_EINVAL; \
   } while (0)
 
+// Whether two operands of as many rows share memory: wa bytes every lda from a, wb bytes every ldb from b (column ranges of one buffer do not)
+inline bool savit_rows_overlap(const void* a, long lda, long wa, const void* b, long ldb, long wb, long rows) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b, a1 = a0 + (rows - 1) * lda + wa, b1 = b0 + (rows - 1) * ldb + wb;
+  if (!a || !b || rows <= 0 || a1 <= b0 || b1 <= a0) return false;
+  if (lda != ldb || rows == 1) return true;
+  const long d = b0 >= a0 ? (long)((b0 - a0) % lda) : (lda - (long)((a0 - b0) % lda)) % lda;
+  return d < wa || d + wb > lda;
+}
+
 #define SAVIT_LAUNCH_RET() return (int)hipGetLastError()
 
 // CUs the persistent kernels (one workgroup per CU walking over work items: attention forward / backward) may count on; 0 = all.

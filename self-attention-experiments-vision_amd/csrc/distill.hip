@@ -624,7 +624,9 @@ extern "C" int savit_distill_xent(const void* logits, long ld_logits, int logits
   SAVIT_CHECK_ARG(temperature >= 1e-30f && temperature <= 1e30f && (hard_weight == 0.f || labels) && label_smoothing >= 0.f && label_smoothing <= 1.f);
   SAVIT_CHECK_ARG((dlogits || loss_rows) && (!dlogits || ld_dlogits >= C) && (!dbias || dlogits));
   SAVIT_CHECK_ARG(((uintptr_t)logits % (logits_bf16 ? 2 : 4)) == 0 && ((uintptr_t)dlogits % (dlogits_bf16 ? 2 : 4)) == 0);
-  SAVIT_CHECK_ARG(dlogits != logits || (logits_bf16 == dlogits_bf16 && ld_logits == ld_dlogits));
+  const long zs = logits_bf16 ? 2 : 4, ds = dlogits_bf16 ? 2 : 4;
+  SAVIT_CHECK_ARG(dlogits == logits ? logits_bf16 == dlogits_bf16 && ld_logits == ld_dlogits
+                                    : !savit_rows_overlap(dlogits, ld_dlogits * ds, C * ds, logits, ld_logits * zs, C * zs, R));
   if (R == 0) return SAVIT_OK;
   DistillParams p{};
   p.z = logits; p.top = teacher_logits; p.at = teacher_index; p.lse = teacher_lse; p.labels = labels; p.weight = row_weight;

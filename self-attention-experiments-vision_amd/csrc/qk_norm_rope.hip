@@ -453,7 +453,8 @@ extern "C" int savit_qk_norm_rope_fwd(const void* qkv, long ld, const float* wq,
   const int q16 = is_bf16 ? 8 : 4;
   SAVIT_CHECK_ARG(ld >= cols && ld_out >= cols && ld % q16 == 0 && ld_out % q16 == 0 && aligned16(qkv) && aligned16(out) && aligned16(table));
   SAVIT_CHECK_ARG(table == nullptr || table_rows >= (positions ? 1 : (rows < N ? rows : N)));
-  SAVIT_CHECK_ARG(out != qkv || ld == ld_out);
+  const int esz = is_bf16 ? 2 : 4;
+  SAVIT_CHECK_ARG(out == qkv ? ld == ld_out : !savit_rows_overlap(out, ld_out * esz, cols * esz, qkv, ld * esz, cols * esz, rows));
   if (rows == 0) return SAVIT_OK;
   QknParams p{};
   p.x = qkv; p.y = out; p.wq = wq; p.wk = wk; p.table = table; p.pos = positions;
@@ -494,7 +495,9 @@ extern "C" int savit_qk_norm_rope_bwd(const void* dqkv, long ld_dqkv, const void
   SAVIT_CHECK_ARG(ld >= cols && ld_out >= cols && ld_dqkv >= cols && ld % q16 == 0 && ld_out % q16 == 0 && ld_dqkv % q16 == 0);
   SAVIT_CHECK_ARG(aligned16(qkv) && aligned16(out) && aligned16(dqkv) && aligned16(table) && ((uintptr_t)workspace % 4) == 0);
   SAVIT_CHECK_ARG(table == nullptr || table_rows >= (positions ? 1 : (rows < N ? rows : N)));
-  SAVIT_CHECK_ARG(out != dqkv || ld_dqkv == ld_out);
+  const int esz = is_bf16 ? 2 : 4;
+  SAVIT_CHECK_ARG(out == dqkv ? ld_dqkv == ld_out : !savit_rows_overlap(out, ld_out * esz, cols * esz, dqkv, ld_dqkv * esz, cols * esz, rows));
+  SAVIT_CHECK_ARG(!savit_rows_overlap(out, ld_out * esz, cols * esz, qkv, ld * esz, (long)(H + Hk) * head_dim * esz, rows));  // (its values are not read)
   if (rows == 0) return SAVIT_OK;
   QknParams p{};
   p.x = qkv; p.g = dqkv; p.y = out; p.wq = wq; p.wk = wk; p.table = table; p.pos = positions;

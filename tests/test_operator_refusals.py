@@ -122,6 +122,17 @@ def test_distill_nothing_to_do(L):
     assert distill(L, R=0) == 0
 
 
+def test_outputs_over_inputs(L):
+    """An output that shares memory with what is still to be read, but for the places that a call names: one row further, one column over, another pitch."""
+    assert qkn(L, out=P + 384) == EINVAL and qkn(L, out=P + 16) == EINVAL and qkn(L, out=P + 384, ldo=200) == EINVAL and qkn(L, ld=384, ldo=384, out=P + 368) == EINVAL
+    assert qkn(L, bwd=True, out=3 * P + 384) == EINVAL and qkn(L, bwd=True, out=P + 384) == EINVAL and qkn(L, bwd=True, out=P - 384) == EINVAL
+    assert qkn(L, bf16=0, out=P + 768) == EINVAL and qkn(L, bf16=0, out=P + 384 * 50) == EINVAL  # (fp32 rows are twice as long)
+    assert attn(L, o=P + 1152 * 99) == EINVAL and attn(L, qkv=3 * P, o=3 * P - 16) == EINVAL
+    assert attn(L, bwd=True, dqkv=P + 1152) == EINVAL and attn(L, bwd=True, do=2 * P + 1152) == EINVAL and attn(L, bwd=True, dbias=P + 208) == EINVAL
+    assert attn(L, bwd=True, dbias=P + 16, ldb=100) == EINVAL
+    assert distill(L, dz=P + 4) == EINVAL and distill(L, dz=P + 400) == EINVAL and distill(L, dz=P + 2, db=1) == EINVAL and distill(L, dz=P + 396, ld=100, ldz=200) == EINVAL
+
+
 def test_wrappers_refuse_cpu_tensors():
     from savit_amd import ops
 

@@ -94,6 +94,33 @@ def test_bias_attention_gradient_of_wide_rows(ops, N):  # noqa: F811
     assert torch.equal(dqkv, want) and torch.equal(db, wb)
 
 
+def test_outputs_beside_their_inputs(ops):  # noqa: F811
+    """Column ranges of one buffer share its rows and no memory: inputs and outputs next to each other."""
+    B, N, H, hd = 2, 50, 2, 32
+    g, qkv, bias, d_o = attention_inputs(ops, B, N, H, hd, 3)
+    w = 3 * H * hd
+    both = torch.zeros(B * N, 2 * w + 16, dtype=torch.bfloat16, device="cuda")
+    both[:, :w] = qkv
+    both_bias = torch.zeros(H * N * 120 + 64, device="cuda")[: H * N * 120].view(H, N, 120)  # (rows of 120, the last one's from column 60 on too)
+    both_bias[:, :, :N] = bias
+    o, lse = ops.bias_attention_fwd(both[:, :w], both_bias[:, :, :N], B, N, H, head_dim=hd)
+    dqkv, db = ops.bias_attention_bwd(both[:, :w], both_bias[:, :, :N], d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd, dqkv=both[:, w + 8:2 * w + 8], dbias=both_bias[:, :, 60:60 + N])
+    want, wb = ops.bias_attention_bwd(qkv, bias, d_o, lse, B, N, H, dq_scale=1.0, head_dim=hd)
+    assert torch.equal(dqkv, want) and torch.equal(db, wb) and torch.equal(both[:, :w], qkv) and bool((both[:, 2 * w + 8:] == 0).all())
+    wq = 1 + randn(g, hd, scale=0.1)
+    y = ops.qk_norm_rope_fwd(both[:, :w], wq, wq, None, N, H, head_dim=hd, out=both[:, w:2 * w])
+    assert torch.equal(y, ops.qk_norm_rope_fwd(qkv, wq, wq, None, N, H, head_dim=hd))
+    dw = torch.zeros(4, hd, device="cuda")
+    dx = ops.qk_norm_rope_bwd(want, both[:, :w], wq, wq, None, dw[0], dw[1], N, H, head_dim=hd, out=both[:, w + 8:2 * w + 8])
+    assert torch.equal(dx, ops.qk_norm_rope_bwd(want, qkv, wq, wq, None, dw[2], dw[3], N, H, head_dim=hd, out=torch.empty_like(want))) and torch.equal(dw[:2], dw[2:])
+    z = torch.zeros(9, 210, device="cuda")
+    z[:, :100] = randn(g, 9, 100)
+    top, at = z[:, :100].topk(5, dim=1)
+    dz = torch.empty(9, 100, device="cuda")
+    loss = ops.distill_xent(z[:, :100].contiguous(), top, at.int(), dlogits=dz)
+    assert torch.equal(ops.distill_xent(z[:, :100], top, at.int(), dlogits=z[:, 101:201]), loss) and torch.equal(z[:, 101:201], dz)
+
+
 # --------------------------------------------------------------------------------------------- query / key norm
 # enough rows that a group of lanes takes four heads in bf16 and two in fp32; numbers of heads that leave a last group fewer
 MANY = [(24001, 5, 3, 64), (11000, 7, 1, 256), (33000, 6, 2, 48), (66001, 9, 9, 16)]
