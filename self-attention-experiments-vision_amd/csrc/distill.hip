@@ -8,8 +8,9 @@
 // Bound by HBM: z is read once and dz written once.  The row stays in registers between the pass that finds the maximum and the sums and the pass
 // that writes the gradient (C 16-byte pieces a thread; what does not fit is read a second time), so there is one block reduction and no re-read.
 // A thread keeps the sums relative to its own maximum and the block joins (maximum, sum) pairs: one barrier instead of two.
-// Measured, with gradient: [2048 x 131072] 260 us (1075 MB, 4.1 TB/s; the loss alone 139; a copy of the bytes takes 216), [1024 x 21843] 39 us (135 MB, 3.5 TB/s), [128 x 1000]
-// 7 to 8 us: a launch, and the 64-bit logarithms and exponentials of the pairs one after the other.  What is left above the copy: a row's loads do not overlap the stores of the row before it in the same registers, and the exponentials (10 %).
+// Measured, with gradient: [2048 x 131072] 255 us (1075 MB, 4.2 TB/s; with the sum of the logits 276; the loss alone 139; a copy of the bytes takes 216),
+// [1024 x 21843] 40 us with that sum (135 MB, 3.4 TB/s), [128 x 1000] 8 us: a launch, and the 64-bit logarithms and exponentials of the pairs one after the
+// other.  What is left above the copy: a row's loads do not overlap the stores of the row before it in the same registers, and the exponentials (10 %).
 // Exponentials are v_exp_f32 on (z - max) * (log2 e / T), per-thread sums fp32; everything that exists once a row - the pairs, the
 // normalisers, the sum of the logits, the loss - is in 64 bits: a divergence near zero is the difference of numbers a hundred times its size.
 // The gradient is written for every class as if no pair named it, then the at most K + 1 classes with a pair or the label are written again.
