@@ -17,7 +17,7 @@
 // delta, sums and dbias are fp32.
 //
 // What bounds it: at [128 x 12 x 197], heads of 64, the bytes take 31 us forward (59 measured) and 55 backward (107 dQ and dbias, 104 dK and dV), the
-// products 19 and 44: with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
+// products 20 and 50 (the low parts counted): with 2 to 3 waves a SIMD it is the chain LDS read - product - exponential - product of a tile, not one of the pipes, that the time
 // goes into.  One segment or long rows come nearer: [2048 x 4 x 49], heads of 32, 26 us forward (bytes 21), 33 dK and dV (31 from memory; some of it is
 // still in the caches), 37 dQ and dbias.
 //
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * W, W == 2 ? 2 : 3) void bias_attn_dkv_kernel(c
   constexpr int T = Seg::SEG / 16;
   __shared__ __attribute__((aligned(16))) char smem[(ONE ? 2 : 4) * Seg::IMG];
   constexpr int SL = (3 * Seg::SEG + 64 * W - 1) / (64 * W);
-  __shared__ float stats[ONE ? 1 : 2][64 * W * SL];  // of the two buffers: SEG of each of the three statistics (and what the other threads write)
+  __shared__ __attribute__((aligned(16))) float stats[ONE ? 1 : 2][64 * W * SL];  // of the two buffers: SEG of each of the three statistics (and what the other threads write)
   const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, b, blk;
